@@ -79,6 +79,68 @@ GTM_API int gtm_attention_decode_rows(uint32_t q_heads, uint32_t kv_heads, uint3
                                       const uint32_t* positions, float* ctx_dev, void* workspace_dev,
                                       size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * One-byte ring KV caches for serving many sequences (no counterpart in the reference, whose
+ * caches are fp32): written in the pass that norms and rotates a step's queries and keys, read
+ * back, and attended with one prefix shared by all rows of a step.
+ *
+ * A vector is head_dim values of one position and kv head, held as head_dim one-byte codes and
+ * one fp32 scale; a value is code * scale. With M = 127 (GTM_KV_INT8: codes -127..127) or 448
+ * (GTM_KV_E4M3: 8-bit floats with 4 exponent and 3 fraction bits, no infinity), scale =
+ * fp32(max(max|y| / M, 2^-100)) and code = y / scale rounded to nearest, ties to even. A vector
+ * holding an infinity or NaN has the scale NaN and codes 0, and reads back as NaN.
+ * Position t of a sequence is ring row t % capacity, as in the fp32 caches.
+ * ------------------------------------------------------------------------------------- */
+enum { GTM_KV_INT8 = 0, GTM_KV_E4M3 = 1 };
+
+typedef struct GtmKvCache {
+    void* k_dev;                 /* codes [num_seqs][capacity][kv_heads][head_dim], 16-byte aligned */
+    void* v_dev;
+    float* k_scale_dev;          /* [num_seqs][kv_heads][capacity]                                  */
+    float* v_scale_dev;          /* attention takes scales in [2^-100, 2^20] (and NaN)              */
+    uint32_t format;             /* GTM_KV_*                                                        */
+    uint32_t num_seqs, capacity, kv_heads, head_dim;   /* head_dim 128, 256 or 512                  */
+    uint32_t reserved;           /* 0                                                               */
+} GtmKvCache;
+
+/* QKVEpilogue of n rows' queries, keys and values in one launch, keys and values going into the
+ * cache: row i (n <= 512, i-th row of q_dev, k_dev and v_dev, whose rows are *_stride floats
+ * apart) belongs to sequence seqs[i] at positions[i] (HOST arrays, as in the *_rows entries).
+ *   q: RMS norm per head with weight q_w_dev (bf16, NULL = none), rotation -> q_out_dev
+ *      [n][q_heads * head_dim] (q_out_dev may be q_dev where q_stride is q_heads * head_dim)
+ *   k: RMS norm with k_w_dev, rotation -> cache;   v: RMS norm without a weight -> cache
+ * v_dev may be k_dev. The rotation is NeoX over the first rotated_pairs pairs, angle position *
+ * theta^(-2i / head_dim). Norms, angles and the codes' rounding are in 64 bits, each result
+ * rounded once, so codes do not depend on the order of a sum and far positions keep their angles
+ * (gtm_qkv_epilogue forms both in fp32, as the reference does). Two rows with the same ring row
+ * are refused. */
+GTM_API int gtm_qkv_cache_rows(const GtmKvCache* cache, uint32_t q_heads, uint32_t n, const float* q_dev,
+                               const float* k_dev, const float* v_dev, uint64_t q_stride, uint64_t k_stride,
+                               uint64_t v_stride, const uint16_t* q_w_dev, const uint16_t* k_w_dev, float eps,
+                               uint32_t rotated_pairs, float theta, const uint32_t* positions, const uint32_t* seqs,
+                               float* q_out_dev, void* stream);
+/* Positions [first, first + count) of sequence `seq` as fp32 into k_out_dev and v_out_dev
+ * [count][kv_heads * head_dim] (either may be NULL); count <= capacity. */
+GTM_API int gtm_kv_read(const GtmKvCache* cache, uint32_t seq, uint32_t first, uint32_t count, float* k_out_dev,
+                        float* v_out_dev, void* stream);
+/* Workspace of gtm_attention_kv_rows for at most n rows (0 for unsupported shapes); no
+ * initialisation. A workspace serves one stream at a time. */
+GTM_API size_t gtm_attention_kv_workspace_bytes(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t n);
+/* Attention of n rows (n <= 512) at positions[i] of sequences seqs[i] (HOST arrays): row i attends
+ * [first, positions[i]] with first = max(0, positions[i] + 1 - window) (window 0 = all), scores
+ * q.k with scale 1.0, softmax, weighted V into ctx_dev row i. Positions below prefix_len are read
+ * from sequence prefix_seq of `prefix` (row t % its capacity), the others from sequence seqs[i] of
+ * `cache`; the prefix's tiles are read and multiplied once for all rows. prefix_len 0: no prefix
+ * (`prefix` may be NULL). Rows of one sequence's prompt are attended causally by giving that
+ * sequence's own cache as the prefix, with prefix_len one past the last row's position.
+ * `prefix` has the cache's format, kv_heads and head_dim. A row's span must fit the rings: its
+ * own positions within capacity, and prefix_len - first within the prefix's. q_heads a multiple of
+ * kv_heads, at most 8 query heads per kv head. q_dev and ctx_dev [n][q_heads * head_dim]. */
+GTM_API int gtm_attention_kv_rows(const GtmKvCache* cache, const GtmKvCache* prefix, uint32_t prefix_seq,
+                                  uint32_t prefix_len, uint32_t q_heads, uint32_t n, uint32_t window,
+                                  const float* q_dev, const uint32_t* seqs, const uint32_t* positions, float* ctx_dev,
+                                  void* workspace_dev, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

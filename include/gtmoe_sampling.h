@@ -80,6 +80,39 @@ GTM_API int gtm_sample_token(const float* logits_dev, uint32_t vocab, const GtmS
                              uint32_t* token_dev, uint32_t* status_dev, void* workspace_dev, size_t workspace_bytes,
                              void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * One token for each row of a batch, from given uniforms (no counterpart in the reference, which
+ * samples one sequence per call). Row i's logits are at logits_dev + i * row_stride.
+ *
+ * Ids are ranked by logit, ties to the lower id; p = softmax of the row at temperature 1. Kept are
+ * the first m ids, m the least of
+ *   top_p < 1: the shortest run with a sum of p of at least top_p (the reference's nucleus rule),
+ *   min_p > 0: the ids with p >= min_p * (the largest p),
+ *   top_k > 0: top_k,
+ * and at least 1. The token is the lowest id whose running sum of exp((l - max) / temperature)
+ * over the kept ids in id order exceeds u times their whole sum; temperature 0 takes the first
+ * id. All cuts see the full distribution (no shortlist: top_k is not bounded by 256). Weights are
+ * formed in 64 bits and summed as integers, so a row's token depends neither on the other rows
+ * nor on the order of a sum. A logit of NaN counts as -infinity. A row whose largest logit is
+ * infinite has no token: 0xFFFFFFFF, kept 0, logprob NaN.
+ * ------------------------------------------------------------------------------------- */
+typedef struct GtmSamplingRow {
+    float temperature;          /* >= 0; 0 = greedy                */
+    float top_p;                /* (0, 1]; 1 = no nucleus cut      */
+    float min_p;                /* [0, 1]; 0 = no min-p cut        */
+    int32_t top_k;              /* >= 0; 0 = no top-k cut          */
+} GtmSamplingRow;
+
+#define GTM_SAMPLE_MAX_ROWS 512
+
+/* rows: n <= 512 HOST structs, checked on the host and passed by value. uniform_dev: n doubles in
+ * [0, 1) on the device (others are clamped into it, NaN to 0); read for rows with a temperature.
+ * token_dev: n uint32. kept_dev (m) and logprob_dev (natural logarithm of the token's p) may be
+ * NULL. Asynchronous on `stream`; no workspace. */
+GTM_API int gtm_sample_rows(const float* logits_dev, uint32_t n, uint32_t vocab, uint64_t row_stride,
+                            const GtmSamplingRow* rows, const double* uniform_dev, uint32_t* token_dev,
+                            uint32_t* kept_dev, float* logprob_dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

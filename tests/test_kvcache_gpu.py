@@ -1,0 +1,480 @@
+"""One-byte ring KV caches on the device (include/gtmoe_attention.h): writing, reading back and
+attending, against plain 64-bit numpy forms.
+
+Bars. Codes and scales: equal (both sides form them in 64 bits, where a value is within ~1e-15 of a
+rounding border with a chance of ~1e-13). Queries: half an fp32 step, 2^-24 relative, plus the
+64-bit forms' 1e-12. Reads: one fp32 product of an exact code, half a step. Attention, fp32 sums
+against 64 bits: a score of head_dim products is summed in at most 64 dependent steps of one fp32
+rounding (2^-23 of S = sum |q k|, truncated), so it is off by at most ds = 64 * 2^-23 * S; exp turns
+that into a relative error of the weights, so an output is off by at most 2 (ds + 2^-20) times the
+largest |v| attended, 2^-20 covering the weights' and outputs' own sums. Roundings average out over
+a whole output, whose 2-norm is held to 2e-5 (eight times 2^-24 of S ~ 40).
+"""
+from __future__ import annotations
+
+import os
+import sys
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path[:0] = [ROOT, os.path.join(ROOT, "turbo-winfare_b200")]
+
+pytestmark = pytest.mark.gpu
+
+MOST = {"int8": 127.0, "e4m3": 448.0}
+
+
+# ---- plain forms --------------------------------------------------------------------------------
+
+def e4m3_table():
+    v = np.zeros(256)
+    for b in range(256):
+        e, m = (b >> 3) & 15, b & 7
+        v[b] = (m * 2.0 ** -9 if e == 0 else (8 + m) * 2.0 ** (e - 10)) * (-1 if b & 128 else 1)
+    return v
+
+
+E4M3 = e4m3_table()
+
+
+def code_values(codes, fmt):
+    """Raw bytes to the values they stand for."""
+    return codes.view(np.int8).astype(np.float64) if fmt == "int8" else E4M3[codes.view(np.uint8)]
+
+
+def to_code(u, fmt):
+    """The nearest code's value; ties to the even code."""
+    if fmt == "int8":
+        return np.clip(np.rint(u), -127, 127)
+    pos = E4M3[:127]   # 0 .. 448
+    a = np.minimum(np.abs(u), 448.0)
+    hi = np.clip(np.searchsorted(pos, a), 1, 126)
+    lo = hi - 1
+    up = (a - pos[lo] > pos[hi] - a) | ((a - pos[lo] == pos[hi] - a) & (hi % 2 == 0))
+    return np.copysign(np.where(up, pos[hi], pos[lo]), u)
+
+
+def norm_rotate(x, w, eps, pos, pairs, theta):
+    """x [n][heads][hd]; pos [n], or None for values."""
+    hd = x.shape[-1]
+    y = x / np.sqrt((x * x).mean(-1, keepdims=True) + float(np.float32(eps)))
+    if w is not None:
+        y = y * w
+    if pos is not None and pairs:
+        a = pos.astype(np.float64)[:, None] * theta ** (-2.0 * np.arange(pairs) / hd)
+        c, s = np.cos(a)[:, None], np.sin(a)[:, None]
+        y0, y1 = y[..., :pairs].copy(), y[..., hd // 2:hd // 2 + pairs].copy()
+        y[..., :pairs], y[..., hd // 2:hd // 2 + pairs] = y0 * c - y1 * s, y0 * s + y1 * c
+    return y
+
+
+def quantise(y, fmt):
+    s = np.maximum(np.abs(y).max(-1) / MOST[fmt], 2.0 ** -100).astype(np.float32)
+    return to_code(y / s.astype(np.float64)[..., None], fmt), s
+
+
+def raw(t):
+    import torch
+    return t.view(torch.uint8).cpu().numpy()
+
+
+def values(cache, which):
+    """A cache's values [num_seqs][capacity][kv_heads][hd] in 64 bits."""
+    codes = code_values(raw(getattr(cache, which)), cache.fmt)
+    return codes * getattr(cache, which + "_scale").cpu().numpy().astype(np.float64).transpose(0, 2, 1)[..., None]
+
+
+def fill(cache, seed, spread=1.0):
+    """Quantised normal vectors in every ring row."""
+    import torch
+    g = torch.Generator().manual_seed(seed)
+    shape = tuple(cache.k.shape)
+    for name in ("k", "v"):
+        x = torch.randn(shape, generator=g).numpy().astype(np.float64)
+        if spread != 1.0:
+            x *= spread ** torch.randn(shape[:3] + (1,), generator=g).numpy()
+        codes, s = quantise(x, cache.fmt)
+        if cache.fmt == "int8":
+            b = codes.astype(np.int8).view(np.uint8)
+        else:
+            b = torch.from_numpy(codes).float().to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+        getattr(cache, name).view(torch.uint8).copy_(torch.from_numpy(b.copy()))
+        getattr(cache, name + "_scale").copy_(torch.from_numpy(s.transpose(0, 2, 1).copy()))
+
+
+def attend(q, cache, seqs, pos, window, prefix, pseq, plen):
+    """Row by row in 64 bits: (ctx, largest allowed error of each row)."""
+    n = q.shape[0]
+    KV, hd = cache.kv_heads, cache.head_dim
+    q = q.reshape(n, KV, -1, hd)
+    own = {w: values(cache, w) for w in "kv"}
+    pre = {w: values(prefix, w)[pseq] for w in "kv"} if plen else None
+    ctx, tol = np.zeros(q.shape), np.zeros(n)
+    for i in range(n):
+        first = max(0, pos[i] + 1 - window) if window else 0
+        t = np.arange(first, pos[i] + 1)
+        kv = []
+        for w in "kv":
+            parts = []
+            if plen and (t < plen).any():
+                parts.append(pre[w][t[t < plen] % prefix.capacity])
+            if (t >= plen).any():
+                parts.append(own[w][seqs[i]][t[t >= plen] % cache.capacity])
+            kv.append(np.concatenate(parts))
+        k, v = kv
+        s = np.einsum("hgd,thd->hgt", q[i], k)
+        p = np.exp(s - s.max(-1, keepdims=True))
+        ctx[i] = np.einsum("hgt,thd->hgd", p / p.sum(-1, keepdims=True), v)
+        S = np.einsum("hgd,thd->hgt", np.abs(q[i]), np.abs(k)).max()
+        tol[i] = 2 * (64 * 2.0 ** -23 * S + 2.0 ** -20) * np.abs(v).max()
+    return ctx.reshape(n, -1), tol
+
+
+def run_attention(cache, q, seqs, pos, window=0, prefix=None, pseq=0, plen=0, stream=None, op=None):
+    import torch
+    from gtmoe.kvcache import KvAttention
+    H = q.shape[1] // cache.head_dim
+    op = op or KvAttention(H, cache.kv_heads, cache.head_dim, max(1, q.shape[0]))
+    ctx = torch.full((q.shape[0], q.shape[1]), 777.0, device="cuda")
+    op(q, cache, seqs, pos, ctx, window=window, prefix=prefix, prefix_seq=pseq, prefix_len=plen, stream=stream)
+    return ctx
+
+
+def check_attention(cache, q, seqs, pos, window=0, prefix=None, pseq=0, plen=0):
+    got = run_attention(cache, q, seqs, pos, window, prefix, pseq, plen).cpu().numpy().astype(np.float64)
+    want, tol = attend(q.cpu().numpy().astype(np.float64), cache, seqs, pos, window, prefix, pseq, plen)
+    off = np.abs(got - want).max(1)
+    assert (off <= tol).all(), (off / tol).max()
+    rel = np.linalg.norm(got - want) / np.linalg.norm(want)
+    assert rel <= 2e-5, rel
+
+
+def queries(n, H, hd, seed=5):
+    import torch
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(n, H * hd, generator=g) * (3.0 / hd ** 0.5)).cuda()
+
+
+# ---- writing ------------------------------------------------------------------------------------
+
+WRITES = [  # n, q_heads, kv_heads, hd, pairs, theta, positions, seqs, capacity, v is k
+    (1, 16, 8, 256, 128, 1e4, [0], [0], 4, False),
+    (1, 16, 2, 512, 64, 1e6, [131071], [2], 100, True),
+    (7, 3, 3, 128, 64, 1e4, [5, 6, 7, 8, 9, 10, 11], [1] * 7, 9, False),
+    (33, 21, 7, 512, 0, 1e4, list(range(0, 330, 10)), [i % 3 for i in range(33)], 400, False),
+    (64, 8, 1, 256, 7, 1e6, list(range(1000000, 1000064)), [0] * 64, 64, False),
+    (512, 4, 2, 128, 33, 5e5, list(range(3000, 3512)), [0] * 512, 600, True),
+]
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("case", WRITES)
+def test_write(case, fmt):
+    import torch
+    from gtmoe.kvcache import KvCache
+    n, H, KV, hd, pairs, theta, pos, seqs, cap, shared = case
+    g = torch.Generator().manual_seed(n)
+    q, k, v = (torch.randn(n, heads * hd, generator=g) * m for heads, m in ((H, 2.0), (KV, 0.3), (KV, 30.0)))
+    v = k if shared else v
+    q_w, k_w = ((1 + 0.2 * torch.randn(hd, generator=g)).to(torch.bfloat16) for _ in range(2))
+    cache = KvCache(3, cap, KV, hd, fmt)
+    fill(cache, 1)
+    before = {x: raw(getattr(cache, x)).copy() for x in ("k", "v", "k_scale", "v_scale")}
+    out = torch.zeros(n, H * hd, device="cuda")
+    kd = k.cuda()
+    cache.write(q.cuda(), kd, kd if shared else v.cuda(), out, pos, seqs, q_w=q_w.cuda(), k_w=k_w.cuda(), eps=1e-6,
+                rotated_pairs=pairs, theta=theta)
+    p = np.array(pos)
+    want = norm_rotate(q.double().numpy().reshape(n, H, hd), q_w.double().numpy(), 1e-6, p, pairs, theta).reshape(n, -1)
+    got = out.cpu().double().numpy()
+    assert (np.abs(got - want) <= 2.0 ** -24 * np.abs(want) + 1e-12).all()
+    slots = p % cap
+    for name, x, w, ps in (("k", k, k_w.double().numpy(), p), ("v", v, None, None)):
+        y = norm_rotate(x.double().numpy().reshape(n, KV, hd), w, 1e-6, ps, pairs, theta)
+        codes, s = quantise(y, fmt)
+        r, rs = raw(getattr(cache, name)), getattr(cache, name + "_scale").cpu().numpy()
+        assert np.array_equal(rs[seqs, :, slots], s)
+        assert np.array_equal(code_values(r[seqs, slots], fmt), codes)
+        # every other ring row stays as it was
+        r[seqs, slots] = before[name][seqs, slots]
+        assert np.array_equal(r, before[name])
+        rs[seqs, :, slots] = before[name + "_scale"].view(np.float32).reshape(rs.shape)[seqs, :, slots]
+        assert np.array_equal(rs, before[name + "_scale"].view(np.float32).reshape(rs.shape))
+
+
+def test_write_strided_unaligned_and_in_place():
+    import torch
+    from gtmoe.kvcache import KvCache
+    n, H, KV, hd = 5, 4, 2, 128
+    g = torch.Generator().manual_seed(2)
+    flat = torch.randn(n * 1100 + 3, generator=g).cuda()
+    rows = flat[1:1 + n * 1100].view(n, 1100)          # one packed projection, 4-byte aligned
+    q, k, v = rows[:, :512], rows[:, 512:768], rows[:, 768:1024]
+    pos, seqs = [9, 8, 7, 6, 5], [0, 0, 1, 1, 0]
+    a, b = KvCache(2, 16, KV, hd), KvCache(2, 16, KV, hd)
+    oa = torch.zeros(n, H * hd, device="cuda")
+    a.write(q, k, v, oa, pos, seqs, rotated_pairs=64)
+    ob = q.contiguous()
+    b.write(ob, k.contiguous(), v.contiguous(), ob, pos, seqs, rotated_pairs=64)
+    assert torch.equal(oa, ob)
+    for x in ("k", "v", "k_scale", "v_scale"):
+        assert torch.equal(getattr(a, x), getattr(b, x))
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_write_zeros_ties_and_nonfinite(fmt):
+    import torch
+    from gtmoe.kvcache import KvCache
+    hd, cap = 128, 8
+    c = KvCache(1, cap, 1, hd, fmt)
+    x = torch.zeros(4, hd)
+    x[1, 3] = float("nan")
+    x[2, 100] = float("-inf")
+    x[3] = torch.arange(hd) - 64.0   # every half step and both ends
+    v = x.clone()
+    out = torch.zeros(4, hd, device="cuda")
+    c.write(torch.ones(4, hd).cuda(), x.cuda(), v.cuda(), out, [0, 1, 2, 3], [0] * 4, eps=1.0)
+    k, kv = c.read(0, 0, 4)
+    for got in (k.cpu().numpy(), kv.cpu().numpy()):
+        assert (got[0] == 0).all() and np.isnan(got[1]).all() and np.isnan(got[2]).all()
+        y = norm_rotate(x[3].double().numpy()[None, None], None, 1.0, None, 0, 1e4)[0, 0]
+        codes, s = quantise(y, fmt)
+        assert np.array_equal(got[3], (codes * s).astype(np.float32))
+    assert c.k_scale[0, 0, 0].item() == 2.0 ** -100 and not raw(c.k)[0, 1:3].any()
+
+
+# ---- reading ------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("hd,KV,cap,first,count", [(128, 1, 1, 0, 1), (256, 3, 37, 30, 37), (512, 2, 1000, 4294967000, 296),
+                                                   (128, 5, 64, 63, 2)])
+def test_read(fmt, hd, KV, cap, first, count):
+    import torch
+    from gtmoe.kvcache import KvCache
+    c = KvCache(2, cap, KV, hd, fmt)
+    fill(c, 3)
+    k, v = c.read(1, first, count)
+    at = np.arange(first, first + count) % cap
+    for got, name in ((k, "k"), (v, "v")):
+        want = values(c, name)[1][at].reshape(count, -1)
+        assert np.array_equal(got.cpu().numpy(), want.astype(np.float32))   # one product, rounded once
+    only = torch.full_like(v, 5.0)
+    assert c.read(1, first, count, None, only)[0] is None and torch.equal(only, v)
+    only = torch.full_like(k, 5.0)
+    c.read(1, first, count, only, None)
+    assert torch.equal(only, k)
+
+
+# ---- attention ----------------------------------------------------------------------------------
+
+ATTENDS = [  # n, q_heads, kv_heads, hd, window, prefix, prefix capacity, own lengths
+    (1, 16, 8, 256, 0, 0, 0, [1]),
+    (1, 16, 2, 512, 0, 0, 0, [1000]),
+    (3, 4, 4, 128, 0, 0, 0, [1, 2, 129]),
+    (5, 21, 7, 256, 50, 0, 0, [1, 49, 50, 51, 333]),
+    (2, 24, 3, 512, 0, 1, 1, [1, 70]),
+    (9, 16, 2, 512, 0, 700, 700, [1, 2, 3, 63, 64, 65, 127, 128, 400]),
+    (40, 16, 8, 256, 100, 300, 200, list(range(1, 121, 3))),
+    (33, 8, 1, 128, 0, 1025, 2000, [5] * 33),
+    (70, 6, 3, 256, 0, 130, 130, [(i * 37) % 90 + 1 for i in range(70)]),
+    (64, 16, 2, 512, 64, 4000, 64, [1 + i for i in range(64)]),
+    (20, 5, 1, 512, 0, 257, 257, [3] * 20),
+]
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("case", ATTENDS)
+def test_attention(case, fmt):
+    from gtmoe.kvcache import KvCache
+    n, H, KV, hd, window, P, pcap, lens = case
+    cap = max(min(m, window) if window else m for m in lens) + 3
+    cache = KvCache(n, cap, KV, hd, fmt)
+    fill(cache, 11)
+    prefix = None
+    if P:
+        prefix = KvCache(2, pcap, KV, hd, fmt)
+        fill(prefix, 12)
+    seqs = [(i * 7 + 3) % n if n % 7 else i for i in range(n)]
+    check_attention(cache, queries(n, H, hd), seqs, [P + m - 1 for m in lens], window, prefix, 1, P)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("n,H,KV,hd,start,window", [(2, 16, 8, 256, 0, 0), (130, 16, 2, 512, 77, 0), (200, 6, 2, 128, 1000, 333),
+                                                    (300, 8, 4, 256, 3, 17), (512, 2, 1, 128, 0, 0)])
+def test_attention_causal_rows_of_one_sequence(fmt, n, H, KV, hd, start, window):
+    from gtmoe.kvcache import KvCache
+    cap = start + n if not window else min(start + n, window + n + 5)
+    cache = KvCache(2, cap, KV, hd, fmt)
+    fill(cache, 21)
+    check_attention(cache, queries(n, H, hd), [1] * n, list(range(start, start + n)), window, cache, 1, start + n)
+
+
+def test_attention_rows_inside_a_prefix_and_beyond():
+    from gtmoe.kvcache import KvCache
+    cache, prefix = KvCache(4, 40, 2, 256), KvCache(1, 90, 2, 256)
+    fill(cache, 31)
+    fill(prefix, 32)
+    check_attention(cache, queries(4, 16, 256), [0, 1, 2, 3], [0, 44, 89, 129], 0, prefix, 0, 90)
+
+
+@pytest.mark.parametrize("spread", [1e3, 1e-3])
+def test_attention_uneven_scales(spread):
+    # vectors whose scales differ by many powers of ten: the weighted sum keeps the large ones' precision
+    from gtmoe.kvcache import KvCache
+    cache = KvCache(2, 200, 2, 128)
+    fill(cache, 41)
+    f = np.float32(spread) ** np.random.default_rng(1).uniform(-2, 2, tuple(cache.v_scale.shape)).astype(np.float32)
+    import torch
+    cache.v_scale.mul_(torch.from_numpy(f).cuda())
+    check_attention(cache, queries(2, 8, 128), [1, 0], [199, 100])
+    prefix = cache
+    check_attention(cache, queries(30, 8, 128), [0] * 30, [150] * 30, 0, prefix, 1, 151)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("many", [1, 40])
+def test_masked_rows_of_a_cache_do_not_matter(fmt, many):
+    import torch
+    from gtmoe.kvcache import KvCache
+    P, cap = 100, 64
+    cache, prefix = KvCache(2, cap, 2, 256, fmt), KvCache(1, 128, 2, 256, fmt)
+    fill(cache, 51)
+    fill(prefix, 52)
+    pos = [P + 20] * many
+    q = queries(many, 16, 256)
+    seqs = [1] * many
+    clean = run_attention(cache, q, seqs, pos, 90, prefix, 0, P)
+    # everything outside [pos + 1 - window, pos]: NaN and infinite scales, codes of all ones
+    first = P + 20 + 1 - 90
+    for c, lo, hi, s in ((prefix, first, P, 0), (cache, P, P + 21, 1)):
+        live = np.zeros(c.capacity, bool)
+        live[np.arange(lo, hi) % c.capacity] = True
+        dead = torch.from_numpy(~live).cuda()
+        for x in ("k", "v"):
+            getattr(c, x).view(torch.uint8)[s][dead] = 0x7F
+            sc = getattr(c, x + "_scale")[s]
+            sc[:, dead] = float("nan") if x == "k" else float("inf")
+    assert torch.equal(run_attention(cache, q, seqs, pos, 90, prefix, 0, P), clean)
+
+
+def test_nan_vectors_reach_the_rows_that_attend_them_only():
+    import torch
+    from gtmoe.kvcache import KvCache
+    cache = KvCache(1, 64, 2, 128)
+    fill(cache, 61)
+    q = queries(12, 4, 128)
+    pos = list(range(20, 32))
+    clean = run_attention(cache, q, [0] * 12, pos, 0, cache, 0, 64)
+    cache.v_scale[0, 1, 25] = float("nan")   # kv head 1, position 25
+    got = run_attention(cache, q, [0] * 12, pos, 0, cache, 0, 64).view(12, 4, 128)
+    clean = clean.view(12, 4, 128)
+    assert torch.equal(got[:, :2], clean[:, :2]) and torch.equal(got[:5], clean[:5])
+    assert torch.isnan(got[5:, 2:]).all()
+
+
+def test_rows_behind_the_last_stay_and_repeats_are_equal():
+    import torch
+    from gtmoe.kvcache import KvAttention, KvCache
+    cache = KvCache(4, 300, 2, 512)
+    fill(cache, 71)
+    op = KvAttention(16, 2, 512, 8)
+    ctx = torch.full((8, 16 * 512), 3.5, device="cuda")
+    q = queries(8, 16, 512)
+    op(q[:3], cache, [2, 2, 0], [299, 299, 10], ctx[:3], prefix=cache, prefix_seq=1, prefix_len=5)
+    assert (ctx[3:] == 3.5).all()
+    again = torch.empty_like(ctx[:3])
+    op(q[:3], cache, [2, 2, 0], [299, 299, 10], again, prefix=cache, prefix_seq=1, prefix_len=5)
+    assert torch.equal(again, ctx[:3])
+
+
+def test_streams_and_graphs():
+    import torch
+    from gtmoe.kvcache import KvAttention, KvCache
+    cache = KvCache(2, 128, 2, 256)
+    fill(cache, 81)
+    H, n = 8, 6
+    q, kv = queries(n, H, 256, 1), queries(n, 4, 256, 2)
+    k, v = kv[:, :512].contiguous(), kv[:, 512:].contiguous()
+    pos, seqs = [40, 41, 42, 43, 44, 45], [1] * n
+    op = KvAttention(H, 2, 256, n)
+    qo, ctx = torch.empty_like(q), torch.empty_like(q)
+
+    def step(stream=None):
+        cache.write(q, k, v, qo, pos, seqs, rotated_pairs=128, stream=stream)
+        op(qo, cache, seqs, pos, ctx, prefix=cache, prefix_seq=1, prefix_len=46, stream=stream)
+
+    step()
+    want = ctx.clone()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    ctx.zero_()
+    s.wait_stream(torch.cuda.current_stream())
+    step(s)
+    s.synchronize()
+    assert torch.equal(ctx, want)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    q2 = q.flip(0).contiguous()
+    q.copy_(q2)
+    g.replay()
+    torch.cuda.synchronize()
+    got = ctx.clone()
+    step()
+    assert torch.equal(got, ctx) and not torch.equal(got, want)
+
+
+def test_a_cache_beyond_4_gib():
+    import torch
+    from gtmoe.kvcache import KvCache
+    cap, seqs = 131072, 34   # 131072 * 1024 bytes a sequence: the last starts at 4.4e9
+    c = KvCache(seqs, cap, 2, 512)
+    n = 64
+    g = torch.Generator().manual_seed(9)
+    k, q = torch.randn(n, 1024, generator=g).cuda(), torch.randn(n, 8 * 512, generator=g).cuda()
+    qo = torch.empty_like(q)
+    pos = list(range(cap - 32, cap + 32))
+    c.write(q, k, k, qo, pos, [seqs - 1] * n, rotated_pairs=64, theta=1e6)
+    got, _ = c.read(seqs - 1, cap - 32, n)
+    small = KvCache(1, 64, 2, 512)
+    small.write(q, k, k, qo, pos, [0] * n, rotated_pairs=64, theta=1e6)
+    want, _ = small.read(0, cap - 32, n)
+    assert torch.equal(got, want) and (c.k[:seqs - 1] == 0).all()
+    a = run_attention(c, qo[:2] * 0.1, [seqs - 1] * 2, pos[-2:], 60)
+    b = run_attention(small, qo[:2] * 0.1, [0] * 2, pos[-2:], 60)
+    assert torch.equal(a, b)
+
+
+def test_a_step_of_write_read_and_attend_together():
+    """Three sequences behind one prompt, written token by token, against fp32 attention in numpy on
+    the values that the cache holds."""
+    import torch
+    from gtmoe.kvcache import KvAttention, KvCache
+    H, KV, hd, P, n = 16, 8, 256, 37, 3
+    prefix, cache = KvCache(1, P, KV, hd), KvCache(n, 20, KV, hd)
+    op = KvAttention(H, KV, hd, P)
+    g = torch.Generator().manual_seed(4)
+
+    def rows(m):
+        return [(torch.randn(m, heads * hd, generator=g)).cuda() for heads in (H, KV, KV)]
+
+    q, k, v = rows(P)
+    qo, ctx = torch.empty_like(q), torch.empty_like(q)
+    prefix.write(q, k, v, qo, range(P), [0] * P, rotated_pairs=128)
+    qo *= 0.2
+    op(qo, prefix, [0] * P, range(P), ctx, prefix=prefix, prefix_len=P)
+    want, tol = attend(qo.cpu().double().numpy(), prefix, [0] * P, list(range(P)), 0, prefix, 0, P)
+    assert (np.abs(ctx.cpu().numpy() - want).max(1) <= tol).all()
+    for step in range(10):
+        q, k, v = rows(n)
+        qo, ctx = torch.empty_like(q), torch.empty_like(q)
+        pos = [P + step] * n
+        cache.write(q, k, v, qo, pos, [2, 0, 1], rotated_pairs=128)
+        qo *= 0.2
+        op(qo, cache, [2, 0, 1], pos, ctx, window=30, prefix=prefix, prefix_len=P)
+    want, tol = attend(qo.cpu().double().numpy(), cache, [2, 0, 1], pos, 30, prefix, 0, P)
+    assert (np.abs(ctx.cpu().numpy() - want).max(1) <= tol).all()
+    kr, _ = cache.read(2, P, 10)
+    assert np.array_equal(kr.cpu().numpy(), values(cache, "k")[2][np.arange(P, P + 10) % 20].reshape(10, -1).astype(np.float32))

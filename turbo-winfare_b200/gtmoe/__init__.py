@@ -103,6 +103,18 @@ class Sampling(C.Structure):
                 ("seed", C.c_uint64)]
 
 
+class KvCacheDesc(C.Structure):
+    """GtmKvCache (include/gtmoe_attention.h)."""
+    _fields_ = [("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("k_scale_dev", C.c_void_p), ("v_scale_dev", C.c_void_p),
+                ("format", C.c_uint32), ("num_seqs", C.c_uint32), ("capacity", C.c_uint32), ("kv_heads", C.c_uint32),
+                ("head_dim", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class SamplingRow(C.Structure):
+    """GtmSamplingRow (include/gtmoe_sampling.h)."""
+    _fields_ = [("temperature", C.c_float), ("top_p", C.c_float), ("min_p", C.c_float), ("top_k", C.c_int32)]
+
+
 _lib = None
 
 # (name, restype, argtypes) for every entry point in include/gtmoe.h, include/gtmoe_synth.h,
@@ -183,6 +195,12 @@ SIGNATURES = {
     "gtm_attention_rows_workspace_bytes": (_SZ, [_U32, _U32, _U32, _U32]),
     "gtm_attention_decode_rows": (_I, [_U32, _U32, _U32, _U32, _U32, _U32, _P, _P, _P, C.POINTER(_U32), _U32,
                                        C.POINTER(_U32), _P, _P, _SZ, _P]),
+    "gtm_qkv_cache_rows": (_I, [C.POINTER(KvCacheDesc), _U32, _U32, _P, _P, _P, _U64, _U64, _U64, _P, _P, _F, _U32, _F,
+                                _P, _P, _P, _P]),
+    "gtm_kv_read": (_I, [C.POINTER(KvCacheDesc), _U32, _U32, _U32, _P, _P, _P]),
+    "gtm_attention_kv_workspace_bytes": (_SZ, [_U32, _U32, _U32, _U32]),
+    "gtm_attention_kv_rows": (_I, [C.POINTER(KvCacheDesc), C.POINTER(KvCacheDesc), _U32, _U32, _U32, _U32, _U32, _P, _P, _P,
+                                   _P, _P, _SZ, _P]),
     "gtm_sampling_validate": (_I, [C.POINTER(Sampling)]),
     "gtm_sampling_splitmix64": (_U64, [_U64]),
     "gtm_sampling_seed_for": (_U64, [C.POINTER(Sampling), _I]),
@@ -190,6 +208,7 @@ SIGNATURES = {
     "gtm_sample_workspace_bytes": (_SZ, [_U32]),
     "gtm_repetition_penalty": (_I, [_P, _U32, _P, _U32, _F, _F, _P, _SZ, _P]),
     "gtm_sample_token": (_I, [_P, _U32, C.POINTER(Sampling), _U64, _P, _P, _P, _SZ, _P]),
+    "gtm_sample_rows": (_I, [_P, _U32, _U32, _U64, C.POINTER(SamplingRow), _P, _P, _P, _P, _P]),
     "gtm_synth_expert_layout": (_I, [_U32, _U32, C.POINTER(_U64), C.POINTER(_U64)]),
     "gtm_synth_resident_layout": (_I, [_U32, _U32, _U32, C.POINTER(_U64), C.POINTER(_U64)]),
     "gtm_synth_experts": (_I, [_U64, _U32, _U32, _U32, _U32, _U32, _P, _P]),

@@ -8,8 +8,9 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
+from typing import NamedTuple
 
-from . import ERR_INVALID, GtmError, Sampling, _stream, check, lib, ptr
+from . import ERR_INVALID, GtmError, Sampling, SamplingRow, _stream, check, lib, ptr
 
 MAX_TOP_K = 256
 DEGENERATE, NEAR_CUT, NEAR_DRAW = 1, 2, 4   # bits of the device status word
@@ -80,3 +81,61 @@ class Sampler:
         check(lib().gtm_sample_token(ptr(logits), self.vocab, C.byref(c), seed, ptr(self.token[0:1]),
                                      ptr(self.token[1:2]), self.ws_ptr, self.ws_bytes, _stream(stream)))
         return self.token
+
+
+# ---- one token for each row of a batch (gtm_sample_rows) ------------------------------------------
+
+@dataclass
+class RowParams:
+    """A row's settings (GtmSamplingRow): temperature 0 = greedy, top_p 1, min_p 0 and top_k 0 = no cut."""
+    temperature: float = 0.0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    top_k: int = 0
+
+
+def sampling_rows(params):
+    """The rows of a call, from RowParams; kept by a caller whose settings do not change."""
+    return (SamplingRow * max(1, len(params)))(*[SamplingRow(p.temperature, p.top_p, p.min_p, p.top_k) for p in params])
+
+
+class RowTokens(NamedTuple):
+    """Views of the sampler's buffers, overwritten by its next call: int32 tokens (-1: the row has none),
+    int32 counts of the ids the cuts kept, fp32 log probabilities."""
+    tokens: object
+    kept: object
+    logprobs: object
+
+
+class RowSampler:
+    """Tokens for up to max_rows rows of logits over a vocabulary of `vocab` ids."""
+
+    def __init__(self, vocab: int, max_rows: int, device: str = "cuda"):
+        import torch
+        self.vocab, self.max_rows = vocab, max_rows
+        self.tokens, self.kept = (torch.zeros(max_rows, dtype=torch.int32, device=device) for _ in range(2))
+        self.logprobs = torch.zeros(max_rows, dtype=torch.float32, device=device)
+
+    def __call__(self, logits, rows, uniforms=None, stream=None) -> RowTokens:
+        """logits: fp32 [n, vocab], rows contiguous but possibly strided; rows: sampling_rows(...) or a
+        list of RowParams, n of them; uniforms: float64 [n] on the device, None where every row is greedy."""
+        import torch
+        n = logits.shape[0]
+        if logits.dim() != 2 or logits.shape[1] != self.vocab or logits.dtype != torch.float32 or logits.stride(1) != 1 or \
+                logits.device != self.tokens.device:
+            raise GtmError(ERR_INVALID, f"logits must be float32 [n, {self.vocab}] on {self.tokens.device} with contiguous rows")
+        if n > self.max_rows:
+            raise GtmError(ERR_INVALID, f"{n} rows for a sampler of {self.max_rows}")
+        if uniforms is not None and (uniforms.dtype != torch.float64 or uniforms.numel() != n or not uniforms.is_contiguous() or
+                                     uniforms.device != logits.device):
+            raise GtmError(ERR_INVALID, f"uniforms must be {n} contiguous float64 values on {logits.device}")
+        if isinstance(rows, (list, tuple)):
+            if len(rows) != n:
+                raise GtmError(ERR_INVALID, f"{len(rows)} settings for {n} rows")
+            rows = sampling_rows(rows)
+        elif len(rows) < n:
+            raise GtmError(ERR_INVALID, f"{len(rows)} settings for {n} rows")
+        stride = self.vocab if n <= 1 else logits.stride(0)
+        check(lib().gtm_sample_rows(ptr(logits), n, self.vocab, stride, rows, ptr(uniforms), ptr(self.tokens), ptr(self.kept),
+                                    ptr(self.logprobs), _stream(stream)))
+        return RowTokens(self.tokens[:n], self.kept[:n], self.logprobs[:n])
