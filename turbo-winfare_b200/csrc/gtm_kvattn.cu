@@ -1,37 +1,37 @@
 // Attention over the one-byte KV caches (include/gtmoe_attention.h).
 //
-// kv_partial: one CTA per (kv head, chunk of positions, row), the row's prefix and own positions
-// taken as one list; online softmax over tiles of 64 positions in fp32; kv_combine merges a row's
-// chunks.
+// softmax(q K^T) V with K = codes * ks and V = codes * vs, one scale per position. Codes are exact
+// in fp16 (int8 directly, e4m3 with its exponent bias moved: the value times 2^-8), so the tensor
+// cores multiply them as they are and only the other operand is split: q and the weights p are
+// carried as an fp16 high and low part (22 bits), two products each, accumulated in fp32. The
+// scales stay outside: a score is multiplied by its position's ks, a weight by its vs.
+//
+// Running softmax in base 2 per query head: with s2 = log2(e) * q.k the stabiliser is m >= max(s2 +
+// log2 vs), so a carried weight p = exp2(s2 - m) * vs is at most about 1 whatever the scales are
+// (fp16 keeps 2^-25 of the largest one), while l = sum of exp2(s2 - m) and the weighted sum O stay
+// in fp32. Masked positions take a weight of exactly 0 by selection, so nothing that a ring row
+// outside a row's span holds reaches a sum. A partial result (m, l, O) is merged by kv_combine.
+//
+// kv_rows: a CTA per (row, kv head, run of positions), for positions that one row attends.
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 #include <algorithm>
 #include <cmath>
 
+#include "gtm_frag.cuh"
 #include "gtm_kvcache.cuh"
 
 namespace gtm {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kTile = 64;
 constexpr uint32_t kMaxGroup = 8;
+constexpr float kLog2e = 1.4426950408889634f;
 
 // One side (prefix or own cache) as the kernels address it.
 struct Side {
     const uint8_t *k, *v;
     const float *ks, *vs;
     uint32_t capacity;
-};
-
-struct AttnArgs {
-    Side own, pre;
-    const float* q;
-    float* part;     // [n][q_heads][splits][head_dim]
-    float2* ml;      // [n][q_heads][splits]: largest score, sum of exp(score - largest)
-    float* ctx;
-    uint32_t q_heads, kv_heads, splits, window, prefix_len;
 };
 
 struct Span {
@@ -50,142 +50,377 @@ __host__ __device__ __forceinline__ Span row_span(uint32_t pos, uint32_t window,
     return s;
 }
 
-template <int FMT>
-__device__ __forceinline__ float2 two_codes(uint32_t two) {
-    if constexpr (FMT == GTM_KV_INT8) {
-        return make_float2(static_cast<float>(static_cast<int8_t>(two & 0xFFu)),
-                           static_cast<float>(static_cast<int8_t>((two >> 8) & 0xFFu)));
-    } else {
-        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xFFFFu), __NV_E4M3);
-        return __half22float2(__half2(h));
-    }
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 
+// Code words (4 codes) as half2 pairs. Int8: 1024 + (code + 128) is the half 0x6400 | byte, minus
+// 1152. E4m3: sign and 7 bits moved to a half's sign, exponent and top mantissa bits: value * 2^-8,
+// exact, subnormals included.
+template <int FMT>
+__device__ __forceinline__ uint32_t bias_codes(uint32_t w) {
+    return FMT == GTM_KV_INT8 ? w ^ 0x80808080u : w;
+}
+__device__ __forceinline__ uint32_t hsub1152(uint32_t h) {
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t e4m3_halves(uint32_t v) {   // codes in bytes 1 and 3
+    return (v & 0x80008000u) | ((v >> 1) & 0x3F803F80u);
+}
+// codes 2i, 2i + 1 of one (biased) word
+template <int FMT, int I>
+__device__ __forceinline__ uint32_t pair_in_word(uint32_t w) {
+    if constexpr (FMT == GTM_KV_INT8) return hsub1152(__byte_perm(w, 0x64646464u, I ? 0x4342 : 0x4140));
+    return e4m3_halves(__byte_perm(w, 0u, I ? 0x3424 : 0x1404));
+}
+// code i of word a (low half) and of word b (high half)
+template <int FMT>
+__device__ __forceinline__ uint32_t pair_of_words(uint32_t a, uint32_t b, int i) {
+    if constexpr (FMT == GTM_KV_INT8) {
+        const uint32_t x = __byte_perm(a, b, i | ((4 + i) << 4));
+        return hsub1152(__byte_perm(x, 0x64646464u, 0x4140));
+    }
+    return e4m3_halves(__byte_perm(a, b, (i << 4) | ((4 + i) << 12)));
+}
+
+// ---- rows over their own positions ----------------------------------------------------------------
+
+struct RowsArgs {
+    Side own, pre;
+    const float* q;
+    float* ctx;
+    float* part;     // [item][kv_heads][group][head_dim]
+    float2* ml;      // [item][kv_heads][group]: m (base 2), l
+    uint32_t q_heads, kv_heads, n, window, prefix_len, chunk;
+    bool list_prefix, direct;   // prefix positions are in the rows' lists; rows of one item write ctx
+};
+struct Starts {
+    uint32_t v[kMaxBatchRows + 1];   // first item of each row, then the number of items
+};
+
+template <int HD>
+struct RowsShape {
+    static constexpr int kWarps = HD == 128 ? 4 : 8;
+    static constexpr int kTile = 16 * kWarps;
+    static constexpr int kDims = HD / kWarps;   // V dims of a warp
+    static constexpr int kD = kDims / 8;        // contiguous V codes of a thread: 8 or 4
+    static constexpr int kChunks = HD / 64;
+};
+
+// A tile: each warp scores 16 positions (A = K: 16 positions x 16 dims; B = q: 16 dims x 8 heads),
+// the CTA agrees on the heads' maxima, and each warp adds all the tile's positions to its share of
+// the dims (A = V^T: 16 dims x 16 positions; B = p). The order of dims and positions inside a
+// product is free, so threads read contiguous codes: 16 of a K vector, kD of a V vector. Codes of
+// the next tile are loaded into the registers that the products have just emptied.
 template <int HD, int FMT>
-__global__ void __launch_bounds__(kThreads) kv_partial(const __grid_constant__ AttnArgs a, const __grid_constant__ RowU32 pos,
-                                                       const __grid_constant__ RowU32 seq) {
-    constexpr int L = HD / 32;   // codes of a vector per lane
-    __shared__ float qs[kMaxGroup * HD];
-    __shared__ float sc[kMaxGroup][kTile];
-    __shared__ float vs_s[kTile], m_s[kMaxGroup], f_s[kMaxGroup], l_s[kMaxGroup];
-    const uint32_t kvh = blockIdx.x, split = blockIdx.y, row = blockIdx.z;
+__global__ void __launch_bounds__(RowsShape<HD>::kWarps * 32, HD == 512 ? 1 : 2)
+    kv_rows(const __grid_constant__ RowsArgs a, const __grid_constant__ Starts starts, const __grid_constant__ RowU32 pos,
+            const __grid_constant__ RowU32 seq) {
+    using S = RowsShape<HD>;
+    constexpr int T = S::kTile, W = S::kWarps, D = S::kD, C = S::kChunks;
+    constexpr int kPad = T + 8;   // halves per head row of P
+    __shared__ uint4 qf_s[C][2][2][32];               // [64-dim chunk][limb][half][lane]: B fragments of q
+    __shared__ __align__(16) __half p_s[2][8][kPad];  // [limb][head][position]
+    __shared__ __align__(16) uint64_t kaddr[2][T], vaddr[2][T];
+    __shared__ float2 sc_s[2][T];                     // ks, vs
+    __shared__ float wmax[W][8], qscale[8], lsum[W][8];
+
+    const uint32_t item = blockIdx.x, kvh = blockIdx.y;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane & 3, oct = lane >> 2;
+    uint32_t row = 0;
+    for (uint32_t step = 256; step; step >>= 1)
+        if (row + step < a.n && starts.v[row + step] <= item) row += step;
+    // rows without positions share their start with the next row: the last row with start <= item is meant
+    const uint32_t items = starts.v[row + 1] - starts.v[row];
     const int grp = static_cast<int>(a.q_heads / a.kv_heads);
-    const Span sp = row_span(pos.v[row], a.window, a.prefix_len);
+    Span sp = row_span(pos.v[row], a.window, a.prefix_len);
+    if (!a.list_prefix) sp.pn = 0;
     const uint32_t total = sp.pn + sp.on;
-    const uint32_t chunk = (total + a.splits - 1) / a.splits;
-    const uint64_t b0 = static_cast<uint64_t>(split) * chunk;
-    const uint32_t j0 = static_cast<uint32_t>(b0 < total ? b0 : total), j1 = min(total, j0 + chunk);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const float* q = a.q + (static_cast<size_t>(row) * a.q_heads + static_cast<size_t>(kvh) * grp) * HD;
-    for (int i = threadIdx.x; i < grp * HD; i += kThreads) qs[i] = q[i];
-    if (threadIdx.x < kMaxGroup) m_s[threadIdx.x] = -INFINITY, l_s[threadIdx.x] = 0.0f;
-    float acc[kMaxGroup][2] = {};
-    // list position j -> the vector's index in its side's codes, and its scale's index
-    auto place = [&](uint32_t j, const Side*& s, size_t& vec, size_t& sca) {
-        const bool pre = j < sp.pn;
-        s = pre ? &a.pre : &a.own;
-        const uint32_t t = pre ? sp.pa + j : sp.oa + (j - sp.pn);
-        const uint32_t slot = t % s->capacity;
-        const size_t sq = pre ? 0 : seq.v[row];
-        vec = ((sq * s->capacity + slot) * a.kv_heads + kvh) * HD;
-        sca = (sq * a.kv_heads + kvh) * s->capacity + slot;
+    const uint32_t j0 = (item - starts.v[row]) * a.chunk, j1 = min(total, j0 + a.chunk);
+    const uint32_t pslot = sp.pn ? sp.pa % a.pre.capacity : 0, oslot = sp.oa % a.own.capacity;
+    const uint64_t own_vec = static_cast<uint64_t>(seq.v[row]) * a.own.capacity * a.kv_heads + kvh;
+    const uint64_t own_sc = (static_cast<uint64_t>(seq.v[row]) * a.kv_heads + kvh) * a.own.capacity;
+
+    // list position j: addresses of its K and V codes, and its scales
+    auto place = [&](uint32_t j, uint64_t& ka, uint64_t& va, float2& s) {
+        const bool p = j < sp.pn;
+        const uint32_t cap = p ? a.pre.capacity : a.own.capacity;
+        uint64_t slot = p ? static_cast<uint64_t>(pslot) + j : static_cast<uint64_t>(oslot) + (j - sp.pn);
+        if (slot >= cap) slot -= cap;
+        const uint64_t vec = ((p ? kvh : own_vec) + slot * a.kv_heads) * HD;
+        const uint64_t sc = (p ? static_cast<uint64_t>(kvh) * cap : own_sc) + slot;
+        ka = reinterpret_cast<uint64_t>((p ? a.pre.k : a.own.k) + vec);
+        va = reinterpret_cast<uint64_t>((p ? a.pre.v : a.own.v) + vec);
+        s = make_float2(__ldg((p ? a.pre.ks : a.own.ks) + sc), __ldg((p ? a.pre.vs : a.own.vs) + sc));
     };
-    for (uint32_t t0 = j0; t0 < j1; t0 += kTile) {
-        const int n = static_cast<int>(min(j1 - t0, static_cast<uint32_t>(kTile)));
-        __syncthreads();
-        for (int j = warp; j < n; j += kThreads / 32) {
-            const Side* s;
-            size_t vec, sca;
-            place(t0 + j, s, vec, sca);
-            const float ks = s->ks[sca];
-            if (lane == 0) vs_s[j] = s->vs[sca];
-            for (int g = 0; g < grp; ++g) {
-                float d = 0.0f;
-#pragma unroll
-                for (int i = 0; i < L / 2; ++i) {
-                    const int c = 2 * lane + 64 * i;
-                    const float2 k = two_codes<FMT>(*reinterpret_cast<const uint16_t*>(s->k + vec + c));
-                    d += qs[g * HD + c] * k.x + qs[g * HD + c + 1] * k.y;
-                }
-                for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-                if (lane == 0) sc[g][j] = d * ks;
-            }
+    // entry tid of tile t: the last position stands in for those past the run (their weight is 0)
+    auto write_places = [&](uint32_t t, float2& s) {
+        if (tid < T) {
+            uint64_t ka, va;
+            place(min(j0 + t * T + tid, j1 - 1), ka, va, s);
+            kaddr[t & 1][tid] = ka, vaddr[t & 1][tid] = va;
         }
-        __syncthreads();
-        if (warp < grp) {
-            float m = m_s[warp];
-            const float old = m;
-            for (int j = lane; j < n; j += 32) m = fmaxf(m, sc[warp][j]);
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            float l = 0.0f;
-            for (int j = lane; j < n; j += 32) {
-                const float e = expf(sc[warp][j] - m);
-                l += e;
-                sc[warp][j] = e * vs_s[j];
-            }
-            for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            if (lane == 0) {
-                const float f = expf(old - m);
-                f_s[warp] = f;
-                l_s[warp] = l_s[warp] * f + l;
-                m_s[warp] = m;
-            }
+    };
+
+    float2 sc_next = make_float2(0.0f, 0.0f);
+    write_places(0, sc_next);
+    if (tid < T) sc_s[0][tid] = sc_next;
+    // q of head h: scaled by a power of two into [1, 2), then high and low fp16 parts
+    for (int h = warp; h < 8; h += W) {
+        const float* src = a.q + (static_cast<size_t>(row) * a.q_heads + static_cast<size_t>(kvh) * grp + h) * HD;
+        float x[HD / 32], top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < HD / 128; ++i) {
+            const float4 v = h < grp ? __ldg(reinterpret_cast<const float4*>(src) + lane + 32 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
         }
-        __syncthreads();
 #pragma unroll
-        for (int g = 0; g < static_cast<int>(kMaxGroup); ++g)
-            if (g < grp) acc[g][0] *= f_s[g], acc[g][1] *= f_s[g];
-        for (int j = 0; j < n; ++j) {
-            const Side* s;
-            size_t vec, sca;
-            place(t0 + j, s, vec, sca);
-            if (2 * threadIdx.x < HD) {
-                const float2 v = two_codes<FMT>(*reinterpret_cast<const uint16_t*>(s->v + vec + 2 * threadIdx.x));
+        for (int i = 0; i < HD / 32; ++i) top = fmaxf(top, fabsf(x[i]));
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int e = top > 0.0f ? max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127)) : 0;
+        const float down = __int_as_float((127 - e) << 23);
+        if (lane == 0) qscale[h] = __int_as_float((127 + e) << 23) * kLog2e * (FMT == GTM_KV_E4M3 ? 256.0f : 1.0f);
 #pragma unroll
-                for (int g = 0; g < static_cast<int>(kMaxGroup); ++g)
-                    if (g < grp) acc[g][0] += sc[g][j] * v.x, acc[g][1] += sc[g][j] * v.y;
+        for (int i = 0; i < HD / 128; ++i) {
+            const int d = 4 * lane + 128 * i;   // four dims of one 16-dim run
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float u = x[4 * i + 2 * j] * down, v = x[4 * i + 2 * j + 1] * down;
+                hi[j] = cvt2(u, v);
+                const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi[j]));
+                lo[j] = cvt2(u - b.x, v - b.y);
             }
+            const int c = d >> 6, t = (d >> 4) & 3, half = (d >> 3) & 1, at = (d >> 2) & 1;
+            reinterpret_cast<uint2*>(&qf_s[c][0][half][h * 4 + t])[at] = make_uint2(hi[0], hi[1]);
+            reinterpret_cast<uint2*>(&qf_s[c][1][half][h * 4 + t])[at] = make_uint2(lo[0], lo[1]);
         }
     }
     __syncthreads();
-    for (int g = 0; g < grp; ++g) {
-        const size_t at = (static_cast<size_t>(row) * a.q_heads + static_cast<size_t>(kvh) * grp + g) * a.splits + split;
-        if (threadIdx.x == 0) a.ml[at] = make_float2(m_s[g], l_s[g]);
-        if (2 * threadIdx.x < HD)
-            *reinterpret_cast<float2*>(a.part + at * HD + 2 * threadIdx.x) = make_float2(acc[g][0], acc[g][1]);
+
+    uint4 kr[2][C];
+    uint32_t vr[T / 16][4][D / 4];
+    auto load_k = [&](uint32_t t) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const uint4* p = reinterpret_cast<const uint4*>(kaddr[t & 1][warp * 16 + oct + 8 * r]) + quad;
+#pragma unroll
+            for (int c = 0; c < C; ++c) kr[r][c] = __ldg(p + 4 * c);
+        }
+    };
+    const uint64_t vdim = static_cast<uint64_t>(warp * S::kDims + oct * D);
+    auto load_v = [&](uint32_t t, int ks) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint64_t p = vaddr[t & 1][16 * ks + 4 * quad + r] + vdim;
+            if constexpr (D == 8) {
+                const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+                vr[ks][r][0] = w.x, vr[ks][r][1] = w.y;
+            } else {
+                vr[ks][r][0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+            }
+        }
+    };
+    const uint32_t tiles = (j1 - j0 + T - 1) / T;
+    load_k(0);
+#pragma unroll
+    for (int ks = 0; ks < T / 16; ++ks) load_v(0, ks);
+
+    float o[D / 2][4];
+#pragma unroll
+    for (int i = 0; i < D / 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    const float qs[2] = {qscale[2 * quad], qscale[2 * quad + 1]};
+    for (uint32_t t = 0; t < tiles; ++t) {
+        const bool more = t + 1 < tiles;
+        if (more) write_places(t + 1, sc_next);
+        // four sums per score (limb, half of the dims' runs): short chains, as each product's addition
+        // to the accumulator is cut to fp32 rather than rounded, and four products in flight
+        float part[4][4] = {};
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const uint32_t w0[4] = {kr[0][c].x, kr[0][c].y, kr[0][c].z, kr[0][c].w};
+            const uint32_t w1[4] = {kr[1][c].x, kr[1][c].y, kr[1][c].z, kr[1][c].w};
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint4 hi = qf_s[c][0][half][lane], lo = qf_s[c][1][half][lane];
+                const uint32_t bh[4] = {hi.x, hi.y, hi.z, hi.w}, bl[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t b0 = bias_codes<FMT>(w0[2 * half + j]), b1 = bias_codes<FMT>(w1[2 * half + j]);
+                    const uint32_t a0 = pair_in_word<FMT, 0>(b0), a2 = pair_in_word<FMT, 1>(b0);
+                    const uint32_t a1 = pair_in_word<FMT, 0>(b1), a3 = pair_in_word<FMT, 1>(b1);
+                    mma16816(part[j], a0, a1, a2, a3, bh[2 * j], bh[2 * j + 1]);
+                    mma16816(part[2 + j], a0, a1, a2, a3, bl[2 * j], bl[2 * j + 1]);
+                }
+            }
+        }
+        float s[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = (part[0][i] + part[1][i]) + (part[2][i] + part[3][i]);
+        // s: positions oct and oct + 8 of the warp's 16, heads 2 quad and 2 quad + 1
+        float vs[2], top[2] = {-INFINITY, -INFINITY};
+        bool valid[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int p = warp * 16 + oct + 8 * r;
+            const float2 sc = sc_s[t & 1][p];
+            valid[r] = j0 + t * T + p < j1;
+            vs[r] = sc.y;
+            const float lg = log2f(fmaxf(sc.y, kKvTiny));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                s[2 * r + h] = valid[r] ? s[2 * r + h] * sc.x * qs[h] : -INFINITY;
+                top[h] = fmaxf(top[h], s[2 * r + h] + (valid[r] ? lg : 0.0f));
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            for (int x = 4; x < 32; x <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], x));
+        }
+        if (oct == 0) *reinterpret_cast<float2*>(&wmax[warp][2 * quad]) = make_float2(top[0], top[1]);
+        __syncthreads();
+        if (more) {
+            load_k(t + 1);
+            if (tid < T) sc_s[(t + 1) & 1][tid] = sc_next;
+        }
+        float mn[2] = {m[0], m[1]}, fs[2];
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float2 x = *reinterpret_cast<const float2*>(&wmax[w][2 * quad]);
+            mn[0] = fmaxf(mn[0], x.x), mn[1] = fmaxf(mn[1], x.y);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            fs[h] = m[h] == mn[h] ? 1.0f : ex2(m[h] - mn[h]);
+            m[h] = mn[h];
+            l[h] *= fs[h];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float e = valid[r] ? ex2(s[2 * r + h] - mn[h]) : 0.0f;
+                l[h] += e;
+                const float p = valid[r] ? e * vs[r] : 0.0f;
+                const __half hi = __float2half_rn(p);
+                const int at = warp * 16 + oct + 8 * r;
+                p_s[0][2 * quad + h][at] = hi;
+                p_s[1][2 * quad + h][at] = __float2half_rn(p - __half2float(hi));
+            }
+        }
+        __syncthreads();
+        float add[D / 2][4] = {};   // this tile's share, added to o in fp32 (see above)
+#pragma unroll
+        for (int ks = 0; ks < T / 16; ++ks) {
+            const uint2 bh = *reinterpret_cast<const uint2*>(&p_s[0][oct][16 * ks + 4 * quad]);
+            const uint2 bl = *reinterpret_cast<const uint2*>(&p_s[1][oct][16 * ks + 4 * quad]);
+#pragma unroll
+            for (int wd = 0; wd < D / 4; ++wd) {
+                uint32_t w[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) w[r] = bias_codes<FMT>(vr[ks][r][wd]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t a0 = pair_of_words<FMT>(w[0], w[1], 2 * i), a1 = pair_of_words<FMT>(w[0], w[1], 2 * i + 1);
+                    const uint32_t a2 = pair_of_words<FMT>(w[2], w[3], 2 * i), a3 = pair_of_words<FMT>(w[2], w[3], 2 * i + 1);
+                    mma16816(add[2 * wd + i], a0, a1, a2, a3, bh.x, bh.y);
+                    mma16816(add[2 * wd + i], a0, a1, a2, a3, bl.x, bl.y);
+                }
+            }
+            if (more) load_v(t + 1, ks);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] = o[i][j] * fs[j & 1] + add[i][j];
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        for (int x = 4; x < 32; x <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], x);
+    }
+    if (oct == 0) lsum[warp][2 * quad] = l[0], lsum[warp][2 * quad + 1] = l[1];
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        l[h] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) l[h] += lsum[w][2 * quad + h];
+    }
+    const bool direct = a.direct && items == 1;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int head = 2 * quad + h;
+        if (head >= grp) continue;
+        const float f = (FMT == GTM_KV_E4M3 ? 256.0f : 1.0f) / (direct ? l[h] : 1.0f);
+        const size_t at = (static_cast<size_t>(item) * a.kv_heads + kvh) * grp + head;
+        float* dst = direct ? a.ctx + (static_cast<size_t>(row) * a.q_heads + static_cast<size_t>(kvh) * grp + head) * HD : a.part + at * HD;
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i)
+            *reinterpret_cast<float4*>(dst + vdim + 4 * i) =
+                make_float4(o[2 * i][h] * f, o[2 * i][h + 2] * f, o[2 * i + 1][h] * f, o[2 * i + 1][h + 2] * f);
+        if (!direct && warp == 0 && oct == 0) a.ml[at] = make_float2(m[h], l[h]);
     }
 }
 
-// One CTA per (query head, row): the chunks' (largest, sum, weighted V) merged.
-__global__ void __launch_bounds__(512) kv_combine(const __grid_constant__ AttnArgs a, uint32_t hd) {
-    const size_t at = static_cast<size_t>(blockIdx.y) * a.q_heads + blockIdx.x;
-    const float2* ml = a.ml + at * a.splits;
-    const float* p = a.part + at * a.splits * hd;
-    float m = -INFINITY;
-    for (uint32_t s = 0; s < a.splits; ++s) m = fmaxf(m, ml[s].x);
-    float l = 0.0f, o = 0.0f;
-    for (uint32_t s = 0; s < a.splits; ++s) {
-        if (ml[s].x == -INFINITY && ml[s].y == 0.0f) continue;   // an empty chunk
-        const float f = expf(ml[s].x - m);
-        l += ml[s].y * f;
-        o += p[static_cast<size_t>(s) * hd + threadIdx.x] * f;
+// One CTA per (query head, row): the row's partial results merged.
+template <int HD>
+__global__ void __launch_bounds__(HD / 4) kv_combine(const __grid_constant__ RowsArgs a, const __grid_constant__ Starts starts) {
+    const uint32_t head = blockIdx.x, row = blockIdx.y;
+    const uint32_t first = starts.v[row], items = starts.v[row + 1] - first;
+    if (a.direct && items == 1) return;
+    const size_t at = static_cast<size_t>(first) * a.q_heads + head, step = a.q_heads;   // [item][kv head][group]
+    float m = -INFINITY, l = 0.0f;
+    for (uint32_t s = 0; s < items; ++s) m = fmaxf(m, a.ml[at + s * step].x);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t s = 0; s < items; ++s) {
+        const float2 x = a.ml[at + s * step];
+        const float f = ex2(x.x - m);
+        const float4 p = reinterpret_cast<const float4*>(a.part + (at + s * step) * HD)[threadIdx.x];
+        l += x.y * f;
+        o.x += p.x * f, o.y += p.y * f, o.z += p.z * f, o.w += p.w * f;
     }
-    a.ctx[at * hd + threadIdx.x] = o / l;
+    const float r = 1.0f / l;
+    reinterpret_cast<float4*>(a.ctx + (static_cast<size_t>(row) * a.q_heads + head) * HD)[threadIdx.x] =
+        make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
 }
 
-uint32_t splits_for(uint32_t kv_heads, uint32_t n) {
-    const uint32_t want = (592 + n * kv_heads - 1) / (n * kv_heads);
-    return std::max(1u, want);
-}
+// Items of all rows are at most n plus this (a chunk is at least the total / kTargetItems).
+constexpr uint32_t kTargetCtas = 592;
 
 template <int HD>
-void launch(const AttnArgs& a, const RowU32& pos, const RowU32& seq, uint32_t n, uint32_t fmt, cudaStream_t st) {
-    const dim3 grid(a.kv_heads, a.splits, n);
-    if (fmt == GTM_KV_INT8)
-        kv_partial<HD, GTM_KV_INT8><<<grid, kThreads, 0, st>>>(a, pos, seq);
-    else
-        kv_partial<HD, GTM_KV_E4M3><<<grid, kThreads, 0, st>>>(a, pos, seq);
-    kv_combine<<<dim3(a.q_heads, n), HD, 0, st>>>(a, HD);
+void launch_rows(RowsArgs& a, Starts& starts, const RowU32& pos, const RowU32& seq, uint32_t fmt, cudaStream_t st) {
+    using S = RowsShape<HD>;
+    uint64_t sum = 0;
+    uint32_t len[kMaxBatchRows];
+    for (uint32_t i = 0; i < a.n; ++i) {
+        const Span s = row_span(pos.v[i], a.window, a.prefix_len);
+        len[i] = s.on + (a.list_prefix ? s.pn : 0);
+        sum += len[i];
+    }
+    const uint32_t target = std::max(1u, kTargetCtas / a.kv_heads);
+    const uint64_t want = (sum + target - 1) / target;
+    a.chunk = static_cast<uint32_t>((want + S::kTile - 1) / S::kTile * S::kTile);
+    if (a.chunk < S::kTile) a.chunk = S::kTile;
+    bool merge = !a.direct;
+    starts.v[0] = 0;
+    for (uint32_t i = 0; i < a.n; ++i) {
+        const uint32_t items = (len[i] + a.chunk - 1) / a.chunk;
+        starts.v[i + 1] = starts.v[i] + items;
+        merge = merge || items > 1;
+    }
+    const uint32_t items = starts.v[a.n];
+    a.ml = reinterpret_cast<float2*>(a.part + static_cast<size_t>(items) * a.q_heads * HD);
+    const dim3 grid(items, a.kv_heads);
+    if (items) {
+        if (fmt == GTM_KV_INT8)
+            kv_rows<HD, GTM_KV_INT8><<<grid, S::kWarps * 32, 0, st>>>(a, starts, pos, seq);
+        else
+            kv_rows<HD, GTM_KV_E4M3><<<grid, S::kWarps * 32, 0, st>>>(a, starts, pos, seq);
+    }
+    if (merge) kv_combine<HD><<<dim3(a.q_heads, a.n), HD / 4, 0, st>>>(a, starts);
 }
 
 bool heads_ok(uint32_t q_heads, uint32_t kv_heads) {
@@ -202,9 +437,9 @@ extern "C" {
 GTM_API size_t gtm_attention_kv_workspace_bytes(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t n) {
     if (!heads_ok(q_heads, kv_heads) || (head_dim != 128 && head_dim != 256 && head_dim != 512) || n == 0 || n > kMaxBatchRows)
         return 0;
-    // n' * splits(n') over n' <= n rows is at most this many partials per query head
-    const size_t rows = static_cast<size_t>(n) + 592 / kv_heads + 1;
-    return rows * q_heads * (head_dim + 2) * sizeof(float) + 256;
+    // rows' items: sum of ceil(len / chunk) <= n + sum / chunk <= n + target
+    const size_t items = static_cast<size_t>(n) + std::max(1u, kTargetCtas / kv_heads);
+    return items * q_heads * (head_dim + 2) * sizeof(float) + 256;
 }
 
 GTM_API int gtm_attention_kv_rows(const GtmKvCache* c, const GtmKvCache* prefix, uint32_t prefix_seq, uint32_t prefix_len,
@@ -244,28 +479,28 @@ GTM_API int gtm_attention_kv_rows(const GtmKvCache* c, const GtmKvCache* prefix,
     }
     const size_t need = gtm_attention_kv_workspace_bytes(q_heads, c->kv_heads, c->head_dim, n);
     if (!ws || ws_bytes < need) return set_error(GTM_ERR_WORKSPACE, "%s: workspace needs %zu bytes", fn, need);
-    AttnArgs a;
     const auto side = [](const GtmKvCache* x, size_t s) {
         const size_t vec = s * x->capacity * x->kv_heads;
         return Side{static_cast<const uint8_t*>(x->k_dev) + vec * x->head_dim, static_cast<const uint8_t*>(x->v_dev) + vec * x->head_dim,
                     x->k_scale_dev + vec, x->v_scale_dev + vec, x->capacity};
     };
+    RowsArgs a;
     a.own = side(c, 0);
     a.pre = prefix_len ? side(prefix, prefix_seq) : a.own;
     a.q = q;
-    a.q_heads = q_heads, a.kv_heads = c->kv_heads;
-    a.window = window, a.prefix_len = prefix_len;
-    a.splits = splits_for(c->kv_heads, n);
-    a.part = static_cast<float*>(ws);
-    a.ml = reinterpret_cast<float2*>(a.part + static_cast<size_t>(n) * q_heads * a.splits * c->head_dim);
     a.ctx = ctx;
+    a.part = static_cast<float*>(ws);
+    a.q_heads = q_heads, a.kv_heads = c->kv_heads, a.n = n;
+    a.window = window, a.prefix_len = prefix_len;
+    a.list_prefix = true, a.direct = true;
+    Starts starts;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (c->head_dim == 128)
-        launch<128>(a, pos, seq, n, c->format, st);
+        launch_rows<128>(a, starts, pos, seq, c->format, st);
     else if (c->head_dim == 256)
-        launch<256>(a, pos, seq, n, c->format, st);
+        launch_rows<256>(a, starts, pos, seq, c->format, st);
     else
-        launch<512>(a, pos, seq, n, c->format, st);
+        launch_rows<512>(a, starts, pos, seq, c->format, st);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return set_cuda_error(fn, e);
     clear_error();
