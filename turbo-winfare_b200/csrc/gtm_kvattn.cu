@@ -13,78 +13,15 @@
 // outside a row's span holds reaches a sum. A partial result (m, l, O) is merged by kv_combine.
 //
 // kv_rows: a CTA per (row, kv head, run of positions), for positions that one row attends.
-#include <cuda_fp16.h>
-
+// kv_shared (gtm_kvshared.cu): the prefix, for all rows at once.
 #include <algorithm>
 #include <cmath>
 
 #include "gtm_frag.cuh"
-#include "gtm_kvcache.cuh"
+#include "gtm_kvattn.cuh"
 
 namespace gtm {
 namespace {
-
-constexpr uint32_t kMaxGroup = 8;
-constexpr float kLog2e = 1.4426950408889634f;
-
-// One side (prefix or own cache) as the kernels address it.
-struct Side {
-    const uint8_t *k, *v;
-    const float *ks, *vs;
-    uint32_t capacity;
-};
-
-struct Span {
-    uint32_t pa, pn, oa, on;   // prefix: first and count; own: first and count
-};
-__host__ __device__ __forceinline__ Span row_span(uint32_t pos, uint32_t window, uint32_t prefix_len) {
-    const uint64_t end = static_cast<uint64_t>(pos) + 1;
-    const uint64_t first = window && end > window ? end - window : 0;
-    const uint64_t P = prefix_len;
-    Span s;
-    const uint64_t pe = end < P ? end : P;
-    s.pa = static_cast<uint32_t>(first < P ? first : P);
-    s.pn = static_cast<uint32_t>(pe > first ? pe - first : 0);
-    s.oa = static_cast<uint32_t>(first > P ? first : P);
-    s.on = static_cast<uint32_t>(end > s.oa ? end - s.oa : 0);
-    return s;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
-// Code words (4 codes) as half2 pairs. Int8: 1024 + (code + 128) is the half 0x6400 | byte, minus
-// 1152. E4m3: sign and 7 bits moved to a half's sign, exponent and top mantissa bits: value * 2^-8,
-// exact, subnormals included.
-template <int FMT>
-__device__ __forceinline__ uint32_t bias_codes(uint32_t w) {
-    return FMT == GTM_KV_INT8 ? w ^ 0x80808080u : w;
-}
-__device__ __forceinline__ uint32_t hsub1152(uint32_t h) {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t e4m3_halves(uint32_t v) {   // codes in bytes 1 and 3
-    return (v & 0x80008000u) | ((v >> 1) & 0x3F803F80u);
-}
-// codes 2i, 2i + 1 of one (biased) word
-template <int FMT, int I>
-__device__ __forceinline__ uint32_t pair_in_word(uint32_t w) {
-    if constexpr (FMT == GTM_KV_INT8) return hsub1152(__byte_perm(w, 0x64646464u, I ? 0x4342 : 0x4140));
-    return e4m3_halves(__byte_perm(w, 0u, I ? 0x3424 : 0x1404));
-}
-// code i of word a (low half) and of word b (high half)
-template <int FMT>
-__device__ __forceinline__ uint32_t pair_of_words(uint32_t a, uint32_t b, int i) {
-    if constexpr (FMT == GTM_KV_INT8) {
-        const uint32_t x = __byte_perm(a, b, i | ((4 + i) << 4));
-        return hsub1152(__byte_perm(x, 0x64646464u, 0x4140));
-    }
-    return e4m3_halves(__byte_perm(a, b, (i << 4) | ((4 + i) << 12)));
-}
 
 // ---- rows over their own positions ----------------------------------------------------------------
 
@@ -95,8 +32,13 @@ struct RowsArgs {
     float* part;     // [item][kv_heads][group][head_dim]
     float2* ml;      // [item][kv_heads][group]: m (base 2), l
     uint32_t q_heads, kv_heads, n, window, prefix_len, chunk;
-    bool list_prefix, direct;   // prefix positions are in the rows' lists; rows of one item write ctx
+    bool list_prefix;   // prefix positions are in the rows' lists, not in kv_shared
 };
+
+// A row of one item with nothing elsewhere is written to ctx at once.
+__device__ __forceinline__ bool is_whole(const RowsArgs& a, uint32_t items, const Span& sp) {
+    return items == 1 && (a.list_prefix || sp.pn == 0);
+}
 struct Starts {
     uint32_t v[kMaxBatchRows + 1];   // first item of each row, then the number of items
 };
@@ -137,6 +79,7 @@ __global__ void __launch_bounds__(RowsShape<HD>::kWarps * 32, HD == 512 ? 1 : 2)
     const uint32_t items = starts.v[row + 1] - starts.v[row];
     const int grp = static_cast<int>(a.q_heads / a.kv_heads);
     Span sp = row_span(pos.v[row], a.window, a.prefix_len);
+    const bool direct = is_whole(a, items, sp);
     if (!a.list_prefix) sp.pn = 0;
     const uint32_t total = sp.pn + sp.on;
     const uint32_t j0 = (item - starts.v[row]) * a.chunk, j1 = min(total, j0 + a.chunk);
@@ -349,7 +292,6 @@ __global__ void __launch_bounds__(RowsShape<HD>::kWarps * 32, HD == 512 ? 1 : 2)
 #pragma unroll
         for (int w = 0; w < W; ++w) l[h] += lsum[w][2 * quad + h];
     }
-    const bool direct = a.direct && items == 1;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int head = 2 * quad + h;
@@ -365,20 +307,34 @@ __global__ void __launch_bounds__(RowsShape<HD>::kWarps * 32, HD == 512 ? 1 : 2)
     }
 }
 
-// One CTA per (query head, row): the row's partial results merged.
+// One CTA per (query head, row): the row's partial results merged, its own items' and the shared part's.
 template <int HD>
-__global__ void __launch_bounds__(HD / 4) kv_combine(const __grid_constant__ RowsArgs a, const __grid_constant__ Starts starts) {
+__global__ void __launch_bounds__(HD / 4) kv_combine(const __grid_constant__ RowsArgs a, const __grid_constant__ Starts starts,
+                                                     const __grid_constant__ RowU32 pos, const __grid_constant__ SharedPlan sh) {
     const uint32_t head = blockIdx.x, row = blockIdx.y;
     const uint32_t first = starts.v[row], items = starts.v[row + 1] - first;
-    if (a.direct && items == 1) return;
-    const size_t at = static_cast<size_t>(first) * a.q_heads + head, step = a.q_heads;   // [item][kv head][group]
+    const Span sp = row_span(pos.v[row], a.window, a.prefix_len);
+    if (is_whole(a, items, sp)) return;
+    // result s < items: [item][kv head][group]; then slots c + u of the CTAs that took the unit's tiles
+    const size_t at = static_cast<size_t>(first) * a.q_heads + head;
+    const uint32_t grp = a.q_heads / a.kv_heads, kvh = head / grp, qr = row * grp + head % grp;
+    uint32_t parts = items;
+    size_t slot = 0;
+    if (!a.list_prefix && sp.pn) {
+        const uint32_t u = qr / kSharedRows, g = kvh * sh.start[sh.units] + sh.start[u], tiles = sh.start[u + 1] - sh.start[u];
+        const uint32_t c0 = g / sh.per, c1 = (g + tiles - 1) / sh.per;
+        slot = (static_cast<size_t>(c0) + kvh * sh.units + u) * kSharedRows + qr % kSharedRows;
+        parts += c1 - c0 + 1;
+    }
+    auto ml = [&](uint32_t s) { return s < items ? a.ml[at + static_cast<size_t>(s) * a.q_heads] : sh.ml[slot + static_cast<size_t>(s - items) * kSharedRows]; };
     float m = -INFINITY, l = 0.0f;
-    for (uint32_t s = 0; s < items; ++s) m = fmaxf(m, a.ml[at + s * step].x);
+    for (uint32_t s = 0; s < parts; ++s) m = fmaxf(m, ml(s).x);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t s = 0; s < items; ++s) {
-        const float2 x = a.ml[at + s * step];
+    for (uint32_t s = 0; s < parts; ++s) {
+        const float2 x = ml(s);
         const float f = ex2(x.x - m);
-        const float4 p = reinterpret_cast<const float4*>(a.part + (at + s * step) * HD)[threadIdx.x];
+        const float* src = s < items ? a.part + (at + static_cast<size_t>(s) * a.q_heads) * HD : sh.part + (slot + static_cast<size_t>(s - items) * kSharedRows) * HD;
+        const float4 p = reinterpret_cast<const float4*>(src)[threadIdx.x];
         l += x.y * f;
         o.x += p.x * f, o.y += p.y * f, o.z += p.z * f, o.w += p.w * f;
     }
@@ -387,24 +343,26 @@ __global__ void __launch_bounds__(HD / 4) kv_combine(const __grid_constant__ Row
         make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
 }
 
-// Items of all rows are at most n plus this (a chunk is at least the total / kTargetItems).
+// Items of all rows are at most n plus this (a chunk is at least the total / target).
 constexpr uint32_t kTargetCtas = 592;
+uint32_t target_items(uint32_t kv_heads) { return std::max(1u, kTargetCtas / kv_heads); }
 
 template <int HD>
-void launch_rows(RowsArgs& a, Starts& starts, const RowU32& pos, const RowU32& seq, uint32_t fmt, cudaStream_t st) {
+int launch_rows(RowsArgs& a, Starts& starts, const RowU32& pos, const RowU32& seq, const SharedPlan& sh, uint32_t fmt, cudaStream_t st) {
     using S = RowsShape<HD>;
     uint64_t sum = 0;
     uint32_t len[kMaxBatchRows];
+    bool merge = false;
     for (uint32_t i = 0; i < a.n; ++i) {
         const Span s = row_span(pos.v[i], a.window, a.prefix_len);
         len[i] = s.on + (a.list_prefix ? s.pn : 0);
+        merge = merge || (!a.list_prefix && s.pn);
         sum += len[i];
     }
-    const uint32_t target = std::max(1u, kTargetCtas / a.kv_heads);
-    const uint64_t want = (sum + target - 1) / target;
-    a.chunk = static_cast<uint32_t>((want + S::kTile - 1) / S::kTile * S::kTile);
-    if (a.chunk < S::kTile) a.chunk = S::kTile;
-    bool merge = !a.direct;
+    const uint64_t want = (sum + target_items(a.kv_heads) - 1) / target_items(a.kv_heads);
+    const uint64_t chunk = std::max<uint64_t>(1, (want + S::kTile - 1) / S::kTile) * S::kTile;
+    if (chunk > 0x7FFFFFFFull) return set_error(GTM_ERR_UNSUPPORTED, "gtm_attention_kv_rows: %llu positions", (unsigned long long)sum);
+    a.chunk = static_cast<uint32_t>(chunk);
     starts.v[0] = 0;
     for (uint32_t i = 0; i < a.n; ++i) {
         const uint32_t items = (len[i] + a.chunk - 1) / a.chunk;
@@ -420,11 +378,33 @@ void launch_rows(RowsArgs& a, Starts& starts, const RowU32& pos, const RowU32& s
         else
             kv_rows<HD, GTM_KV_E4M3><<<grid, S::kWarps * 32, 0, st>>>(a, starts, pos, seq);
     }
-    if (merge) kv_combine<HD><<<dim3(a.q_heads, a.n), HD / 4, 0, st>>>(a, starts);
+    if (merge) kv_combine<HD><<<dim3(a.q_heads, a.n), HD / 4, 0, st>>>(a, starts, pos, sh);
+    return GTM_OK;
 }
 
 bool heads_ok(uint32_t q_heads, uint32_t kv_heads) {
-    return kv_heads > 0 && q_heads > 0 && q_heads <= 65535u && q_heads % kv_heads == 0 && q_heads / kv_heads <= kMaxGroup;
+    return kv_heads > 0 && q_heads > 0 && q_heads <= 65535u && q_heads % kv_heads == 0 && q_heads / kv_heads <= kKvMaxGroup;
+}
+
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+// rows' items: sum of ceil(len / chunk) <= n + sum / chunk <= n + target
+size_t rows_bytes(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t n) {
+    return up256((static_cast<size_t>(n) + target_items(kv_heads)) * q_heads * (head_dim + 2) * sizeof(float));
+}
+size_t shared_bytes(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t n, int sms) {
+    return up256(shared_slots(q_heads, kv_heads, n, sms) * kSharedRows * (head_dim + 2) * sizeof(float));
+}
+
+// The SM count of the current device; 148 (a B200's) where there is no device to ask, so that a
+// workspace can be planned on a host without one.
+cudaError_t num_sms(int* sms) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) {
+        cudaGetLastError();
+        *sms = 148;
+        return cudaSuccess;
+    }
+    return cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
 }
 
 }  // namespace
@@ -437,9 +417,9 @@ extern "C" {
 GTM_API size_t gtm_attention_kv_workspace_bytes(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t n) {
     if (!heads_ok(q_heads, kv_heads) || (head_dim != 128 && head_dim != 256 && head_dim != 512) || n == 0 || n > kMaxBatchRows)
         return 0;
-    // rows' items: sum of ceil(len / chunk) <= n + sum / chunk <= n + target
-    const size_t items = static_cast<size_t>(n) + std::max(1u, kTargetCtas / kv_heads);
-    return items * q_heads * (head_dim + 2) * sizeof(float) + 256;
+    int sms = 0;
+    if (num_sms(&sms) != cudaSuccess) return 0;
+    return rows_bytes(q_heads, kv_heads, head_dim, n) + shared_bytes(q_heads, kv_heads, head_dim, n, sms);
 }
 
 GTM_API int gtm_attention_kv_rows(const GtmKvCache* c, const GtmKvCache* prefix, uint32_t prefix_seq, uint32_t prefix_len,
@@ -458,7 +438,7 @@ GTM_API int gtm_attention_kv_rows(const GtmKvCache* c, const GtmKvCache* prefix,
     }
     if (!heads_ok(q_heads, c->kv_heads))
         return set_error(GTM_ERR_UNSUPPORTED, "%s: q_heads %u / kv_heads %u (a group of 1..%u)", fn, q_heads, c->kv_heads,
-                         kMaxGroup);
+                         kKvMaxGroup);
     if (n == 0) {
         clear_error();
         return GTM_OK;
@@ -492,15 +472,29 @@ GTM_API int gtm_attention_kv_rows(const GtmKvCache* c, const GtmKvCache* prefix,
     a.part = static_cast<float*>(ws);
     a.q_heads = q_heads, a.kv_heads = c->kv_heads, a.n = n;
     a.window = window, a.prefix_len = prefix_len;
-    a.list_prefix = true, a.direct = true;
-    Starts starts;
+    int sms = 0;
+    const cudaError_t de = num_sms(&sms);
+    if (de != cudaSuccess) return set_cuda_error(fn, de);
+    SharedPlan plan;
+    plan.units = 0;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    a.list_prefix = !(prefix_len && n > 1);
+    if (!a.list_prefix) {
+        const SharedCall call{prefix, prefix_seq, prefix_len, q_heads, c->kv_heads, c->head_dim, n, window, q};
+        plan_shared(call, pos, sms, plan);
+        plan.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + rows_bytes(q_heads, c->kv_heads, c->head_dim, n));
+        plan.ml = reinterpret_cast<float2*>(plan.part + shared_slots(q_heads, c->kv_heads, n, sms) * kSharedRows * c->head_dim);
+        if (plan.start[plan.units]) rc = launch_shared(call, pos, plan, sms, st);
+        if (rc) return rc;
+    }
+    Starts starts;
     if (c->head_dim == 128)
-        launch_rows<128>(a, starts, pos, seq, c->format, st);
+        rc = launch_rows<128>(a, starts, pos, seq, plan, c->format, st);
     else if (c->head_dim == 256)
-        launch_rows<256>(a, starts, pos, seq, c->format, st);
+        rc = launch_rows<256>(a, starts, pos, seq, plan, c->format, st);
     else
-        launch_rows<512>(a, starts, pos, seq, c->format, st);
+        rc = launch_rows<512>(a, starts, pos, seq, plan, c->format, st);
+    if (rc) return rc;
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return set_cuda_error(fn, e);
     clear_error();

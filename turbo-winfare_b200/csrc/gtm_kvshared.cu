@@ -1,0 +1,612 @@
+// The shared prefix of a step's rows (include/gtmoe_attention.h), computed once for all of them on
+// the tcgen05 tensor cores.
+//
+// A unit is a kv head and 64 query rows (row, query head of the group). Per tile of 128 ring rows:
+//   S^T [128 positions x 64 rows] = K q^T: K's codes become fp16 in tensor memory (operand A, a
+//     position per lane), q's high and low limbs wait in shared memory (operand B);
+//   softmax weights, a position per thread: p = exp2(s2 - m) * vs, its limbs into shared memory;
+//   O^T [dims x 64 rows] += V^T p: V's codes become fp16 in shared memory (operand A, dims
+//     contiguous), p is operand B. O stays in tensor memory.
+// Rows on the N side make a unit of any number of rows cost what its 64 columns cost, and a
+// position per lane lets a thread apply its own scales; the maxima over positions take one redux
+// per column and warp. m only moves when a score passes it by 8 (a factor of 256 that fp16 has room
+// for), so O is rarely rescaled. Tiles follow ring slots, not positions: softmax does not mind the
+// order, no tile wraps, and each row's span is a mask on the slot's position.
+//
+// The work is the flat list of (kv head, unit, tile), cut into equal runs, one per CTA; a CTA leaves a
+// partial result for each unit it touches.
+//
+// Roles: warps 0-3 softmax and O; 4-7 K; 8-11 V; 12 and 14 TMA loads of K and V codes; 13 MMA. Every
+// wait is bounded (1 s); one that runs out stops the CTA and marks its results NaN.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "gtm_frag.cuh"
+#include "gtm_kvattn.cuh"
+#include "gtm_tcgen05.cuh"
+
+namespace gtm {
+namespace {
+
+constexpr int N = kSharedRows;
+constexpr int TP = 128;              // positions of a tile
+constexpr int kThreads = 480;
+constexpr uint64_t kWaitNs = 1000000000ull;
+constexpr int KA = 4;                // K chunks (64 dims) in tensor memory
+constexpr uint32_t kLongest = 32;    // tiles summed in tensor memory before the result goes to memory
+
+template <int HD>
+struct Shape {
+    static constexpr int kChunks = HD / 64;      // K chunks of a tile
+    static constexpr int kVStages = HD / 64;     // V stages of a tile: 128 dims x 64 positions
+    static constexpr int RK = HD == 512 ? 2 : 4, RV = HD == 512 ? 2 : 4, VST = HD == 512 ? 2 : 4;
+    static constexpr int kQ = 2 * kChunks * 8192, kP = 2 * 16384, kV = VST * 16384, kRawK = RK * 8192, kRawV = RV * 8192;
+    static constexpr int kBars = 2 * RK + 2 * RV + 2 * KA + 2 * VST + 4 + 2;
+    static constexpr int kSmall = (4 * N + 4 * N + 2 * N) * 4 + kBars * 8 + 16;
+    static constexpr int kSmem = kQ + kP + kV + kRawK + kRawV + kSmall;
+    static constexpr uint32_t kOCol = 0, kSCol = HD / 128 * N, kACol = kSCol + 2 * N;   // tensor memory columns
+    static_assert(kACol + KA * 32 <= 512, "tensor memory");
+    static_assert(kSmem <= 232448, "shared memory");
+};
+
+struct SharedArgs {
+    CUtensorMap k_map, v_map;      // the prefix's codes [capacity][kv_heads * head_dim]
+    const float *ks, *vs;          // [kv_heads][capacity]
+    const float* q;
+    uint32_t q_heads, kv_heads, n, grp, capacity, ring_tiles, window, prefix_len, total;
+    uint32_t lo[kMaxUnitsPerHead], first[kMaxUnitsPerHead];   // a unit's first position and its ring tile
+    SharedPlan plan;
+};
+
+__device__ __forceinline__ float redux_max(float x) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+}
+// Whether any of the 128 softmax threads says so (hardware barrier 1).
+__device__ __forceinline__ bool any_of_128(bool x) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"(x ? 1u : 0u) : "memory");
+    return r != 0;
+}
+// Operand whose M or N side is contiguous: rows (K) of 64 fp16, 8-row atoms of 1,024 bytes in the
+// 128-byte swizzle; `block` bytes to the next 64 of M or N.
+__device__ __forceinline__ uint64_t sdesc_mn(uint32_t addr, uint32_t block) {
+    uint64_t d = 0;
+    d |= (uint64_t)((addr >> 4) & 0x3FFFu);
+    d |= (uint64_t)((block >> 4) & 0x3FFFu) << 16;
+    d |= (uint64_t)(1024u >> 4) << 32;
+    d |= (uint64_t)1u << 46;
+    d |= (uint64_t)2u << 61;
+    return d;
+}
+
+// 16 codes to 8 + 8 fp16
+template <int FMT>
+__device__ __forceinline__ void widen(const uint4& w, uint32_t (&o)[8]) {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t b = bias_codes<FMT>(x[i]);
+        o[2 * i] = pair_in_word<FMT, 0>(b);
+        o[2 * i + 1] = pair_in_word<FMT, 1>(b);
+    }
+}
+
+struct Segment {
+    uint32_t kvh, unit, tile, tiles, slot;
+};
+__device__ __forceinline__ Segment segment_at(const SharedArgs& a, uint32_t g, uint32_t end) {
+    Segment s;
+    const uint32_t per_head = a.plan.start[a.plan.units];
+    s.kvh = g / per_head;
+    const uint32_t r = g - s.kvh * per_head;
+    uint32_t u = 0;
+    for (uint32_t step = kMaxUnitsPerHead / 2; step; step >>= 1)
+        if (u + step < a.plan.units && a.plan.start[u + step] <= r) u += step;
+    s.unit = u;
+    s.tile = r - a.plan.start[u];
+    s.tiles = min(min(a.plan.start[u + 1] - r, end - g), kLongest);
+    s.slot = blockIdx.x + s.kvh * a.plan.units + u;
+    return s;
+}
+
+template <int HD, int FMT>
+__global__ void __launch_bounds__(kThreads, 1)
+    kv_shared(const __grid_constant__ SharedArgs a, const __grid_constant__ RowU32 pos) {
+    using S = Shape<HD>;
+    constexpr int RK = S::RK, RV = S::RV, VST = S::VST, C = S::kChunks, MT = HD / 128;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* sQ = smem;                    // [limb][chunk][64 rows][128 B]
+    uint8_t* sP = sQ + S::kQ;              // [limb][128 positions][128 B]
+    uint8_t* sV = sP + S::kP;              // [stage][dims 0-63, 64-127][64 positions][128 B]
+    uint8_t* sRawK = sV + S::kV;           // [stage][128 positions][64 B], 64-byte swizzle
+    uint8_t* sRawV = sRawK + S::kRawK;     // [stage][64 positions][128 B], 128-byte swizzle
+    float* wtop = reinterpret_cast<float*>(sRawV + S::kRawV);   // [4 warps][64]
+    float* m_s = wtop + 4 * N;             // running maxima
+    float* f_s = m_s + N;                  // factors of a rescale
+    float* qf_s = f_s + N;                 // q's power of two and log2(e)
+    float* g_s = qf_s + N;                 // a second factor, when results merge
+    uint32_t* rlo = reinterpret_cast<uint32_t*>(g_s + N);   // rows' spans, from the unit's first position
+    uint32_t* rhi = rlo + N;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(rhi + N);
+    uint64_t *rk_full = bars, *rk_empty = rk_full + RK, *rv_full = rk_empty + RK, *rv_empty = rv_full + RV,
+             *ka_full = rv_empty + RV, *ka_empty = ka_full + KA, *v_full = ka_empty + KA, *v_empty = v_full + VST,
+             *s_full = v_empty + VST, *s_empty = s_full + 2, *p_full = s_empty + 2, *p_empty = p_full + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_empty + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < RK; ++i) tc::mbar_init(&rk_full[i], 1), tc::mbar_init(&rk_empty[i], 128);
+        for (int i = 0; i < RV; ++i) tc::mbar_init(&rv_full[i], 1), tc::mbar_init(&rv_empty[i], 128);
+        for (int i = 0; i < KA; ++i) tc::mbar_init(&ka_full[i], 128), tc::mbar_init(&ka_empty[i], 1);
+        for (int i = 0; i < VST; ++i) tc::mbar_init(&v_full[i], 128), tc::mbar_init(&v_empty[i], 1);
+        for (int i = 0; i < 2; ++i) tc::mbar_init(&s_full[i], 1), tc::mbar_init(&s_empty[i], 128);
+        tc::mbar_init(p_full, 128), tc::mbar_init(p_empty, 1);
+        *abort_flag = (tc::smem_u32(smem) & 1023u) ? 1 : 0;   // the swizzled layouts need it
+        tc::mbar_fence_init();
+    }
+    if (warp == 13) tc::tmem_alloc(tmem_slot, 512);
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    const uint32_t g0 = min(a.total, blockIdx.x * a.plan.per), g1 = min(a.total, g0 + a.plan.per);
+    uint32_t kc = 0, vc = 0, ti = 0;   // K chunks, V stages and tiles so far, the same for every role
+    uint32_t done_slot = 0xFFFFFFFFu;  // the slot that already holds this CTA's result
+    for (uint32_t g = g0; g < g1;) {
+        const Segment sg = segment_at(a, g, g1);
+        g += sg.tiles;
+        if (__syncthreads_or(*abort_flag)) {
+            if (tid < N) a.plan.ml[static_cast<size_t>(sg.slot) * N + tid] = make_float2(0.0f, __int_as_float(0x7FC00000));
+            done_slot = sg.slot;
+            continue;
+        }
+        // ---- q's limbs and the rows' spans
+        for (int r = warp; r < N; r += kThreads / 32) {
+            const uint32_t qr = sg.unit * N + r, row = qr / a.grp, h = qr - row * a.grp;
+            const bool live = row < a.n;
+            const float* src = a.q + (static_cast<size_t>(row) * a.q_heads + sg.kvh * a.grp + h) * HD;
+            float x[HD / 32], top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < HD / 128; ++i) {
+                const float4 v = live ? __ldg(reinterpret_cast<const float4*>(src) + lane + 32 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+            }
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i) top = fmaxf(top, fabsf(x[i]));
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const int e = top > 0.0f ? max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127)) : 0;
+            const float down = __int_as_float((127 - e) << 23);
+#pragma unroll
+            for (int i = 0; i < HD / 128; ++i) {
+                const int d = 4 * lane + 128 * i;
+                uint32_t hi[2], lo[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float u = x[4 * i + 2 * j] * down, v = x[4 * i + 2 * j + 1] * down;
+                    hi[j] = cvt2(u, v);
+                    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi[j]));
+                    lo[j] = cvt2(u - b.x, v - b.y);
+                }
+                const int c = d >> 6, unit16 = (d & 63) >> 3;
+                const int off = c * 8192 + r * 128 + ((unit16 ^ (r & 7)) << 4) + (d & 4) * 2;
+                *reinterpret_cast<uint2*>(sQ + off) = make_uint2(hi[0], hi[1]);
+                *reinterpret_cast<uint2*>(sQ + C * 8192 + off) = make_uint2(lo[0], lo[1]);
+            }
+            if (lane == 0) {
+                qf_s[r] = __int_as_float((127 + e) << 23) * kLog2e * (FMT == GTM_KV_E4M3 ? 256.0f : 1.0f);
+                m_s[r] = -INFINITY;
+                const Span sp = live ? row_span(pos.v[row], a.window, a.prefix_len) : Span{0, 0, 0, 0};
+                // columns without a row are never read: they need no mask
+                rlo[r] = !live ? 0u : sp.pn ? sp.pa - a.lo[sg.unit] : 1u;
+                rhi[r] = !live ? 0xFFFFFFFFu : sp.pn ? sp.pa - a.lo[sg.unit] + sp.pn : 0u;
+            }
+        }
+        tc::fence_proxy_async_smem();
+        __syncthreads();
+        auto ring_tile = [&](uint32_t t) {
+            const uint32_t b = a.first[sg.unit] + sg.tile + t;
+            return b >= a.ring_tiles ? b - a.ring_tiles : b;
+        };
+
+        if (warp == 12) {   // ---- K codes
+            if (lane == 0) {
+                uint32_t it = kc;
+                for (uint32_t t = 0; t < sg.tiles; ++t) {
+                    const int y = static_cast<int>(ring_tile(t) * TP);
+                    for (int c = 0; c < C; ++c, ++it) {
+                        if (!tc::mbar_wait(&rk_empty[it % RK], ((it / RK) & 1) ^ 1, abort_flag, kWaitNs)) goto k_out;
+                        tc::mbar_arrive_expect_tx(&rk_full[it % RK], 8192);
+                        tc::tma_load_2d(sRawK + (it % RK) * 8192, &a.k_map, static_cast<int>(sg.kvh * HD + c * 64), y, &rk_full[it % RK]);
+                    }
+                }
+            k_out:
+                if (*abort_flag) {   // no exit while copies into this CTA's shared memory are in flight
+                    volatile int never = 0;
+                    for (uint32_t j = it > RK ? it - RK : 0; j < it; ++j) tc::mbar_wait(&rk_full[j % RK], (j / RK) & 1, &never, kWaitNs);
+                }
+            }
+        } else if (warp == 14) {   // ---- V codes
+            if (lane == 0) {
+                uint32_t it = vc;
+                for (uint32_t t = 0; t < sg.tiles; ++t) {
+                    const int y = static_cast<int>(ring_tile(t) * TP);
+                    for (int c = 0; c < S::kVStages; ++c, ++it) {
+                        if (!tc::mbar_wait(&rv_empty[it % RV], ((it / RV) & 1) ^ 1, abort_flag, kWaitNs)) goto v_out;
+                        tc::mbar_arrive_expect_tx(&rv_full[it % RV], 8192);
+                        tc::tma_load_2d(sRawV + (it % RV) * 8192, &a.v_map, static_cast<int>(sg.kvh * HD + (c >> 1) * 128), y + (c & 1) * 64,
+                                        &rv_full[it % RV]);
+                    }
+                }
+            v_out:
+                if (*abort_flag) {
+                    volatile int never = 0;
+                    for (uint32_t j = it > RV ? it - RV : 0; j < it; ++j) tc::mbar_wait(&rv_full[j % RV], (j / RV) & 1, &never, kWaitNs);
+                }
+            }
+        } else if (warp >= 4 && warp < 8) {   // ---- K: codes to fp16 in tensor memory, a position per lane
+            const int p = 32 * (warp & 3) + lane;
+            const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + S::kACol;
+            uint32_t it = kc;
+            const uint32_t end = kc + sg.tiles * C;
+            for (; it < end; ++it) {
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(&rk_full[it % RK], (it / RK) & 1, abort_flag, kWaitNs))) break;
+                const uint8_t* raw = sRawK + (it % RK) * 8192 + p * 64;
+                uint32_t o[32];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(raw + ((j ^ ((p >> 1) & 3)) << 4));
+                    uint32_t h[8];
+                    widen<FMT>(w, h);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[8 * j + i] = h[i];
+                }
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(&ka_empty[it % KA], ((it / KA) & 1) ^ 1, abort_flag, kWaitNs))) break;
+                tc::tc_fence_after();
+                tc::tmem_st32(lane_addr + (it % KA) * 32, o);
+                tc::tmem_st_wait();
+                tc::tc_fence_before();
+                tc::mbar_arrive(&ka_full[it % KA]);
+                tc::mbar_arrive(&rk_empty[it % RK]);   // only after the words were used (see gtm_tokens.cu)
+            }
+        } else if (warp >= 8 && warp < 12) {   // ---- V: codes to fp16 in shared memory, dims contiguous
+            const int p = (tid - 256) & 63, half = (tid - 256) >> 6;
+            uint32_t it = vc;
+            const uint32_t end = vc + sg.tiles * S::kVStages;
+            for (; it < end; ++it) {
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(&rv_full[it % RV], (it / RV) & 1, abort_flag, kWaitNs))) break;
+                const uint8_t* raw = sRawV + (it % RV) * 8192 + p * 128;
+                uint4 w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4*>(raw + (((half * 4 + j) ^ (p & 7)) << 4));
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(&v_empty[it % VST], ((it / VST) & 1) ^ 1, abort_flag, kWaitNs))) break;
+                uint8_t* dst = sV + (it % VST) * 16384 + half * 8192 + p * 128;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t h[8];
+                    widen<FMT>(w[j], h);
+                    *reinterpret_cast<uint4*>(dst + (((2 * j) ^ (p & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4*>(dst + (((2 * j + 1) ^ (p & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+                }
+                tc::fence_proxy_async_smem();
+                tc::mbar_arrive(&v_full[it % VST]);
+                tc::mbar_arrive(&rv_empty[it % RV]);
+            }
+        } else if (warp == 13) {   // ---- MMA issue (the whole warp; one elected lane issues)
+            constexpr uint32_t kQk = tc::idesc_f16(128, N);
+            constexpr uint32_t kPv = tc::idesc_f16(128, N) | (1u << 15) | (1u << 16);   // both operands M/N-contiguous
+            uint32_t ik = kc, iv = vc;
+            bool ok = true;
+            for (uint32_t t = 0; t <= sg.tiles && ok; ++t) {
+                if (t < sg.tiles) {
+                    const uint32_t x = ti + t, b = x & 1;
+                    if (!__all_sync(0xffffffffu, tc::mbar_wait(&s_empty[b], ((x >> 1) & 1) ^ 1, abort_flag, kWaitNs))) break;
+                    const uint32_t d = tmem + S::kSCol + b * N;
+                    for (int c = 0; c < C; ++c, ++ik) {
+                        if (!__all_sync(0xffffffffu, tc::mbar_wait(&ka_full[ik % KA], (ik / KA) & 1, abort_flag, kWaitNs))) { ok = false; break; }
+                        tc::tc_fence_after();
+                        const uint32_t ka = tmem + S::kACol + (ik % KA) * 32;
+                        const uint64_t qh = tc::sdesc_sw128(tc::smem_u32(sQ) + c * 8192);
+                        const uint64_t ql = tc::sdesc_sw128(tc::smem_u32(sQ) + (C + c) * 8192);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            tc::mma_f16_ts(d, ka + 8 * k, ql + 2 * k, kQk, (c > 0 || k > 0) ? 1u : 0u);
+                            tc::mma_f16_ts(d, ka + 8 * k, qh + 2 * k, kQk, 1u);
+                        }
+                        tc::mma_commit(&ka_empty[ik % KA]);
+                    }
+                    if (!ok) break;
+                    tc::mma_commit(&s_full[b]);
+                }
+                if (t > 0) {
+                    if (!__all_sync(0xffffffffu, tc::mbar_wait(p_full, (ti + t - 1) & 1, abort_flag, kWaitNs))) break;
+                    for (int c = 0; c < S::kVStages; ++c, ++iv) {
+                        if (!__all_sync(0xffffffffu, tc::mbar_wait(&v_full[iv % VST], (iv / VST) & 1, abort_flag, kWaitNs))) { ok = false; break; }
+                        tc::tc_fence_after();
+                        const uint32_t d = tmem + S::kOCol + (c >> 1) * N;
+                        const uint32_t va = tc::smem_u32(sV) + (iv % VST) * 16384;
+                        const uint32_t pb = tc::smem_u32(sP) + (c & 1) * 64 * 128;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint64_t ad = sdesc_mn(va + k * 2048, 8192);
+                            tc::mma_f16(d, ad, sdesc_mn(pb + 16384 + k * 2048, 8192), kPv, (t > 1 || (c & 1) || k > 0) ? 1u : 0u);
+                            tc::mma_f16(d, ad, sdesc_mn(pb + k * 2048, 8192), kPv, 1u);
+                        }
+                        tc::mma_commit(&v_empty[iv % VST]);
+                    }
+                    if (!ok) break;
+                    tc::mma_commit(p_empty);
+                }
+            }
+            if (*abort_flag) {   // issued MMAs end before tensor memory is released
+                volatile int never = 0;
+                if (ik > 0) tc::mbar_wait(&ka_empty[(ik - 1) % KA], ((ik - 1) / KA) & 1, &never, kWaitNs);
+                if (iv > 0) tc::mbar_wait(&v_empty[(iv - 1) % VST], ((iv - 1) / VST) & 1, &never, kWaitNs);
+            }
+        } else if (warp < 4) {   // ---- softmax: a position per thread
+            const int p = tid;
+            const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * warp) << 16);
+            const uint32_t s0 = a.lo[sg.unit] % a.capacity;
+            const float *ksp = a.ks + static_cast<size_t>(sg.kvh) * a.capacity, *vsp = a.vs + static_cast<size_t>(sg.kvh) * a.capacity;
+            const uint32_t max_lo = __reduce_max_sync(0xffffffffu, max(rlo[lane], rlo[lane + 32]));
+            const uint32_t min_hi = __reduce_min_sync(0xffffffffu, min(rhi[lane], rhi[lane + 32]));
+            float l[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) l[i] = 0.0f;
+            uint32_t slot = ring_tile(0) * TP + p;
+            float ks_next = slot < a.capacity ? __ldg(ksp + slot) : 1.0f, vs_next = slot < a.capacity ? __ldg(vsp + slot) : 1.0f;
+            bool ok = true;
+            for (uint32_t t = 0; t < sg.tiles; ++t) {
+                const uint32_t x = ti + t, b = x & 1;
+                const float ks = ks_next, vs = vs_next, lg = log2f(fmaxf(vs, kKvTiny));
+                const bool in_ring = slot < a.capacity;
+                const uint32_t at = slot - s0 + (slot < s0 ? a.capacity : 0u);   // from the unit's first position
+                if (t + 1 < sg.tiles) {
+                    slot = ring_tile(t + 1) * TP + p;
+                    ks_next = slot < a.capacity ? __ldg(ksp + slot) : 1.0f;
+                    vs_next = slot < a.capacity ? __ldg(vsp + slot) : 1.0f;
+                }
+                const bool all_in = __all_sync(0xffffffffu, in_ring && at >= max_lo && at < min_hi);
+                ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&s_full[b], (x >> 1) & 1, abort_flag, kWaitNs));
+                // the four warps meet in barriers below, so they leave together or not at all
+                if (any_of_128(!ok)) { ok = false; break; }
+                tc::tc_fence_after();
+                const uint32_t sa = lane_addr + S::kSCol + b * N;
+                float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int c0 = 0; c0 < N; c0 += 16) {
+                    uint32_t v[16];
+                    tc::tmem_ld16_sync(sa + c0, v);
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        float s = fmaf(__uint_as_float(v[c]), ks * qf_s[c0 + c], lg);
+                        if (!all_in) s = in_ring && at >= rlo[c0 + c] && at < rhi[c0 + c] ? s : -INFINITY;
+                        const float r = redux_max(s);
+                        if (lane == ((c0 + c) & 31)) top[(c0 + c) >> 5] = r;
+                    }
+                }
+                if (any_of_128(top[0] > m_s[lane] + 8.0f || top[1] > m_s[lane + 32] + 8.0f)) {
+                    wtop[warp * N + lane] = top[0], wtop[warp * N + lane + 32] = top[1];
+                    tc::named_bar_sync(1, 128);
+                    if (tid < N) {
+                        const float old = m_s[tid];
+                        const float now = fmaxf(fmaxf(fmaxf(wtop[tid], wtop[N + tid]), fmaxf(wtop[2 * N + tid], wtop[3 * N + tid])), old);
+                        f_s[tid] = old == now ? 1.0f : ex2(old - now);
+                        m_s[tid] = now;
+                    }
+                    tc::named_bar_sync(1, 128);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) l[i] *= f_s[i];
+                    if (t > 0) {
+                        ok = __all_sync(0xffffffffu, tc::mbar_wait(p_empty, (x & 1) ^ 1, abort_flag, kWaitNs));
+                        tc::tc_fence_after();
+                        for (int c0 = 0; c0 < MT * N; c0 += 16) {
+                            uint32_t v[16];
+                            tc::tmem_ld16_sync(lane_addr + S::kOCol + c0, v);
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * f_s[(c0 & (N - 1)) + c]);
+                            asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                                         :: "r"(lane_addr + S::kOCol + c0), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+                                            "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
+                                            "r"(v[14]), "r"(v[15]) : "memory");
+                        }
+                        tc::tmem_st_wait();
+                    }
+                }
+                ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(p_empty, (x & 1) ^ 1, abort_flag, kWaitNs));
+                uint8_t* prow = sP + p * 128;
+#pragma unroll
+                for (int c0 = 0; c0 < N; c0 += 16) {
+                    uint32_t v[16], hi[8], lo[8];
+                    tc::tmem_ld16_sync(sa + c0, v);
+#pragma unroll
+                    for (int c = 0; c < 16; c += 2) {
+                        float e[2];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const int r = c0 + c + j;
+                            const bool keep = all_in || (in_ring && at >= rlo[r] && at < rhi[r]);
+                            e[j] = ex2(fmaf(__uint_as_float(v[c + j]), ks * qf_s[r], -m_s[r]));
+                            l[r] += keep ? e[j] : 0.0f;
+                            e[j] = keep ? e[j] * vs : 0.0f;
+                        }
+                        hi[c >> 1] = cvt2(e[0], e[1]);
+                        const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&hi[c >> 1]));
+                        lo[c >> 1] = cvt2(e[0] - w.x, e[1] - w.y);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int off = ((c0 / 8 + u) ^ (p & 7)) << 4;
+                        *reinterpret_cast<uint4*>(prow + off) = make_uint4(hi[4 * u], hi[4 * u + 1], hi[4 * u + 2], hi[4 * u + 3]);
+                        *reinterpret_cast<uint4*>(prow + 16384 + off) = make_uint4(lo[4 * u], lo[4 * u + 1], lo[4 * u + 2], lo[4 * u + 3]);
+                    }
+                }
+                tc::tc_fence_before();
+                tc::mbar_arrive(&s_empty[b]);
+                tc::fence_proxy_async_smem();
+                tc::mbar_arrive(p_full);
+            }
+            const uint32_t last = ti + sg.tiles - 1;
+            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(p_empty, last & 1, abort_flag, kWaitNs));
+            ok = !any_of_128(!ok);
+            // ---- the segment's result, merged into what this CTA left in the slot before
+            float2* ml = a.plan.ml + static_cast<size_t>(sg.slot) * N;
+            float* part = a.plan.part + static_cast<size_t>(sg.slot) * N * HD;
+            const bool merge = sg.slot == done_slot;
+            if (ok) {
+                tc::tc_fence_after();
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    float s = l[i];
+                    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                    if (lane == (i & 31)) wtop[warp * N + i] = s;
+                }
+                tc::named_bar_sync(1, 128);
+                if (tid < N) {
+                    float sum = (wtop[tid] + wtop[N + tid]) + (wtop[2 * N + tid] + wtop[3 * N + tid]), m = m_s[tid];
+                    float f = 1.0f, gold = 0.0f;
+                    if (merge) {
+                        const float2 old = ml[tid];
+                        const float now = fmaxf(m, old.x);
+                        f = m == now ? 1.0f : ex2(m - now);
+                        gold = old.x == now ? 1.0f : ex2(old.x - now);
+                        sum = sum * f + old.y * gold;
+                        m = now;
+                    }
+                    ml[tid] = make_float2(m, sum);
+                    f_s[tid] = f * (FMT == GTM_KV_E4M3 ? 256.0f : 1.0f);
+                    g_s[tid] = gold;
+                }
+                tc::named_bar_sync(1, 128);
+                for (int c0 = 0; c0 < MT * N; c0 += 16) {
+                    uint32_t v[16];
+                    tc::tmem_ld16_sync(lane_addr + S::kOCol + c0, v);
+                    float* dst = part + static_cast<size_t>(c0 & (N - 1)) * HD + (c0 / N) * 128 + p;
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        const int r = (c0 & (N - 1)) + c;
+                        const float o = __uint_as_float(v[c]) * f_s[r];
+                        dst[c * HD] = merge ? fmaf(dst[c * HD], g_s[r], o) : o;
+                    }
+                }
+                tc::tc_fence_before();
+            } else if (tid < N) {
+                ml[tid] = make_float2(0.0f, __int_as_float(0x7FC00000));
+            }
+        }
+        kc += sg.tiles * C;
+        vc += sg.tiles * S::kVStages;
+        ti += sg.tiles;
+        done_slot = sg.slot;
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    if (warp == 13) {
+        tc::tmem_relinquish();
+        tc::tmem_dealloc(tmem, 512);
+    }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+int map_codes(CUtensorMap* m, const void* codes, uint64_t width, uint64_t rows, uint32_t box_w, uint32_t box_rows,
+              CUtensorMapSwizzle swizzle) {
+    static EncodeTiledFn encode = nullptr;
+    if (!encode) {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+            return set_error(GTM_ERR_CUDA, "cuTensorMapEncodeTiled not available");
+        encode = reinterpret_cast<EncodeTiledFn>(f);
+    }
+    const cuuint64_t dims[2] = {width, rows}, strides[1] = {width};
+    const cuuint32_t box[2] = {box_w, box_rows}, estr[2] = {1, 1};
+    const CUresult r = encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(GTM_ERR_CUDA, "cuTensorMapEncodeTiled (prefix codes) failed (%d)", (int)r);
+    return GTM_OK;
+}
+
+// A unit's first attended position, its ring tile, and its number of tiles.
+struct UnitSpan {
+    uint32_t lo, first, tiles;
+};
+UnitSpan unit_span(const SharedCall& c, const RowU32& pos, uint32_t unit) {
+    const uint32_t grp = c.q_heads / c.kv_heads, cap = c.prefix->capacity;
+    const uint32_t r0 = unit * N / grp, r1 = std::min(c.n, (unit * N + N + grp - 1) / grp);
+    uint32_t lo = 0xFFFFFFFFu, hi = 0;
+    for (uint32_t i = r0; i < r1; ++i) {
+        const Span s = row_span(pos.v[i], c.window, c.prefix_len);
+        if (s.pn) lo = std::min(lo, s.pa), hi = std::max(hi, s.pa + s.pn);
+    }
+    if (hi == 0) return {0, 0, 0};
+    const uint32_t ring = (cap + TP - 1) / TP, s0 = lo % cap, len = hi - lo;   // len <= capacity
+    const uint64_t end = static_cast<uint64_t>(s0) + len;
+    uint64_t tiles;
+    if (end <= cap)
+        tiles = (end - 1) / TP - s0 / TP + 1;
+    else   // wrapped: to the ring's end, then from its start, no tile twice
+        tiles = std::min<uint64_t>(ring, (ring - s0 / TP) + (end - cap - 1) / TP + 1);
+    return {lo, s0 / TP, static_cast<uint32_t>(tiles)};
+}
+
+template <int HD>
+int launch(const SharedArgs& a, const RowU32& pos, uint32_t fmt, uint32_t ctas, cudaStream_t st) {
+    const auto kernel = fmt == GTM_KV_INT8 ? kv_shared<HD, GTM_KV_INT8> : kv_shared<HD, GTM_KV_E4M3>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<HD>::kSmem);
+    if (e != cudaSuccess) return set_cuda_error("gtm_attention_kv_rows", e);
+    kernel<<<ctas, kThreads, Shape<HD>::kSmem, st>>>(a, pos);
+    return GTM_OK;
+}
+
+}  // namespace
+
+size_t shared_slots(uint32_t q_heads, uint32_t kv_heads, uint32_t n, int num_sms) {
+    const uint64_t units = (static_cast<uint64_t>(n) * (q_heads / kv_heads) + N - 1) / N * kv_heads;
+    return units + num_sms;
+}
+
+void plan_shared(const SharedCall& c, const RowU32& pos, int num_sms, SharedPlan& plan) {
+    plan.units = (c.n * (c.q_heads / c.kv_heads) + N - 1) / N;
+    plan.start[0] = 0;
+    for (uint32_t u = 0; u < plan.units; ++u) plan.start[u + 1] = plan.start[u] + unit_span(c, pos, u).tiles;
+    const uint32_t total = plan.start[plan.units] * c.kv_heads;
+    plan.per = std::max(1u, (total + num_sms - 1) / num_sms);
+}
+
+int launch_shared(const SharedCall& c, const RowU32& pos, const SharedPlan& plan, int num_sms, cudaStream_t st) {
+    SharedArgs a;
+    const GtmKvCache* p = c.prefix;
+    const uint64_t width = static_cast<uint64_t>(c.kv_heads) * c.head_dim;
+    const size_t vec = static_cast<size_t>(c.prefix_seq) * p->capacity * c.kv_heads;
+    int rc = map_codes(&a.k_map, static_cast<const uint8_t*>(p->k_dev) + vec * c.head_dim, width, p->capacity, 64, TP,
+                       CU_TENSOR_MAP_SWIZZLE_64B);
+    if (!rc) rc = map_codes(&a.v_map, static_cast<const uint8_t*>(p->v_dev) + vec * c.head_dim, width, p->capacity, 128, 64,
+                            CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+    a.ks = p->k_scale_dev + vec, a.vs = p->v_scale_dev + vec;
+    a.q = c.q;
+    a.q_heads = c.q_heads, a.kv_heads = c.kv_heads, a.n = c.n, a.grp = c.q_heads / c.kv_heads;
+    a.capacity = p->capacity, a.ring_tiles = (p->capacity + TP - 1) / TP;
+    a.window = c.window, a.prefix_len = c.prefix_len;
+    a.total = plan.start[plan.units] * c.kv_heads;
+    for (uint32_t u = 0; u < plan.units; ++u) {
+        const UnitSpan s = unit_span(c, pos, u);
+        a.lo[u] = s.lo, a.first[u] = s.first;
+    }
+    a.plan = plan;
+    const uint32_t ctas = (a.total + plan.per - 1) / plan.per;
+    if (c.head_dim == 128) return launch<128>(a, pos, p->format, ctas, st);
+    if (c.head_dim == 256) return launch<256>(a, pos, p->format, ctas, st);
+    return launch<512>(a, pos, p->format, ctas, st);
+}
+
+}  // namespace gtm
