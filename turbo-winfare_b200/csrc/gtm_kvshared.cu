@@ -13,11 +13,20 @@
 // for), so O is rarely rescaled. Tiles follow ring slots, not positions: softmax does not mind the
 // order, no tile wraps, and each row's span is a mask on the slot's position.
 //
+// A tensor core's addition to its accumulator is cut to fp32, not rounded, which biases a long sum by
+// up to 2^-24 of it per instruction. So a score's limbs are summed apart (HD / 16 instructions each),
+// and O goes to memory after kLongest tiles (16 instructions each), where results are added in fp32.
+//
+// The issue order is PV of tile i and QK of tile i + 2 in turn, 64 dims at a time, while the softmax
+// warps work on tile i + 1: K and V are converted side by side at an even pace. PV takes a tile's
+// positions in two halves, so that one half of p is written while the other is read.
+//
 // The work is the flat list of (kv head, unit, tile), cut into equal runs, one per CTA; a CTA leaves a
 // partial result for each unit it touches.
 //
-// Roles: warps 0-3 softmax and O; 4-7 K; 8-11 V; 12 and 14 TMA loads of K and V codes; 13 MMA. Every
-// wait is bounded (1 s); one that runs out stops the CTA and marks its results NaN.
+// Roles: warps 0-7 softmax and O (32 of the 64 columns each half of them); 8-11 K; 12-13 V; 14 TMA
+// loads of K and V codes, in the issue order; 15 MMA. Every wait is bounded (1 s); one that runs out stops the CTA
+// and marks its results NaN.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -32,10 +41,10 @@ namespace {
 
 constexpr int N = kSharedRows;
 constexpr int TP = 128;              // positions of a tile
-constexpr int kThreads = 480;
+constexpr int kThreads = 512;
 constexpr uint64_t kWaitNs = 1000000000ull;
 constexpr int KA = 4;                // K chunks (64 dims) in tensor memory
-constexpr uint32_t kLongest = 32;    // tiles summed in tensor memory before the result goes to memory
+constexpr uint32_t kLongest = 16;    // tiles summed in tensor memory before the result goes to memory
 
 template <int HD>
 struct Shape {
@@ -43,7 +52,7 @@ struct Shape {
     static constexpr int kVStages = HD / 64;     // V stages of a tile: 128 dims x 64 positions
     static constexpr int RK = HD == 512 ? 2 : 4, RV = HD == 512 ? 2 : 4, VST = HD == 512 ? 2 : 4;
     static constexpr int kQ = 2 * kChunks * 8192, kP = 2 * 16384, kV = VST * 16384, kRawK = RK * 8192, kRawV = RV * 8192;
-    static constexpr int kBars = 2 * RK + 2 * RV + 2 * KA + 2 * VST + 4 + 2;
+    static constexpr int kBars = 2 * RK + 2 * RV + 2 * KA + 2 * VST + 2 + 4;
     static constexpr int kSmall = (4 * N + 4 * N + 2 * N) * 4 + kBars * 8 + 16;
     static constexpr int kSmem = kQ + kP + kV + kRawK + kRawV + kSmall;
     static constexpr uint32_t kOCol = 0, kSCol = HD / 128 * N, kACol = kSCol + 2 * N;   // tensor memory columns
@@ -65,12 +74,17 @@ __device__ __forceinline__ float redux_max(float x) {
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
     return r;
 }
-// Whether any of the 128 softmax threads says so (hardware barrier 1).
-__device__ __forceinline__ bool any_of_128(bool x) {
+// Whether any of a softmax group's 128 threads says so (hardware barrier 1 or 2).
+__device__ __forceinline__ bool any_of_128(uint32_t bar, bool x) {
     uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                 : "=r"(r) : "r"(x ? 1u : 0u) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"(x ? 1u : 0u), "r"(bar) : "memory");
     return r != 0;
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 :: "r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+                    "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
 }
 // Operand whose M or N side is contiguous: rows (K) of 64 fp16, 8-row atoms of 1,024 bytes in the
 // 128-byte swizzle; `block` bytes to the next 64 of M or N.
@@ -135,22 +149,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(rhi + N);
     uint64_t *rk_full = bars, *rk_empty = rk_full + RK, *rv_full = rk_empty + RK, *rv_empty = rv_full + RV,
              *ka_full = rv_empty + RV, *ka_empty = ka_full + KA, *v_full = ka_empty + KA, *v_empty = v_full + VST,
-             *s_full = v_empty + VST, *s_empty = s_full + 2, *p_full = s_empty + 2, *p_empty = p_full + 1;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_empty + 1);
+             *s_full = v_empty + VST, *s_empty = s_full + 1, *p_full = s_empty + 1, *p_empty = p_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_empty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < RK; ++i) tc::mbar_init(&rk_full[i], 1), tc::mbar_init(&rk_empty[i], 128);
-        for (int i = 0; i < RV; ++i) tc::mbar_init(&rv_full[i], 1), tc::mbar_init(&rv_empty[i], 128);
+        for (int i = 0; i < RV; ++i) tc::mbar_init(&rv_full[i], 1), tc::mbar_init(&rv_empty[i], 64);
         for (int i = 0; i < KA; ++i) tc::mbar_init(&ka_full[i], 128), tc::mbar_init(&ka_empty[i], 1);
-        for (int i = 0; i < VST; ++i) tc::mbar_init(&v_full[i], 128), tc::mbar_init(&v_empty[i], 1);
-        for (int i = 0; i < 2; ++i) tc::mbar_init(&s_full[i], 1), tc::mbar_init(&s_empty[i], 128);
-        tc::mbar_init(p_full, 128), tc::mbar_init(p_empty, 1);
+        for (int i = 0; i < VST; ++i) tc::mbar_init(&v_full[i], 64), tc::mbar_init(&v_empty[i], 1);
+        tc::mbar_init(s_full, 1), tc::mbar_init(s_empty, 256);
+        for (int i = 0; i < 2; ++i) tc::mbar_init(&p_full[i], 128), tc::mbar_init(&p_empty[i], 1);   // a half of the positions
         *abort_flag = (tc::smem_u32(smem) & 1023u) ? 1 : 0;   // the swizzled layouts need it
         tc::mbar_fence_init();
     }
-    if (warp == 13) tc::tmem_alloc(tmem_slot, 512);
+    if (warp == 15) tc::tmem_alloc(tmem_slot, 512);
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
@@ -215,42 +229,42 @@ __global__ void __launch_bounds__(kThreads, 1)
             return b >= a.ring_tiles ? b - a.ring_tiles : b;
         };
 
-        if (warp == 12) {   // ---- K codes
+        if (warp == 14) {   // ---- K and V codes, in the order in which they are multiplied
             if (lane == 0) {
-                uint32_t it = kc;
-                for (uint32_t t = 0; t < sg.tiles; ++t) {
-                    const int y = static_cast<int>(ring_tile(t) * TP);
-                    for (int c = 0; c < C; ++c, ++it) {
-                        if (!tc::mbar_wait(&rk_empty[it % RK], ((it / RK) & 1) ^ 1, abort_flag, kWaitNs)) goto k_out;
-                        tc::mbar_arrive_expect_tx(&rk_full[it % RK], 8192);
-                        tc::tma_load_2d(sRawK + (it % RK) * 8192, &a.k_map, static_cast<int>(sg.kvh * HD + c * 64), y, &rk_full[it % RK]);
+                uint32_t ik = kc, iv = vc;
+                bool ok = true;
+                auto load_k = [&](uint32_t t, int c) {
+                    uint64_t* full = &rk_full[ik % RK];
+                    ok = ok && tc::mbar_wait(&rk_empty[ik % RK], ((ik / RK) & 1) ^ 1, abort_flag, kWaitNs);
+                    if (!ok) return;
+                    tc::mbar_arrive_expect_tx(full, 8192);
+                    tc::tma_load_2d(sRawK + (ik % RK) * 8192, &a.k_map, static_cast<int>(sg.kvh * HD + c * 64),
+                                    static_cast<int>(ring_tile(t) * TP), full);
+                    ++ik;
+                };
+                auto load_v = [&](uint32_t t, int c) {
+                    uint64_t* full = &rv_full[iv % RV];
+                    ok = ok && tc::mbar_wait(&rv_empty[iv % RV], ((iv / RV) & 1) ^ 1, abort_flag, kWaitNs);
+                    if (!ok) return;
+                    tc::mbar_arrive_expect_tx(full, 8192);
+                    tc::tma_load_2d(sRawV + (iv % RV) * 8192, &a.v_map, static_cast<int>(sg.kvh * HD + (c % MT) * 128),
+                                    static_cast<int>(ring_tile(t) * TP) + (c / MT) * 64, full);
+                    ++iv;
+                };
+                for (uint32_t t = 0; t < 2 && t < sg.tiles; ++t)
+                    for (int c = 0; c < C && ok; ++c) load_k(t, c);
+                for (uint32_t t = 0; t < sg.tiles && ok; ++t)
+                    for (int c = 0; c < C && ok; ++c) {
+                        load_v(t, c);
+                        if (t + 2 < sg.tiles) load_k(t + 2, c);
                     }
-                }
-            k_out:
                 if (*abort_flag) {   // no exit while copies into this CTA's shared memory are in flight
                     volatile int never = 0;
-                    for (uint32_t j = it > RK ? it - RK : 0; j < it; ++j) tc::mbar_wait(&rk_full[j % RK], (j / RK) & 1, &never, kWaitNs);
+                    for (uint32_t j = ik > RK ? ik - RK : 0; j < ik; ++j) tc::mbar_wait(&rk_full[j % RK], (j / RK) & 1, &never, kWaitNs);
+                    for (uint32_t j = iv > RV ? iv - RV : 0; j < iv; ++j) tc::mbar_wait(&rv_full[j % RV], (j / RV) & 1, &never, kWaitNs);
                 }
             }
-        } else if (warp == 14) {   // ---- V codes
-            if (lane == 0) {
-                uint32_t it = vc;
-                for (uint32_t t = 0; t < sg.tiles; ++t) {
-                    const int y = static_cast<int>(ring_tile(t) * TP);
-                    for (int c = 0; c < S::kVStages; ++c, ++it) {
-                        if (!tc::mbar_wait(&rv_empty[it % RV], ((it / RV) & 1) ^ 1, abort_flag, kWaitNs)) goto v_out;
-                        tc::mbar_arrive_expect_tx(&rv_full[it % RV], 8192);
-                        tc::tma_load_2d(sRawV + (it % RV) * 8192, &a.v_map, static_cast<int>(sg.kvh * HD + (c >> 1) * 128), y + (c & 1) * 64,
-                                        &rv_full[it % RV]);
-                    }
-                }
-            v_out:
-                if (*abort_flag) {
-                    volatile int never = 0;
-                    for (uint32_t j = it > RV ? it - RV : 0; j < it; ++j) tc::mbar_wait(&rv_full[j % RV], (j / RV) & 1, &never, kWaitNs);
-                }
-            }
-        } else if (warp >= 4 && warp < 8) {   // ---- K: codes to fp16 in tensor memory, a position per lane
+        } else if (warp >= 8 && warp < 12) {   // ---- K: codes to fp16 in tensor memory, a position per lane
             const int p = 32 * (warp & 3) + lane;
             const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + S::kACol;
             uint32_t it = kc;
@@ -275,95 +289,106 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc::mbar_arrive(&ka_full[it % KA]);
                 tc::mbar_arrive(&rk_empty[it % RK]);   // only after the words were used (see gtm_tokens.cu)
             }
-        } else if (warp >= 8 && warp < 12) {   // ---- V: codes to fp16 in shared memory, dims contiguous
-            const int p = (tid - 256) & 63, half = (tid - 256) >> 6;
+        } else if (warp == 12 || warp == 13) {   // ---- V: codes to fp16 in shared memory, dims contiguous
+            const int p = tid - 384;
             uint32_t it = vc;
             const uint32_t end = vc + sg.tiles * S::kVStages;
             for (; it < end; ++it) {
                 if (!__all_sync(0xffffffffu, tc::mbar_wait(&rv_full[it % RV], (it / RV) & 1, abort_flag, kWaitNs))) break;
                 const uint8_t* raw = sRawV + (it % RV) * 8192 + p * 128;
-                uint4 w[4];
+                uint4 w[8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4*>(raw + (((half * 4 + j) ^ (p & 7)) << 4));
+                for (int j = 0; j < 8; ++j) w[j] = *reinterpret_cast<const uint4*>(raw + ((j ^ (p & 7)) << 4));
                 if (!__all_sync(0xffffffffu, tc::mbar_wait(&v_empty[it % VST], ((it / VST) & 1) ^ 1, abort_flag, kWaitNs))) break;
-                uint8_t* dst = sV + (it % VST) * 16384 + half * 8192 + p * 128;
+                uint8_t* dst = sV + (it % VST) * 16384 + p * 128;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < 8; ++j) {
                     uint32_t h[8];
                     widen<FMT>(w[j], h);
-                    *reinterpret_cast<uint4*>(dst + (((2 * j) ^ (p & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4*>(dst + (((2 * j + 1) ^ (p & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+                    uint8_t* d = dst + (j >> 2) * 8192;
+                    *reinterpret_cast<uint4*>(d + (((2 * (j & 3)) ^ (p & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4*>(d + (((2 * (j & 3) + 1) ^ (p & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
                 }
                 tc::fence_proxy_async_smem();
                 tc::mbar_arrive(&v_full[it % VST]);
                 tc::mbar_arrive(&rv_empty[it % RV]);
             }
-        } else if (warp == 13) {   // ---- MMA issue (the whole warp; one elected lane issues)
+        } else if (warp == 15) {   // ---- MMA issue (the whole warp; one elected lane issues)
             constexpr uint32_t kQk = tc::idesc_f16(128, N);
             constexpr uint32_t kPv = tc::idesc_f16(128, N) | (1u << 15) | (1u << 16);   // both operands M/N-contiguous
+            const uint32_t qa = tc::smem_u32(sQ), va0 = tc::smem_u32(sV), pa = tc::smem_u32(sP);
             uint32_t ik = kc, iv = vc;
             bool ok = true;
-            for (uint32_t t = 0; t <= sg.tiles && ok; ++t) {
-                if (t < sg.tiles) {
-                    const uint32_t x = ti + t, b = x & 1;
-                    if (!__all_sync(0xffffffffu, tc::mbar_wait(&s_empty[b], ((x >> 1) & 1) ^ 1, abort_flag, kWaitNs))) break;
-                    const uint32_t d = tmem + S::kSCol + b * N;
-                    for (int c = 0; c < C; ++c, ++ik) {
-                        if (!__all_sync(0xffffffffu, tc::mbar_wait(&ka_full[ik % KA], (ik / KA) & 1, abort_flag, kWaitNs))) { ok = false; break; }
-                        tc::tc_fence_after();
-                        const uint32_t ka = tmem + S::kACol + (ik % KA) * 32;
-                        const uint64_t qh = tc::sdesc_sw128(tc::smem_u32(sQ) + c * 8192);
-                        const uint64_t ql = tc::sdesc_sw128(tc::smem_u32(sQ) + (C + c) * 8192);
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_flag, kWaitNs));
+                return ok;
+            };
+            // chunk c of S of tile t (of the segment)
+            auto qk = [&](uint32_t t, int c) {
+                if (c == 0 && !wait(s_empty, ((ti + t) & 1) ^ 1)) return;
+                if (!wait(&ka_full[ik % KA], (ik / KA) & 1)) return;
+                tc::tc_fence_after();
+                const uint32_t ka = tmem + S::kACol + (ik % KA) * 32, d = tmem + S::kSCol;
+                const uint64_t qh = tc::sdesc_sw128(qa + c * 8192), ql = tc::sdesc_sw128(qa + (C + c) * 8192);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            tc::mma_f16_ts(d, ka + 8 * k, ql + 2 * k, kQk, (c > 0 || k > 0) ? 1u : 0u);
-                            tc::mma_f16_ts(d, ka + 8 * k, qh + 2 * k, kQk, 1u);
-                        }
-                        tc::mma_commit(&ka_empty[ik % KA]);
-                    }
-                    if (!ok) break;
-                    tc::mma_commit(&s_full[b]);
+                for (int k = 0; k < 4; ++k) {
+                    tc::mma_f16_ts(d, ka + 8 * k, qh + 2 * k, kQk, (c > 0 || k > 0) ? 1u : 0u);
+                    tc::mma_f16_ts(d + N, ka + 8 * k, ql + 2 * k, kQk, (c > 0 || k > 0) ? 1u : 0u);
                 }
-                if (t > 0) {
-                    if (!__all_sync(0xffffffffu, tc::mbar_wait(p_full, (ti + t - 1) & 1, abort_flag, kWaitNs))) break;
-                    for (int c = 0; c < S::kVStages; ++c, ++iv) {
-                        if (!__all_sync(0xffffffffu, tc::mbar_wait(&v_full[iv % VST], (iv / VST) & 1, abort_flag, kWaitNs))) { ok = false; break; }
-                        tc::tc_fence_after();
-                        const uint32_t d = tmem + S::kOCol + (c >> 1) * N;
-                        const uint32_t va = tc::smem_u32(sV) + (iv % VST) * 16384;
-                        const uint32_t pb = tc::smem_u32(sP) + (c & 1) * 64 * 128;
+                tc::mma_commit(&ka_empty[ik % KA]);
+                ++ik;
+                if (c == C - 1) tc::mma_commit(s_full);
+            };
+            // stage c of O of tile t: 128 dims c % MT, positions' half c / MT
+            auto pv = [&](uint32_t t, int c) {
+                const int half = c / MT, mt = c % MT;
+                if (mt == 0 && !wait(&p_full[half], (ti + t) & 1)) return;
+                if (!wait(&v_full[iv % VST], (iv / VST) & 1)) return;
+                tc::tc_fence_after();
+                const uint32_t d = tmem + S::kOCol + mt * N, va = va0 + (iv % VST) * 16384, pb = pa + half * 64 * 128;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint64_t ad = sdesc_mn(va + k * 2048, 8192);
-                            tc::mma_f16(d, ad, sdesc_mn(pb + 16384 + k * 2048, 8192), kPv, (t > 1 || (c & 1) || k > 0) ? 1u : 0u);
-                            tc::mma_f16(d, ad, sdesc_mn(pb + k * 2048, 8192), kPv, 1u);
-                        }
-                        tc::mma_commit(&v_empty[iv % VST]);
-                    }
-                    if (!ok) break;
-                    tc::mma_commit(p_empty);
+                for (int k = 0; k < 4; ++k) {
+                    const uint64_t ad = sdesc_mn(va + k * 2048, 8192);
+                    tc::mma_f16(d, ad, sdesc_mn(pb + 16384 + k * 2048, 8192), kPv, (t > 0 || half || k > 0) ? 1u : 0u);
+                    tc::mma_f16(d, ad, sdesc_mn(pb + k * 2048, 8192), kPv, 1u);
                 }
-            }
+                tc::mma_commit(&v_empty[iv % VST]);
+                ++iv;
+                if (mt == MT - 1) tc::mma_commit(&p_empty[half]);
+            };
+            for (uint32_t t = 0; t < 2 && t < sg.tiles; ++t)
+                for (int c = 0; c < C && ok; ++c) qk(t, c);
+            for (uint32_t t = 0; t < sg.tiles && ok; ++t)
+                for (int c = 0; c < C && ok; ++c) {
+                    pv(t, c);
+                    if (ok && t + 2 < sg.tiles) qk(t + 2, c);
+                }
             if (*abort_flag) {   // issued MMAs end before tensor memory is released
                 volatile int never = 0;
                 if (ik > 0) tc::mbar_wait(&ka_empty[(ik - 1) % KA], ((ik - 1) / KA) & 1, &never, kWaitNs);
                 if (iv > 0) tc::mbar_wait(&v_empty[(iv - 1) % VST], ((iv - 1) / VST) & 1, &never, kWaitNs);
             }
-        } else if (warp < 4) {   // ---- softmax: a position per thread
-            const int p = tid;
-            const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * warp) << 16);
+        } else if (warp < 8) {   // ---- softmax: a position and 32 columns per thread
+            constexpr int H = N / 2;
+            const int p = tid & 127, grp = warp >> 2, half = p >> 6;
+            const int col0 = grp * H;   // the group's columns
+            const uint32_t bar = 1 + grp;
+            const uint32_t lane_addr = (tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16)) + col0;
+            float *tops = wtop + (warp & 3) * N + col0, *m_c = m_s + col0, *f_c = f_s + col0;
+            const float* qf_c = qf_s + col0;
+            const uint32_t *rlo_c = rlo + col0, *rhi_c = rhi + col0;
             const uint32_t s0 = a.lo[sg.unit] % a.capacity;
             const float *ksp = a.ks + static_cast<size_t>(sg.kvh) * a.capacity, *vsp = a.vs + static_cast<size_t>(sg.kvh) * a.capacity;
-            const uint32_t max_lo = __reduce_max_sync(0xffffffffu, max(rlo[lane], rlo[lane + 32]));
-            const uint32_t min_hi = __reduce_min_sync(0xffffffffu, min(rhi[lane], rhi[lane + 32]));
-            float l[N];
+            const uint32_t max_lo = __reduce_max_sync(0xffffffffu, rlo_c[lane]);
+            const uint32_t min_hi = __reduce_min_sync(0xffffffffu, rhi_c[lane]);
+            float l[H];
 #pragma unroll
-            for (int i = 0; i < N; ++i) l[i] = 0.0f;
+            for (int i = 0; i < H; ++i) l[i] = 0.0f;
             uint32_t slot = ring_tile(0) * TP + p;
             float ks_next = slot < a.capacity ? __ldg(ksp + slot) : 1.0f, vs_next = slot < a.capacity ? __ldg(vsp + slot) : 1.0f;
             bool ok = true;
             for (uint32_t t = 0; t < sg.tiles; ++t) {
-                const uint32_t x = ti + t, b = x & 1;
+                const uint32_t x = ti + t;
                 const float ks = ks_next, vs = vs_next, lg = log2f(fmaxf(vs, kKvTiny));
                 const bool in_ring = slot < a.capacity;
                 const uint32_t at = slot - s0 + (slot < s0 ? a.capacity : 0u);   // from the unit's first position
@@ -373,131 +398,133 @@ __global__ void __launch_bounds__(kThreads, 1)
                     vs_next = slot < a.capacity ? __ldg(vsp + slot) : 1.0f;
                 }
                 const bool all_in = __all_sync(0xffffffffu, in_ring && at >= max_lo && at < min_hi);
-                ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&s_full[b], (x >> 1) & 1, abort_flag, kWaitNs));
-                // the four warps meet in barriers below, so they leave together or not at all
-                if (any_of_128(!ok)) { ok = false; break; }
+                ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(s_full, x & 1, abort_flag, kWaitNs));
+                // the group's warps meet in barriers below, so they leave together or not at all
+                if (any_of_128(bar, !ok)) { ok = false; break; }
                 tc::tc_fence_after();
-                const uint32_t sa = lane_addr + S::kSCol + b * N;
-                float top[2] = {-INFINITY, -INFINITY};
+                float s[H], top = -INFINITY;
 #pragma unroll
-                for (int c0 = 0; c0 < N; c0 += 16) {
-                    uint32_t v[16];
-                    tc::tmem_ld16_sync(sa + c0, v);
+                for (int c0 = 0; c0 < H; c0 += 16) {
+                    uint32_t v[16], w[16];
+                    tc::tmem_ld16_sync(lane_addr + S::kSCol + c0, v);
+                    tc::tmem_ld16_sync(lane_addr + S::kSCol + N + c0, w);
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) {
-                        float s = fmaf(__uint_as_float(v[c]), ks * qf_s[c0 + c], lg);
-                        if (!all_in) s = in_ring && at >= rlo[c0 + c] && at < rhi[c0 + c] ? s : -INFINITY;
-                        const float r = redux_max(s);
-                        if (lane == ((c0 + c) & 31)) top[(c0 + c) >> 5] = r;
-                    }
-                }
-                if (any_of_128(top[0] > m_s[lane] + 8.0f || top[1] > m_s[lane + 32] + 8.0f)) {
-                    wtop[warp * N + lane] = top[0], wtop[warp * N + lane + 32] = top[1];
-                    tc::named_bar_sync(1, 128);
-                    if (tid < N) {
-                        const float old = m_s[tid];
-                        const float now = fmaxf(fmaxf(fmaxf(wtop[tid], wtop[N + tid]), fmaxf(wtop[2 * N + tid], wtop[3 * N + tid])), old);
-                        f_s[tid] = old == now ? 1.0f : ex2(old - now);
-                        m_s[tid] = now;
-                    }
-                    tc::named_bar_sync(1, 128);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) l[i] *= f_s[i];
-                    if (t > 0) {
-                        ok = __all_sync(0xffffffffu, tc::mbar_wait(p_empty, (x & 1) ^ 1, abort_flag, kWaitNs));
-                        tc::tc_fence_after();
-                        for (int c0 = 0; c0 < MT * N; c0 += 16) {
-                            uint32_t v[16];
-                            tc::tmem_ld16_sync(lane_addr + S::kOCol + c0, v);
-#pragma unroll
-                            for (int c = 0; c < 16; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * f_s[(c0 & (N - 1)) + c]);
-                            asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-                                         :: "r"(lane_addr + S::kOCol + c0), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
-                                            "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
-                                            "r"(v[14]), "r"(v[15]) : "memory");
-                        }
-                        tc::tmem_st_wait();
-                    }
-                }
-                ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(p_empty, (x & 1) ^ 1, abort_flag, kWaitNs));
-                uint8_t* prow = sP + p * 128;
-#pragma unroll
-                for (int c0 = 0; c0 < N; c0 += 16) {
-                    uint32_t v[16], hi[8], lo[8];
-                    tc::tmem_ld16_sync(sa + c0, v);
-#pragma unroll
-                    for (int c = 0; c < 16; c += 2) {
-                        float e[2];
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const int r = c0 + c + j;
-                            const bool keep = all_in || (in_ring && at >= rlo[r] && at < rhi[r]);
-                            e[j] = ex2(fmaf(__uint_as_float(v[c + j]), ks * qf_s[r], -m_s[r]));
-                            l[r] += keep ? e[j] : 0.0f;
-                            e[j] = keep ? e[j] * vs : 0.0f;
-                        }
-                        hi[c >> 1] = cvt2(e[0], e[1]);
-                        const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&hi[c >> 1]));
-                        lo[c >> 1] = cvt2(e[0] - w.x, e[1] - w.y);
-                    }
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const int off = ((c0 / 8 + u) ^ (p & 7)) << 4;
-                        *reinterpret_cast<uint4*>(prow + off) = make_uint4(hi[4 * u], hi[4 * u + 1], hi[4 * u + 2], hi[4 * u + 3]);
-                        *reinterpret_cast<uint4*>(prow + 16384 + off) = make_uint4(lo[4 * u], lo[4 * u + 1], lo[4 * u + 2], lo[4 * u + 3]);
-                    }
+                    for (int c = 0; c < 16; ++c) s[c0 + c] = __uint_as_float(v[c]) + __uint_as_float(w[c]);
                 }
                 tc::tc_fence_before();
-                tc::mbar_arrive(&s_empty[b]);
+                tc::mbar_arrive(s_empty);
+#pragma unroll
+                for (int c = 0; c < H; ++c) {
+                    s[c] *= ks * qf_c[c];
+                    if (!all_in) s[c] = in_ring && at >= rlo_c[c] && at < rhi_c[c] ? s[c] : -INFINITY;
+                    const float r = redux_max(s[c] + lg);
+                    if (lane == c) top = r;
+                }
+                if (any_of_128(bar, top > m_c[lane] + 8.0f)) {
+                    tops[lane] = top;
+                    tc::named_bar_sync(bar, 128);
+                    if (p < H) {
+                        const float* w = wtop + col0 + p;
+                        const float old = m_c[p], now = fmaxf(fmaxf(fmaxf(w[0], w[N]), fmaxf(w[2 * N], w[3 * N])), old);
+                        f_c[p] = old == now ? 1.0f : ex2(old - now);
+                        m_c[p] = now;
+                    }
+                    tc::named_bar_sync(bar, 128);
+#pragma unroll
+                    for (int i = 0; i < H; ++i) l[i] *= f_c[i];
+                    if (t > 0) {
+                        ok = __all_sync(0xffffffffu, tc::mbar_wait(&p_empty[1], (x & 1) ^ 1, abort_flag, kWaitNs));
+                        tc::tc_fence_after();
+                        for (int c0 = 0; c0 < MT * 2; ++c0) {
+                            uint32_t v[16];
+                            const uint32_t addr = lane_addr + S::kOCol + (c0 >> 1) * N + (c0 & 1) * 16;
+                            tc::tmem_ld16_sync(addr, v);
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * f_c[(c0 & 1) * 16 + c]);
+                            tmem_st16(addr, v);
+                        }
+                        tc::tmem_st_wait();
+                        tc::tc_fence_before();
+                    }
+                }
+                uint32_t hi[H / 2], lo[H / 2];
+#pragma unroll
+                for (int c = 0; c < H; c += 2) {
+                    float e[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        // a masked score is -infinity, and so may its column's m be; a NaN goes through
+                        e[j] = ex2(s[c + j] - m_c[c + j]);
+                        if (!all_in) e[j] = s[c + j] == -INFINITY ? 0.0f : e[j];
+                        l[c + j] += e[j];
+                        e[j] = !all_in && s[c + j] == -INFINITY ? 0.0f : e[j] * vs;
+                    }
+                    hi[c >> 1] = cvt2(e[0], e[1]);
+                    const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&hi[c >> 1]));
+                    lo[c >> 1] = cvt2(e[0] - w.x, e[1] - w.y);
+                }
+                ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&p_empty[half], (x & 1) ^ 1, abort_flag, kWaitNs));
+                uint8_t* prow = sP + p * 128;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int off = ((col0 / 8 + u) ^ (p & 7)) << 4;
+                    *reinterpret_cast<uint4*>(prow + off) = make_uint4(hi[4 * u], hi[4 * u + 1], hi[4 * u + 2], hi[4 * u + 3]);
+                    *reinterpret_cast<uint4*>(prow + 16384 + off) = make_uint4(lo[4 * u], lo[4 * u + 1], lo[4 * u + 2], lo[4 * u + 3]);
+                }
                 tc::fence_proxy_async_smem();
-                tc::mbar_arrive(p_full);
+                tc::mbar_arrive(&p_full[half]);
             }
             const uint32_t last = ti + sg.tiles - 1;
-            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(p_empty, last & 1, abort_flag, kWaitNs));
-            ok = !any_of_128(!ok);
+            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&p_empty[1], last & 1, abort_flag, kWaitNs));
+            ok = !any_of_128(bar, !ok);
             // ---- the segment's result, merged into what this CTA left in the slot before
-            float2* ml = a.plan.ml + static_cast<size_t>(sg.slot) * N;
-            float* part = a.plan.part + static_cast<size_t>(sg.slot) * N * HD;
+            float2* ml = a.plan.ml + static_cast<size_t>(sg.slot) * N + col0;
+            float* part = a.plan.part + (static_cast<size_t>(sg.slot) * N + col0) * HD;
             const bool merge = sg.slot == done_slot;
             if (ok) {
                 tc::tc_fence_after();
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    float s = l[i];
-                    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                    if (lane == (i & 31)) wtop[warp * N + i] = s;
+                for (int i = 0; i < H; ++i) {
+                    float sum = l[i];
+                    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (lane == i) tops[i] = sum;
                 }
-                tc::named_bar_sync(1, 128);
-                if (tid < N) {
-                    float sum = (wtop[tid] + wtop[N + tid]) + (wtop[2 * N + tid] + wtop[3 * N + tid]), m = m_s[tid];
-                    float f = 1.0f, gold = 0.0f;
+                tc::named_bar_sync(bar, 128);
+                if (p < H) {
+                    const float* w = wtop + col0 + p;
+                    float sum = (w[0] + w[N]) + (w[2 * N] + w[3 * N]), m = m_c[p], f = 1.0f, gold = 0.0f;
                     if (merge) {
-                        const float2 old = ml[tid];
+                        const float2 old = ml[p];
                         const float now = fmaxf(m, old.x);
                         f = m == now ? 1.0f : ex2(m - now);
                         gold = old.x == now ? 1.0f : ex2(old.x - now);
                         sum = sum * f + old.y * gold;
                         m = now;
                     }
-                    ml[tid] = make_float2(m, sum);
-                    f_s[tid] = f * (FMT == GTM_KV_E4M3 ? 256.0f : 1.0f);
-                    g_s[tid] = gold;
+                    ml[p] = make_float2(m, sum);
+                    f_c[p] = f * (FMT == GTM_KV_E4M3 ? 256.0f : 1.0f);
+                    g_s[col0 + p] = gold;
                 }
-                tc::named_bar_sync(1, 128);
-                for (int c0 = 0; c0 < MT * N; c0 += 16) {
+                tc::named_bar_sync(bar, 128);
+                for (int c0 = 0; c0 < MT * 2; ++c0) {
                     uint32_t v[16];
-                    tc::tmem_ld16_sync(lane_addr + S::kOCol + c0, v);
-                    float* dst = part + static_cast<size_t>(c0 & (N - 1)) * HD + (c0 / N) * 128 + p;
+                    const int r0 = (c0 & 1) * 16;
+                    tc::tmem_ld16_sync(lane_addr + S::kOCol + (c0 >> 1) * N + r0, v);
+                    float* dst = part + static_cast<size_t>(r0) * HD + (c0 >> 1) * 128 + p;
+                    float old[16];
+                    if (merge) {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) old[c] = dst[c * HD];
+                    }
 #pragma unroll
                     for (int c = 0; c < 16; ++c) {
-                        const int r = (c0 & (N - 1)) + c;
-                        const float o = __uint_as_float(v[c]) * f_s[r];
-                        dst[c * HD] = merge ? fmaf(dst[c * HD], g_s[r], o) : o;
+                        const float o = __uint_as_float(v[c]) * f_c[r0 + c];
+                        dst[c * HD] = merge ? fmaf(old[c], g_s[col0 + r0 + c], o) : o;
                     }
                 }
                 tc::tc_fence_before();
-            } else if (tid < N) {
-                ml[tid] = make_float2(0.0f, __int_as_float(0x7FC00000));
+            } else if (p < H) {
+                ml[p] = make_float2(0.0f, __int_as_float(0x7FC00000));
             }
         }
         kc += sg.tiles * C;
@@ -507,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc::tc_fence_before();
     __syncthreads();
-    if (warp == 13) {
+    if (warp == 15) {
         tc::tmem_relinquish();
         tc::tmem_dealloc(tmem, 512);
     }
