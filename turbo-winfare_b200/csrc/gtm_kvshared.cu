@@ -55,7 +55,11 @@ struct Shape {
     static constexpr int kBars = 2 * RK + 2 * RV + 2 * KA + 2 * VST + 2 + 4;
     static constexpr int kSmall = (4 * N + 4 * N + 2 * N) * 4 + kBars * 8 + 16;
     static constexpr int kSmem = kQ + kP + kV + kRawK + kRawV + kSmall;
-    static constexpr uint32_t kOCol = 0, kSCol = HD / 128 * N, kACol = kSCol + 2 * N;   // tensor memory columns
+    // tensor memory columns. An MMA of N <= 128 takes the time of N = 128, so a limb pair goes in one
+    // where there is room for two results: always for S, for O up to 256 dims.
+    static constexpr bool kPairO = HD <= 256;
+    static constexpr uint32_t kOWidth = kPairO ? 2 * N : N;
+    static constexpr uint32_t kOCol = 0, kSCol = HD / 128 * kOWidth, kACol = kSCol + 2 * N;
     static_assert(kACol + KA * 32 <= 512, "tensor memory");
     static_assert(kSmem <= 232448, "shared memory");
 };
@@ -134,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     using S = Shape<HD>;
     constexpr int RK = S::RK, RV = S::RV, VST = S::VST, C = S::kChunks, MT = HD / 128;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t* sQ = smem;                    // [limb][chunk][64 rows][128 B]
+    uint8_t* sQ = smem;                    // [chunk][limb][64 rows][128 B]
     uint8_t* sP = sQ + S::kQ;              // [limb][128 positions][128 B]
     uint8_t* sV = sP + S::kP;              // [stage][dims 0-63, 64-127][64 positions][128 B]
     uint8_t* sRawK = sV + S::kV;           // [stage][128 positions][64 B], 64-byte swizzle
@@ -168,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __reduce_or_sync(0xffffffffu, *tmem_slot);   // in a uniform register, as MMA operands are
 
     const uint32_t g0 = min(a.total, blockIdx.x * a.plan.per), g1 = min(a.total, g0 + a.plan.per);
     uint32_t kc = 0, vc = 0, ti = 0;   // K chunks, V stages and tiles so far, the same for every role
@@ -209,9 +213,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     lo[j] = cvt2(u - b.x, v - b.y);
                 }
                 const int c = d >> 6, unit16 = (d & 63) >> 3;
-                const int off = c * 8192 + r * 128 + ((unit16 ^ (r & 7)) << 4) + (d & 4) * 2;
+                const int off = c * 16384 + r * 128 + ((unit16 ^ (r & 7)) << 4) + (d & 4) * 2;
                 *reinterpret_cast<uint2*>(sQ + off) = make_uint2(hi[0], hi[1]);
-                *reinterpret_cast<uint2*>(sQ + C * 8192 + off) = make_uint2(lo[0], lo[1]);
+                *reinterpret_cast<uint2*>(sQ + 8192 + off) = make_uint2(lo[0], lo[1]);
             }
             if (lane == 0) {
                 qf_s[r] = __int_as_float((127 + e) << 23) * kLog2e * (FMT == GTM_KV_E4M3 ? 256.0f : 1.0f);
@@ -314,8 +318,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc::mbar_arrive(&rv_empty[it % RV]);
             }
         } else if (warp == 15) {   // ---- MMA issue (the whole warp; one elected lane issues)
-            constexpr uint32_t kQk = tc::idesc_f16(128, N);
-            constexpr uint32_t kPv = tc::idesc_f16(128, N) | (1u << 15) | (1u << 16);   // both operands M/N-contiguous
+            constexpr uint32_t kQk = tc::idesc_f16(128, 2 * N);
+            constexpr uint32_t kPv = tc::idesc_f16(128, S::kOWidth) | (1u << 15) | (1u << 16);   // both operands M/N-contiguous
             const uint32_t qa = tc::smem_u32(sQ), va0 = tc::smem_u32(sV), pa = tc::smem_u32(sP);
             uint32_t ik = kc, iv = vc;
             bool ok = true;
@@ -329,12 +333,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!wait(&ka_full[ik % KA], (ik / KA) & 1)) return;
                 tc::tc_fence_after();
                 const uint32_t ka = tmem + S::kACol + (ik % KA) * 32, d = tmem + S::kSCol;
-                const uint64_t qh = tc::sdesc_sw128(qa + c * 8192), ql = tc::sdesc_sw128(qa + (C + c) * 8192);
+                const uint64_t qd = tc::sdesc_sw128(qa + c * 16384);   // 64 high rows, then 64 low rows
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    tc::mma_f16_ts(d, ka + 8 * k, qh + 2 * k, kQk, (c > 0 || k > 0) ? 1u : 0u);
-                    tc::mma_f16_ts(d + N, ka + 8 * k, ql + 2 * k, kQk, (c > 0 || k > 0) ? 1u : 0u);
-                }
+                for (int k = 0; k < 4; ++k) tc::mma_f16_ts(d, ka + 8 * k, qd + 2 * k, kQk, (c > 0 || k > 0) ? 1u : 0u);
                 tc::mma_commit(&ka_empty[ik % KA]);
                 ++ik;
                 if (c == C - 1) tc::mma_commit(s_full);
@@ -345,12 +346,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (mt == 0 && !wait(&p_full[half], (ti + t) & 1)) return;
                 if (!wait(&v_full[iv % VST], (iv / VST) & 1)) return;
                 tc::tc_fence_after();
-                const uint32_t d = tmem + S::kOCol + mt * N, va = va0 + (iv % VST) * 16384, pb = pa + half * 64 * 128;
+                const uint32_t d = tmem + S::kOCol + mt * S::kOWidth;
+                const uint64_t vd = sdesc_mn(va0 + (iv % VST) * 16384, 8192), pd = sdesc_mn(pa + half * 64 * 128, 16384);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint64_t ad = sdesc_mn(va + k * 2048, 8192);
-                    tc::mma_f16(d, ad, sdesc_mn(pb + 16384 + k * 2048, 8192), kPv, (t > 0 || half || k > 0) ? 1u : 0u);
-                    tc::mma_f16(d, ad, sdesc_mn(pb + k * 2048, 8192), kPv, 1u);
+                for (int k = 0; k < 4; ++k) {   // 16 positions: 2,048 bytes
+                    tc::mma_f16(d, vd + 128 * k, pd + 128 * k, kPv, (t > 0 || half || k > 0) ? 1u : 0u);
+                    if (!S::kPairO) tc::mma_f16(d, vd + 128 * k, pd + (16384 >> 4) + 128 * k, kPv, 1u);
                 }
                 tc::mma_commit(&v_empty[iv % VST]);
                 ++iv;
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (t > 0) {
                         ok = __all_sync(0xffffffffu, tc::mbar_wait(&p_empty[1], (x & 1) ^ 1, abort_flag, kWaitNs));
                         tc::tc_fence_after();
-                        for (int c0 = 0; c0 < MT * 2; ++c0) {
+                        for (int c0 = 0; c0 < static_cast<int>(S::kSCol / N) * 2; ++c0) {
                             uint32_t v[16];
                             const uint32_t addr = lane_addr + S::kOCol + (c0 >> 1) * N + (c0 & 1) * 16;
                             tc::tmem_ld16_sync(addr, v);
@@ -509,7 +510,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int c0 = 0; c0 < MT * 2; ++c0) {
                     uint32_t v[16];
                     const int r0 = (c0 & 1) * 16;
-                    tc::tmem_ld16_sync(lane_addr + S::kOCol + (c0 >> 1) * N + r0, v);
+                    tc::tmem_ld16_sync(lane_addr + S::kOCol + (c0 >> 1) * S::kOWidth + r0, v);
+                    if (S::kPairO) {
+                        uint32_t w[16];
+                        tc::tmem_ld16_sync(lane_addr + S::kOCol + (c0 >> 1) * S::kOWidth + N + r0, w);
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) + __uint_as_float(w[c]));
+                    }
                     float* dst = part + static_cast<size_t>(r0) * HD + (c0 >> 1) * 128 + p;
                     float old[16];
                     if (merge) {
