@@ -8,9 +8,9 @@
 //   O^T [dims x 64 rows] += V^T p: V's codes become fp16 in shared memory (operand A, dims
 //     contiguous), p is operand B. O stays in tensor memory.
 // Rows on the N side make a unit of any number of rows cost what its 64 columns cost, and a
-// position per lane lets a thread apply its own scales; the maxima over positions take one redux
-// per column and warp. m only moves when a score passes it by 8 (a factor of 256 that fp16 has room
-// for), so O is rarely rescaled. Tiles follow ring slots, not positions: softmax does not mind the
+// position per lane lets a thread apply its own scales. m only moves when a score passes it by 8 (a
+// factor of 256 that fp16 has room for): a tile mostly takes one vote, and neither the maxima over its
+// positions (across lanes) nor a rescaled O. Tiles follow ring slots, not positions: softmax does not mind the
 // order, no tile wraps, and each row's span is a mask on the slot's position.
 //
 // A tensor core's addition to its accumulator is cut to fp32, not rounded, which biases a long sum by
@@ -73,11 +73,6 @@ struct SharedArgs {
     SharedPlan plan;
 };
 
-__device__ __forceinline__ float redux_max(float x) {
-    float r;
-    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
-    return r;
-}
 // Whether any of a softmax group's 128 threads says so (hardware barrier 1 or 2).
 __device__ __forceinline__ bool any_of_128(uint32_t bar, bool x) {
     uint32_t r;
@@ -219,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (lane == 0) {
                 qf_s[r] = __int_as_float((127 + e) << 23) * kLog2e * (FMT == GTM_KV_E4M3 ? 256.0f : 1.0f);
-                m_s[r] = -INFINITY;
+                if (sg.slot != done_slot) m_s[r] = -INFINITY;   // else this unit's maxima go on
                 const Span sp = live ? row_span(pos.v[row], a.window, a.prefix_len) : Span{0, 0, 0, 0};
                 // columns without a row are never read: they need no mask
                 rlo[r] = !live ? 0u : sp.pn ? sp.pa - a.lo[sg.unit] : 1u;
@@ -403,34 +398,63 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // the group's warps meet in barriers below, so they leave together or not at all
                 if (any_of_128(bar, !ok)) { ok = false; break; }
                 tc::tc_fence_after();
-                float s[H], top = -INFINITY;
+                float s[H];
+                // s = s2 - m for the group's columns; whether a weight would pass 2^8
+                auto scores = [&]() {
+                    float over = -INFINITY;
 #pragma unroll
-                for (int c0 = 0; c0 < H; c0 += 16) {
-                    uint32_t v[16], w[16];
-                    tc::tmem_ld16_sync(lane_addr + S::kSCol + c0, v);
-                    tc::tmem_ld16_sync(lane_addr + S::kSCol + N + c0, w);
+                    for (int c0 = 0; c0 < H; c0 += 16) {
+                        uint32_t v[16], w[16];
+                        tc::tmem_ld16_sync(lane_addr + S::kSCol + c0, v);
+                        tc::tmem_ld16_sync(lane_addr + S::kSCol + N + c0, w);
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) s[c0 + c] = __uint_as_float(v[c]) + __uint_as_float(w[c]);
-                }
-                tc::tc_fence_before();
-                tc::mbar_arrive(s_empty);
+                        for (int c = 0; c < 16; c += 4) {
+                            const float4 f = *reinterpret_cast<const float4*>(qf_c + c0 + c), m4 = *reinterpret_cast<const float4*>(m_c + c0 + c);
+                            const float fs[4] = {f.x, f.y, f.z, f.w}, ms[4] = {m4.x, m4.y, m4.z, m4.w};
 #pragma unroll
-                for (int c = 0; c < H; ++c) {
-                    s[c] *= ks * qf_c[c];
-                    if (!all_in) s[c] = in_ring && at >= rlo_c[c] && at < rhi_c[c] ? s[c] : -INFINITY;
-                    const float r = redux_max(s[c] + lg);
-                    if (lane == c) top = r;
-                }
-                if (any_of_128(bar, top > m_c[lane] + 8.0f)) {
-                    tops[lane] = top;
+                            for (int j = 0; j < 4; ++j)
+                                s[c0 + c + j] = fmaf(__uint_as_float(v[c + j]) + __uint_as_float(w[c + j]), ks * fs[j], -ms[j]);
+                        }
+                    }
+                    if (!all_in) {
+#pragma unroll
+                        for (int c = 0; c < H; ++c) s[c] = in_ring && at >= rlo_c[c] && at < rhi_c[c] ? s[c] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int c = 0; c < H; ++c) over = fmaxf(over, s[c]);
+                    return over + lg > 8.0f;
+                };
+                const bool raise = any_of_128(bar, scores());
+                if (raise) {
+                    // new maxima: 31 exchanges leave column `lane` with the lane (a column's maximum over the
+                    // warp's positions), m + s2 - m gives the score back (m is -infinity only in a first tile,
+                    // where a zero stands in for it)
+                    if (p < H) f_c[p] = m_c[p];
+                    tc::named_bar_sync(bar, 128);
+                    if (p < H && m_c[p] == -INFINITY) m_c[p] = 0.0f;
+                    tc::named_bar_sync(bar, 128);
+                    scores();
+#pragma unroll
+                    for (int w = H / 2; w > 0; w >>= 1)
+#pragma unroll
+                        for (int c = 0; c < w; ++c) {
+                            const float keep = (lane & w) ? s[c + w] : s[c], send = (lane & w) ? s[c] : s[c + w];
+                            s[c] = fmaxf(keep + (w == H / 2 ? lg : 0.0f), __shfl_xor_sync(0xffffffffu, send + (w == H / 2 ? lg : 0.0f), w));
+                        }
+                    tops[lane] = s[0] + m_c[lane];
                     tc::named_bar_sync(bar, 128);
                     if (p < H) {
                         const float* w = wtop + col0 + p;
-                        const float old = m_c[p], now = fmaxf(fmaxf(fmaxf(w[0], w[N]), fmaxf(w[2 * N], w[3 * N])), old);
+                        const float old = f_c[p], now = fmaxf(fmaxf(fmaxf(w[0], w[N]), fmaxf(w[2 * N], w[3 * N])), old);
                         f_c[p] = old == now ? 1.0f : ex2(old - now);
                         m_c[p] = now;
                     }
                     tc::named_bar_sync(bar, 128);
+                    scores();
+                }
+                tc::tc_fence_before();
+                tc::mbar_arrive(s_empty);   // before the wait below: PV of the tile before is issued behind QK of the next
+                if (raise) {
 #pragma unroll
                     for (int i = 0; i < H; ++i) l[i] *= f_c[i];
                     if (t > 0) {
@@ -454,11 +478,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     float e[2];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        // a masked score is -infinity, and so may its column's m be; a NaN goes through
-                        e[j] = ex2(s[c + j] - m_c[c + j]);
-                        if (!all_in) e[j] = s[c + j] == -INFINITY ? 0.0f : e[j];
+                        e[j] = ex2(s[c + j]);   // 0 where masked (s is -infinity), whatever m is; a NaN goes through
                         l[c + j] += e[j];
-                        e[j] = !all_in && s[c + j] == -INFINITY ? 0.0f : e[j] * vs;
+                        e[j] = s[c + j] == -INFINITY ? 0.0f : e[j] * vs;
                     }
                     hi[c >> 1] = cvt2(e[0], e[1]);
                     const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&hi[c >> 1]));
