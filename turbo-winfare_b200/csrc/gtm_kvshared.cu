@@ -17,16 +17,17 @@
 // up to 2^-24 of it per instruction. So a score's limbs are summed apart (HD / 16 instructions each),
 // and O goes to memory after kLongest tiles (16 instructions each), where results are added in fp32.
 //
-// The issue order is PV of tile i and QK of tile i + 2 in turn, 64 dims at a time, while the softmax
-// warps work on tile i + 1: K and V are converted side by side at an even pace. PV takes a tile's
-// positions in two halves, so that one half of p is written while the other is read.
+// S and O are issued by two warps, so that neither waits behind the other's barriers: while the
+// softmax works on tile i + 1, O of tile i and S of tile i + 2 are formed side by side, and K and V
+// are converted at an even pace. O takes a tile's positions in two halves, so that one half of p is
+// written while the other is read.
 //
 // The work is the flat list of (kv head, unit, tile), cut into equal runs, one per CTA; a CTA leaves a
 // partial result for each unit it touches.
 //
-// Roles: warps 0-7 softmax and O (32 of the 64 columns each half of them); 8-11 K; 12-13 V; 14 TMA
-// loads of K and V codes, in the issue order; 15 MMA. Every wait is bounded (1 s); one that runs out stops the CTA
-// and marks its results NaN.
+// Roles: warps 0-7 softmax and O (32 of the 64 columns each half of them); 8-11 K; 12-15 V; 16 issues
+// S, 17 O; 18 and 19 load the codes of K and V. Every wait is bounded (1 s); one that runs out stops the
+// CTA and marks its results NaN.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -41,7 +42,7 @@ namespace {
 
 constexpr int N = kSharedRows;
 constexpr int TP = 128;              // positions of a tile
-constexpr int kThreads = 512;
+constexpr int kThreads = 640;
 constexpr uint64_t kWaitNs = 1000000000ull;
 constexpr int KA = 4;                // K chunks (64 dims) in tensor memory
 constexpr uint32_t kLongest = 16;    // tiles summed in tensor memory before the result goes to memory
@@ -79,6 +80,14 @@ __device__ __forceinline__ bool any_of_128(uint32_t bar, bool x) {
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
                  : "=r"(r) : "r"(x ? 1u : 0u), "r"(bar) : "memory");
     return r != 0;
+}
+// One arrival for the warp: 32 lanes' arrivals on one barrier are taken one by one.
+__device__ __forceinline__ void arrive_warp(uint64_t* a, uint64_t* b = nullptr) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+        tc::mbar_arrive(a);
+        if (b) tc::mbar_arrive(b);
+    }
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -154,31 +163,30 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        for (int i = 0; i < RK; ++i) tc::mbar_init(&rk_full[i], 1), tc::mbar_init(&rk_empty[i], 128);
-        for (int i = 0; i < RV; ++i) tc::mbar_init(&rv_full[i], 1), tc::mbar_init(&rv_empty[i], 64);
-        for (int i = 0; i < KA; ++i) tc::mbar_init(&ka_full[i], 128), tc::mbar_init(&ka_empty[i], 1);
-        for (int i = 0; i < VST; ++i) tc::mbar_init(&v_full[i], 64), tc::mbar_init(&v_empty[i], 1);
-        tc::mbar_init(s_full, 1), tc::mbar_init(s_empty, 256);
-        for (int i = 0; i < 2; ++i) tc::mbar_init(&p_full[i], 128), tc::mbar_init(&p_empty[i], 1);   // a half of the positions
+        for (int i = 0; i < RK; ++i) tc::mbar_init(&rk_full[i], 1), tc::mbar_init(&rk_empty[i], 4);
+        for (int i = 0; i < RV; ++i) tc::mbar_init(&rv_full[i], 1), tc::mbar_init(&rv_empty[i], 4);
+        for (int i = 0; i < KA; ++i) tc::mbar_init(&ka_full[i], 4), tc::mbar_init(&ka_empty[i], 1);
+        for (int i = 0; i < VST; ++i) tc::mbar_init(&v_full[i], 4), tc::mbar_init(&v_empty[i], 1);
+        tc::mbar_init(s_full, 1), tc::mbar_init(s_empty, 8);
+        for (int i = 0; i < 2; ++i) tc::mbar_init(&p_full[i], 4), tc::mbar_init(&p_empty[i], 1);   // a half of the positions
         *abort_flag = (tc::smem_u32(smem) & 1023u) ? 1 : 0;   // the swizzled layouts need it
         tc::mbar_fence_init();
     }
-    if (warp == 15) tc::tmem_alloc(tmem_slot, 512);
+    if (warp == 17) tc::tmem_alloc(tmem_slot, 512);
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = __reduce_or_sync(0xffffffffu, *tmem_slot);   // in a uniform register, as MMA operands are
 
     const uint32_t g0 = min(a.total, blockIdx.x * a.plan.per), g1 = min(a.total, g0 + a.plan.per);
-    uint32_t kc = 0, vc = 0, ti = 0;   // K chunks, V stages and tiles so far, the same for every role
-    uint32_t done_slot = 0xFFFFFFFFu;  // the slot that already holds this CTA's result
-    for (uint32_t g = g0; g < g1;) {
-        const Segment sg = segment_at(a, g, g1);
-        g += sg.tiles;
+    // K chunks (as many V stages) and tiles so far, the same for every role; the slot that already holds
+    // this CTA's result
+    uint32_t kc = 0, ti = 0, done_slot = 0xFFFFFFFFu;
+    // Brings a segment's q into shared memory; false once the CTA has given up.
+    auto begin = [&](const Segment& sg) -> bool {
         if (__syncthreads_or(*abort_flag)) {
             if (tid < N) a.plan.ml[static_cast<size_t>(sg.slot) * N + tid] = make_float2(0.0f, __int_as_float(0x7FC00000));
-            done_slot = sg.slot;
-            continue;
+            return false;
         }
         // ---- q's limbs and the rows' spans
         for (int r = warp; r < N; r += kThreads / 32) {
@@ -223,156 +231,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc::fence_proxy_async_smem();
         __syncthreads();
-        auto ring_tile = [&](uint32_t t) {
-            const uint32_t b = a.first[sg.unit] + sg.tile + t;
-            return b >= a.ring_tiles ? b - a.ring_tiles : b;
-        };
-
-        if (warp == 14) {   // ---- K and V codes, in the order in which they are multiplied
-            if (lane == 0) {
-                uint32_t ik = kc, iv = vc;
-                bool ok = true;
-                auto load_k = [&](uint32_t t, int c) {
-                    uint64_t* full = &rk_full[ik % RK];
-                    ok = ok && tc::mbar_wait(&rk_empty[ik % RK], ((ik / RK) & 1) ^ 1, abort_flag, kWaitNs);
-                    if (!ok) return;
-                    tc::mbar_arrive_expect_tx(full, 8192);
-                    tc::tma_load_2d(sRawK + (ik % RK) * 8192, &a.k_map, static_cast<int>(sg.kvh * HD + c * 64),
-                                    static_cast<int>(ring_tile(t) * TP), full);
-                    ++ik;
-                };
-                auto load_v = [&](uint32_t t, int c) {
-                    uint64_t* full = &rv_full[iv % RV];
-                    ok = ok && tc::mbar_wait(&rv_empty[iv % RV], ((iv / RV) & 1) ^ 1, abort_flag, kWaitNs);
-                    if (!ok) return;
-                    tc::mbar_arrive_expect_tx(full, 8192);
-                    tc::tma_load_2d(sRawV + (iv % RV) * 8192, &a.v_map, static_cast<int>(sg.kvh * HD + (c % MT) * 128),
-                                    static_cast<int>(ring_tile(t) * TP) + (c / MT) * 64, full);
-                    ++iv;
-                };
-                for (uint32_t t = 0; t < 2 && t < sg.tiles; ++t)
-                    for (int c = 0; c < C && ok; ++c) load_k(t, c);
-                for (uint32_t t = 0; t < sg.tiles && ok; ++t)
-                    for (int c = 0; c < C && ok; ++c) {
-                        load_v(t, c);
-                        if (t + 2 < sg.tiles) load_k(t + 2, c);
-                    }
-                if (*abort_flag) {   // no exit while copies into this CTA's shared memory are in flight
-                    volatile int never = 0;
-                    for (uint32_t j = ik > RK ? ik - RK : 0; j < ik; ++j) tc::mbar_wait(&rk_full[j % RK], (j / RK) & 1, &never, kWaitNs);
-                    for (uint32_t j = iv > RV ? iv - RV : 0; j < iv; ++j) tc::mbar_wait(&rv_full[j % RV], (j / RV) & 1, &never, kWaitNs);
-                }
+        return true;
+    };
+    auto ring_tile = [&](const Segment& sg, uint32_t t) {
+        const uint32_t b = a.first[sg.unit] + sg.tile + t;
+        return b >= a.ring_tiles ? b - a.ring_tiles : b;
+    };
+    // 640 threads x 96 registers at launch >= 256 x 128 + 384 x 72: the softmax keeps 32 scores and 32 sums
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+        // ---- softmax: a position and 32 columns per thread
+        constexpr int H = N / 2;
+        const int p = tid & 127, grp = warp >> 2, half = p >> 6;
+        const int col0 = grp * H;   // the group's columns
+        const uint32_t bar = 1 + grp;
+        const uint32_t lane_addr = (tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16)) + col0;
+        float *tops = wtop + (warp & 3) * N + col0, *m_c = m_s + col0, *f_c = f_s + col0;
+        const float* qf_c = qf_s + col0;
+        const uint32_t *rlo_c = rlo + col0, *rhi_c = rhi + col0;
+        for (uint32_t g = g0; g < g1;) {
+            const Segment sg = segment_at(a, g, g1);
+            g += sg.tiles;
+            if (!begin(sg)) {
+                done_slot = sg.slot;
+                continue;
             }
-        } else if (warp >= 8 && warp < 12) {   // ---- K: codes to fp16 in tensor memory, a position per lane
-            const int p = 32 * (warp & 3) + lane;
-            const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + S::kACol;
-            uint32_t it = kc;
-            const uint32_t end = kc + sg.tiles * C;
-            for (; it < end; ++it) {
-                if (!__all_sync(0xffffffffu, tc::mbar_wait(&rk_full[it % RK], (it / RK) & 1, abort_flag, kWaitNs))) break;
-                const uint8_t* raw = sRawK + (it % RK) * 8192 + p * 64;
-                uint32_t o[32];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(raw + ((j ^ ((p >> 1) & 3)) << 4));
-                    uint32_t h[8];
-                    widen<FMT>(w, h);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) o[8 * j + i] = h[i];
-                }
-                if (!__all_sync(0xffffffffu, tc::mbar_wait(&ka_empty[it % KA], ((it / KA) & 1) ^ 1, abort_flag, kWaitNs))) break;
-                tc::tc_fence_after();
-                tc::tmem_st32(lane_addr + (it % KA) * 32, o);
-                tc::tmem_st_wait();
-                tc::tc_fence_before();
-                tc::mbar_arrive(&ka_full[it % KA]);
-                tc::mbar_arrive(&rk_empty[it % RK]);   // only after the words were used (see gtm_tokens.cu)
-            }
-        } else if (warp == 12 || warp == 13) {   // ---- V: codes to fp16 in shared memory, dims contiguous
-            const int p = tid - 384;
-            uint32_t it = vc;
-            const uint32_t end = vc + sg.tiles * S::kVStages;
-            for (; it < end; ++it) {
-                if (!__all_sync(0xffffffffu, tc::mbar_wait(&rv_full[it % RV], (it / RV) & 1, abort_flag, kWaitNs))) break;
-                const uint8_t* raw = sRawV + (it % RV) * 8192 + p * 128;
-                uint4 w[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = *reinterpret_cast<const uint4*>(raw + ((j ^ (p & 7)) << 4));
-                if (!__all_sync(0xffffffffu, tc::mbar_wait(&v_empty[it % VST], ((it / VST) & 1) ^ 1, abort_flag, kWaitNs))) break;
-                uint8_t* dst = sV + (it % VST) * 16384 + p * 128;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    uint32_t h[8];
-                    widen<FMT>(w[j], h);
-                    uint8_t* d = dst + (j >> 2) * 8192;
-                    *reinterpret_cast<uint4*>(d + (((2 * (j & 3)) ^ (p & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4*>(d + (((2 * (j & 3) + 1) ^ (p & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
-                }
-                tc::fence_proxy_async_smem();
-                tc::mbar_arrive(&v_full[it % VST]);
-                tc::mbar_arrive(&rv_empty[it % RV]);
-            }
-        } else if (warp == 15) {   // ---- MMA issue (the whole warp; one elected lane issues)
-            constexpr uint32_t kQk = tc::idesc_f16(128, 2 * N);
-            constexpr uint32_t kPv = tc::idesc_f16(128, S::kOWidth) | (1u << 15) | (1u << 16);   // both operands M/N-contiguous
-            const uint32_t qa = tc::smem_u32(sQ), va0 = tc::smem_u32(sV), pa = tc::smem_u32(sP);
-            uint32_t ik = kc, iv = vc;
-            bool ok = true;
-            auto wait = [&](uint64_t* bar, uint32_t parity) {
-                ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_flag, kWaitNs));
-                return ok;
-            };
-            // chunk c of S of tile t (of the segment)
-            auto qk = [&](uint32_t t, int c) {
-                if (c == 0 && !wait(s_empty, ((ti + t) & 1) ^ 1)) return;
-                if (!wait(&ka_full[ik % KA], (ik / KA) & 1)) return;
-                tc::tc_fence_after();
-                const uint32_t ka = tmem + S::kACol + (ik % KA) * 32, d = tmem + S::kSCol;
-                const uint64_t qd = tc::sdesc_sw128(qa + c * 16384);   // 64 high rows, then 64 low rows
-#pragma unroll
-                for (int k = 0; k < 4; ++k) tc::mma_f16_ts(d, ka + 8 * k, qd + 2 * k, kQk, (c > 0 || k > 0) ? 1u : 0u);
-                tc::mma_commit(&ka_empty[ik % KA]);
-                ++ik;
-                if (c == C - 1) tc::mma_commit(s_full);
-            };
-            // stage c of O of tile t: 128 dims c % MT, positions' half c / MT
-            auto pv = [&](uint32_t t, int c) {
-                const int half = c / MT, mt = c % MT;
-                if (mt == 0 && !wait(&p_full[half], (ti + t) & 1)) return;
-                if (!wait(&v_full[iv % VST], (iv / VST) & 1)) return;
-                tc::tc_fence_after();
-                const uint32_t d = tmem + S::kOCol + mt * S::kOWidth;
-                const uint64_t vd = sdesc_mn(va0 + (iv % VST) * 16384, 8192), pd = sdesc_mn(pa + half * 64 * 128, 16384);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {   // 16 positions: 2,048 bytes
-                    tc::mma_f16(d, vd + 128 * k, pd + 128 * k, kPv, (t > 0 || half || k > 0) ? 1u : 0u);
-                    if (!S::kPairO) tc::mma_f16(d, vd + 128 * k, pd + (16384 >> 4) + 128 * k, kPv, 1u);
-                }
-                tc::mma_commit(&v_empty[iv % VST]);
-                ++iv;
-                if (mt == MT - 1) tc::mma_commit(&p_empty[half]);
-            };
-            for (uint32_t t = 0; t < 2 && t < sg.tiles; ++t)
-                for (int c = 0; c < C && ok; ++c) qk(t, c);
-            for (uint32_t t = 0; t < sg.tiles && ok; ++t)
-                for (int c = 0; c < C && ok; ++c) {
-                    pv(t, c);
-                    if (ok && t + 2 < sg.tiles) qk(t + 2, c);
-                }
-            if (*abort_flag) {   // issued MMAs end before tensor memory is released
-                volatile int never = 0;
-                if (ik > 0) tc::mbar_wait(&ka_empty[(ik - 1) % KA], ((ik - 1) / KA) & 1, &never, kWaitNs);
-                if (iv > 0) tc::mbar_wait(&v_empty[(iv - 1) % VST], ((iv - 1) / VST) & 1, &never, kWaitNs);
-            }
-        } else if (warp < 8) {   // ---- softmax: a position and 32 columns per thread
-            constexpr int H = N / 2;
-            const int p = tid & 127, grp = warp >> 2, half = p >> 6;
-            const int col0 = grp * H;   // the group's columns
-            const uint32_t bar = 1 + grp;
-            const uint32_t lane_addr = (tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16)) + col0;
-            float *tops = wtop + (warp & 3) * N + col0, *m_c = m_s + col0, *f_c = f_s + col0;
-            const float* qf_c = qf_s + col0;
-            const uint32_t *rlo_c = rlo + col0, *rhi_c = rhi + col0;
             const uint32_t s0 = a.lo[sg.unit] % a.capacity;
             const float *ksp = a.ks + static_cast<size_t>(sg.kvh) * a.capacity, *vsp = a.vs + static_cast<size_t>(sg.kvh) * a.capacity;
             const uint32_t max_lo = __reduce_max_sync(0xffffffffu, rlo_c[lane]);
@@ -380,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             float l[H];
 #pragma unroll
             for (int i = 0; i < H; ++i) l[i] = 0.0f;
-            uint32_t slot = ring_tile(0) * TP + p;
+            uint32_t slot = ring_tile(sg, 0) * TP + p;
             float ks_next = slot < a.capacity ? __ldg(ksp + slot) : 1.0f, vs_next = slot < a.capacity ? __ldg(vsp + slot) : 1.0f;
             bool ok = true;
             for (uint32_t t = 0; t < sg.tiles; ++t) {
@@ -389,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const bool in_ring = slot < a.capacity;
                 const uint32_t at = slot - s0 + (slot < s0 ? a.capacity : 0u);   // from the unit's first position
                 if (t + 1 < sg.tiles) {
-                    slot = ring_tile(t + 1) * TP + p;
+                    slot = ring_tile(sg, t + 1) * TP + p;
                     ks_next = slot < a.capacity ? __ldg(ksp + slot) : 1.0f;
                     vs_next = slot < a.capacity ? __ldg(vsp + slot) : 1.0f;
                 }
@@ -398,63 +281,57 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // the group's warps meet in barriers below, so they leave together or not at all
                 if (any_of_128(bar, !ok)) { ok = false; break; }
                 tc::tc_fence_after();
-                float s[H];
-                // s = s2 - m for the group's columns; whether a weight would pass 2^8
-                auto scores = [&]() {
-                    float over = -INFINITY;
+                float s[H], over = -INFINITY;   // s2, -infinity where masked; whether a weight would pass 2^8
 #pragma unroll
-                    for (int c0 = 0; c0 < H; c0 += 16) {
-                        uint32_t v[16], w[16];
-                        tc::tmem_ld16_sync(lane_addr + S::kSCol + c0, v);
-                        tc::tmem_ld16_sync(lane_addr + S::kSCol + N + c0, w);
+                for (int c0 = 0; c0 < H; c0 += 16) {
+                    uint32_t v[16], w[16];
+                    tc::tmem_ld16_sync(lane_addr + S::kSCol + c0, v);
+                    tc::tmem_ld16_sync(lane_addr + S::kSCol + N + c0, w);
 #pragma unroll
-                        for (int c = 0; c < 16; c += 4) {
-                            const float4 f = *reinterpret_cast<const float4*>(qf_c + c0 + c), m4 = *reinterpret_cast<const float4*>(m_c + c0 + c);
-                            const float fs[4] = {f.x, f.y, f.z, f.w}, ms[4] = {m4.x, m4.y, m4.z, m4.w};
+                    for (int c = 0; c < 16; ++c) s[c0 + c] = __uint_as_float(v[c]) + __uint_as_float(w[c]);
+                }
+                tc::tc_fence_before();
+                arrive_warp(s_empty);   // the next tile's S may be formed
 #pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                s[c0 + c + j] = fmaf(__uint_as_float(v[c + j]) + __uint_as_float(w[c + j]), ks * fs[j], -ms[j]);
-                        }
-                    }
-                    if (!all_in) {
+                for (int c = 0; c < H; c += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(qf_c + c);
+                    s[c] *= ks * f.x, s[c + 1] *= ks * f.y, s[c + 2] *= ks * f.z, s[c + 3] *= ks * f.w;
+                }
+                if (!all_in) {
 #pragma unroll
-                        for (int c = 0; c < H; ++c) s[c] = in_ring && at >= rlo_c[c] && at < rhi_c[c] ? s[c] : -INFINITY;
-                    }
+                    for (int c = 0; c < H; ++c) s[c] = in_ring && at >= rlo_c[c] && at < rhi_c[c] ? s[c] : -INFINITY;
+                }
 #pragma unroll
-                    for (int c = 0; c < H; ++c) over = fmaxf(over, s[c]);
-                    return over + lg > 8.0f;
-                };
-                const bool raise = any_of_128(bar, scores());
+                for (int c = 0; c < H; c += 4) {   // (-infinity) - (-infinity) is NaN, which fmaxf passes over
+                    const float4 m4 = *reinterpret_cast<const float4*>(m_c + c);
+                    over = fmaxf(over, fmaxf(fmaxf(s[c] - m4.x, s[c + 1] - m4.y), fmaxf(s[c + 2] - m4.z, s[c + 3] - m4.w)));
+                }
+                const bool raise = any_of_128(bar, over + lg > 8.0f);
                 if (raise) {
-                    // new maxima: 31 exchanges leave column `lane` with the lane (a column's maximum over the
-                    // warp's positions), m + s2 - m gives the score back (m is -infinity only in a first tile,
-                    // where a zero stands in for it)
-                    if (p < H) f_c[p] = m_c[p];
-                    tc::named_bar_sync(bar, 128);
-                    if (p < H && m_c[p] == -INFINITY) m_c[p] = 0.0f;
-                    tc::named_bar_sync(bar, 128);
-                    scores();
+                    // new maxima: 15 exchanges and one more leave a column's maximum over the warp's positions
+                    // with two lanes
+                    for (int c0 = 0; c0 < H; c0 += 16) {
+                        float y[16];
 #pragma unroll
-                    for (int w = H / 2; w > 0; w >>= 1)
+                        for (int c = 0; c < 16; ++c) y[c] = (c0 ? s[c + 16] : s[c]) + lg;
 #pragma unroll
-                        for (int c = 0; c < w; ++c) {
-                            const float keep = (lane & w) ? s[c + w] : s[c], send = (lane & w) ? s[c] : s[c + w];
-                            s[c] = fmaxf(keep + (w == H / 2 ? lg : 0.0f), __shfl_xor_sync(0xffffffffu, send + (w == H / 2 ? lg : 0.0f), w));
-                        }
-                    tops[lane] = s[0] + m_c[lane];
+                        for (int w = 8; w > 0; w >>= 1)
+#pragma unroll
+                            for (int c = 0; c < w; ++c) {
+                                const float keep = (lane & w) ? y[c + w] : y[c], send = (lane & w) ? y[c] : y[c + w];
+                                y[c] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, w));
+                            }
+                        y[0] = fmaxf(y[0], __shfl_xor_sync(0xffffffffu, y[0], 16));
+                        if (lane < 16) tops[c0 + lane] = y[0];
+                    }
                     tc::named_bar_sync(bar, 128);
                     if (p < H) {
                         const float* w = wtop + col0 + p;
-                        const float old = f_c[p], now = fmaxf(fmaxf(fmaxf(w[0], w[N]), fmaxf(w[2 * N], w[3 * N])), old);
+                        const float old = m_c[p], now = fmaxf(fmaxf(fmaxf(w[0], w[N]), fmaxf(w[2 * N], w[3 * N])), old);
                         f_c[p] = old == now ? 1.0f : ex2(old - now);
                         m_c[p] = now;
                     }
                     tc::named_bar_sync(bar, 128);
-                    scores();
-                }
-                tc::tc_fence_before();
-                tc::mbar_arrive(s_empty);   // before the wait below: PV of the tile before is issued behind QK of the next
-                if (raise) {
 #pragma unroll
                     for (int i = 0; i < H; ++i) l[i] *= f_c[i];
                     if (t > 0) {
@@ -472,30 +349,35 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tc::tc_fence_before();
                     }
                 }
-                uint32_t hi[H / 2], lo[H / 2];
-#pragma unroll
-                for (int c = 0; c < H; c += 2) {
-                    float e[2];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        e[j] = ex2(s[c + j]);   // 0 where masked (s is -infinity), whatever m is; a NaN goes through
-                        l[c + j] += e[j];
-                        e[j] = s[c + j] == -INFINITY ? 0.0f : e[j] * vs;
-                    }
-                    hi[c >> 1] = cvt2(e[0], e[1]);
-                    const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&hi[c >> 1]));
-                    lo[c >> 1] = cvt2(e[0] - w.x, e[1] - w.y);
-                }
                 ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&p_empty[half], (x & 1) ^ 1, abort_flag, kWaitNs));
                 uint8_t* prow = sP + p * 128;
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int off = ((col0 / 8 + u) ^ (p & 7)) << 4;
-                    *reinterpret_cast<uint4*>(prow + off) = make_uint4(hi[4 * u], hi[4 * u + 1], hi[4 * u + 2], hi[4 * u + 3]);
-                    *reinterpret_cast<uint4*>(prow + 16384 + off) = make_uint4(lo[4 * u], lo[4 * u + 1], lo[4 * u + 2], lo[4 * u + 3]);
+                for (int c0 = 0; c0 < H; c0 += 16) {
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int c = 0; c < 16; c += 2) {
+                        const float2 m2 = *reinterpret_cast<const float2*>(m_c + c0 + c);
+                        float e[2];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {   // 0 where masked, whatever m and vs are; a NaN goes through
+                            const bool out = s[c0 + c + j] == -INFINITY;
+                            e[j] = out ? 0.0f : ex2(s[c0 + c + j] - (j ? m2.y : m2.x));
+                            l[c0 + c + j] += e[j];
+                            e[j] = out ? 0.0f : e[j] * vs;
+                        }
+                        hi[c >> 1] = cvt2(e[0], e[1]);
+                        const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&hi[c >> 1]));
+                        lo[c >> 1] = cvt2(e[0] - w.x, e[1] - w.y);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int off = (((col0 + c0) / 8 + u) ^ (p & 7)) << 4;
+                        *reinterpret_cast<uint4*>(prow + off) = make_uint4(hi[4 * u], hi[4 * u + 1], hi[4 * u + 2], hi[4 * u + 3]);
+                        *reinterpret_cast<uint4*>(prow + 16384 + off) = make_uint4(lo[4 * u], lo[4 * u + 1], lo[4 * u + 2], lo[4 * u + 3]);
+                    }
                 }
                 tc::fence_proxy_async_smem();
-                tc::mbar_arrive(&p_full[half]);
+                arrive_warp(&p_full[half]);
             }
             const uint32_t last = ti + sg.tiles - 1;
             ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&p_empty[1], last & 1, abort_flag, kWaitNs));
@@ -555,15 +437,148 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else if (p < H) {
                 ml[p] = make_float2(0.0f, __int_as_float(0x7FC00000));
             }
+            ti += sg.tiles;
+            done_slot = sg.slot;
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    for (uint32_t g = g0; g < g1;) {
+        const Segment sg = segment_at(a, g, g1);
+        g += sg.tiles;
+        const bool good = begin(sg);
+        done_slot = sg.slot;
+        if (!good) continue;
+        const uint32_t vc = kc;
+        if (warp >= 8 && warp < 12) {   // ---- K: codes to fp16 in tensor memory, a position per lane
+            const int p = 32 * (warp & 3) + lane;
+            const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + S::kACol;
+            uint32_t it = kc;
+            const uint32_t end = kc + sg.tiles * C;
+            for (; it < end; ++it) {
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(&rk_full[it % RK], (it / RK) & 1, abort_flag, kWaitNs))) break;
+                const uint8_t* raw = sRawK + (it % RK) * 8192 + p * 64;
+                uint32_t o[32];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(raw + ((j ^ ((p >> 1) & 3)) << 4));
+                    uint32_t h[8];
+                    widen<FMT>(w, h);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[8 * j + i] = h[i];
+                }
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(&ka_empty[it % KA], ((it / KA) & 1) ^ 1, abort_flag, kWaitNs))) break;
+                tc::tc_fence_after();
+                tc::tmem_st32(lane_addr + (it % KA) * 32, o);
+                tc::tmem_st_wait();
+                tc::tc_fence_before();
+                arrive_warp(&ka_full[it % KA], &rk_empty[it % RK]);   // the raw slot only after its words were used
+            }
+        } else if (warp >= 12 && warp < 16) {   // ---- V: codes to fp16 in shared memory, dims contiguous
+            const int p = (tid - 384) & 63, half = (tid - 384) >> 6;
+            uint32_t it = vc;
+            const uint32_t end = vc + sg.tiles * S::kVStages;
+            for (; it < end; ++it) {
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(&rv_full[it % RV], (it / RV) & 1, abort_flag, kWaitNs))) break;
+                const uint8_t* raw = sRawV + (it % RV) * 8192 + p * 128;
+                uint4 w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4*>(raw + (((half * 4 + j) ^ (p & 7)) << 4));
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(&v_empty[it % VST], ((it / VST) & 1) ^ 1, abort_flag, kWaitNs))) break;
+                uint8_t* dst = sV + (it % VST) * 16384 + half * 8192 + p * 128;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t h[8];
+                    widen<FMT>(w[j], h);
+                    *reinterpret_cast<uint4*>(dst + (((2 * j) ^ (p & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4*>(dst + (((2 * j + 1) ^ (p & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+                }
+                tc::fence_proxy_async_smem();
+                arrive_warp(&v_full[it % VST], &rv_empty[it % RV]);
+            }
+        } else if (warp == 18 || warp == 19) {   // ---- codes of K and of V
+            if (lane == 0) {
+                const bool is_v = warp == 19;
+                const uint32_t R = is_v ? RV : RK, first = is_v ? vc : kc, end = first + sg.tiles * C;
+                uint64_t *full = is_v ? rv_full : rk_full, *empty = is_v ? rv_empty : rk_empty;
+                uint8_t* dst = is_v ? sRawV : sRawK;
+                uint32_t it = first;
+                for (; it < end; ++it) {
+                    const uint32_t c = (it - first) % C;
+                    const int y = static_cast<int>(ring_tile(sg, (it - first) / C) * TP), x = static_cast<int>(sg.kvh * HD);
+                    if (!tc::mbar_wait(&empty[it % R], ((it / R) & 1) ^ 1, abort_flag, kWaitNs)) break;
+                    tc::mbar_arrive_expect_tx(&full[it % R], 8192);
+                    if (is_v)
+                        tc::tma_load_2d(dst + (it % R) * 8192, &a.v_map, x + static_cast<int>(c % MT * 128), y + static_cast<int>(c / MT * 64), &full[it % R]);
+                    else
+                        tc::tma_load_2d(dst + (it % R) * 8192, &a.k_map, x + static_cast<int>(c * 64), y, &full[it % R]);
+                }
+                if (*abort_flag) {   // no exit while copies into this CTA's shared memory are in flight
+                    volatile int never = 0;
+                    for (uint32_t j = it > R ? it - R : 0; j < it; ++j) tc::mbar_wait(&full[j % R], (j / R) & 1, &never, kWaitNs);
+                }
+            }
+        } else if (warp == 16) {   // ---- S: the whole warp, one elected lane issues
+            constexpr uint32_t kQk = tc::idesc_f16(128, 2 * N);
+            const uint32_t qa = tc::smem_u32(sQ), d = tmem + S::kSCol;
+            uint32_t ik = kc;
+            bool ok = true;
+            for (uint32_t t = 0; t < sg.tiles && ok; ++t) {
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(s_empty, ((ti + t) & 1) ^ 1, abort_flag, kWaitNs))) break;
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&ka_full[ik % KA], (ik / KA) & 1, abort_flag, kWaitNs));
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                    const uint32_t ka = tmem + S::kACol + (ik % KA) * 32;
+                    const uint64_t qd = tc::sdesc_sw128(qa + c * 16384);   // 64 high rows, then 64 low rows
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tc::mma_f16_ts(d, ka + 8 * k, qd + 2 * k, kQk, (c > 0 || k > 0) ? 1u : 0u);
+                    tc::mma_commit(&ka_empty[ik % KA]);
+                    ++ik;
+                }
+                if (ok) tc::mma_commit(s_full);
+            }
+            if (*abort_flag && ik > 0) {   // issued MMAs end before tensor memory is released
+                volatile int never = 0;
+                tc::mbar_wait(&ka_empty[(ik - 1) % KA], ((ik - 1) / KA) & 1, &never, kWaitNs);
+            }
+        } else if (warp == 17) {   // ---- O, likewise
+            constexpr uint32_t kPv = tc::idesc_f16(128, S::kOWidth) | (1u << 15) | (1u << 16);   // both operands M/N-contiguous
+            const uint32_t va = tc::smem_u32(sV), pa = tc::smem_u32(sP);
+            uint32_t iv = vc;
+            bool ok = true;
+            for (uint32_t t = 0; t < sg.tiles && ok; ++t) {
+#pragma unroll
+                for (int c = 0; c < C; ++c) {   // 128 dims c % MT, positions' half c / MT
+                    const int half = c / MT, mt = c % MT;
+                    if (mt == 0) ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&p_full[half], (ti + t) & 1, abort_flag, kWaitNs));
+                    ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&v_full[iv % VST], (iv / VST) & 1, abort_flag, kWaitNs));
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                    const uint32_t d = tmem + S::kOCol + mt * S::kOWidth;
+                    const uint64_t vd = sdesc_mn(va + (iv % VST) * 16384, 8192), pd = sdesc_mn(pa + half * 64 * 128, 16384);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {   // 16 positions: 2,048 bytes
+                        tc::mma_f16(d, vd + 128 * k, pd + 128 * k, kPv, (t > 0 || half || k > 0) ? 1u : 0u);
+                        if (!S::kPairO) tc::mma_f16(d, vd + 128 * k, pd + (16384 >> 4) + 128 * k, kPv, 1u);
+                    }
+                    tc::mma_commit(&v_empty[iv % VST]);
+                    ++iv;
+                    if (mt == MT - 1) tc::mma_commit(&p_empty[half]);
+                }
+            }
+            if (*abort_flag && iv > 0) {
+                volatile int never = 0;
+                tc::mbar_wait(&v_empty[(iv - 1) % VST], ((iv - 1) / VST) & 1, &never, kWaitNs);
+            }
         }
         kc += sg.tiles * C;
-        vc += sg.tiles * S::kVStages;
         ti += sg.tiles;
-        done_slot = sg.slot;
+    }
     }
     tc::tc_fence_before();
     __syncthreads();
-    if (warp == 15) {
+    if (warp == 17) {
         tc::tmem_relinquish();
         tc::tmem_dealloc(tmem, 512);
     }
