@@ -6,16 +6,14 @@
 //   1 the largest logit, and its lowest id;
 //   2 the cuts. Ranked by logit, every cut keeps a run from the top, so the kept set is the ids whose
 //     key (logit, then lower id) is at least a border's. Ids are counted per level of max - logit,
-//     1/64 wide; a level's weights agree within 1.6%, so the counts alone bracket the nucleus' border
+//     1/128 wide; a level's weights agree within 0.8%, so the counts alone bracket the nucleus' border
 //     to a few levels. One pass then sums the exact weights (all, above the bracket, per level in
 //     it), and the ids of the level that holds the border are gathered and ranked. More ids than the
 //     gather holds (equal or nearly equal logits) are narrowed by the logit's ordered bits instead;
 //   3 the draw: sums of the kept weights per warp's run of ids, CTA and cluster, then one warp finds
 //     the id in the run that the target falls in.
-// Weights exp(l - max) are formed in 64 bits, rounded to multiples of 2^-(62 - bits of the vocabulary)
-// and summed as 64-bit integers: the sums cannot overflow, do not depend on their order (so the token
-// is reproducible, atomics and all) and are within 2^-44 of the weights' at a vocabulary of 2^18. The
-// 64-bit weights bound a large batch: ~11 double-precision operations each, on units that do 64 a cycle.
+// Weights exp(l - max) are rounded to multiples of 2^-40 and summed as 64-bit integers: the sums cannot
+// overflow, and do not depend on their order, so a token is reproducible, atomics and all.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -35,9 +33,11 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kLevels = 2048;
+constexpr float kPerNat = 128.0f;      // levels of max - logit: 16 and more is the last
 constexpr int kGather = 1024;          // ids of the border's level that are ranked at once
 constexpr uint32_t kSmemIds = 40960;   // ids of a share that stay in shared memory
 constexpr uint64_t kMantissa = (1ull << 52) - 1;
+constexpr int kShift = 40;             // weights are multiples of 2^-40: 2^22 of them stay below 2^63
 
 struct Rows {
     GtmSamplingRow v[GTM_SAMPLE_MAX_ROWS];
@@ -50,7 +50,6 @@ struct SampleArgs {
     uint32_t *token, *kept;
     float* logprob;
     uint32_t vocab, slice;   // ids per CTA, a multiple of 1024
-    int shift;               // weights are multiples of 2^-shift
     bool vec, resident;      // 16-byte loads; the share stays in shared memory
 };
 
@@ -69,10 +68,11 @@ __device__ __forceinline__ unsigned long long key_of(float x, uint32_t id) {
 
 struct Shared {
     double power[256];                  // 2^(j / 256)
+    int power10[1024];                  // 2^(j / 1024) in units of 2^-30
     unsigned long long mass[kLevels];   // also the gathered keys
     uint32_t count[kLevels];
     unsigned long long warp_mass[kWarps], warp_mass2[kWarps];
-    double warp_lo[kWarps], warp_hi[kWarps];
+    float warp_lo[kWarps], warp_hi[kWarps];
     uint32_t warp_count[kWarps];
     unsigned long long cta_key, cta_mass, cta_mass2, draw_mass, border_key;   // each read by the peers: none is reused
     uint32_t tie_count, draw_count, gathered;
@@ -82,27 +82,90 @@ struct Shared {
     uint32_t pick_count;
 };
 
-// exp(d * ln 2 / rate') as a multiple of 2^-shift, rate = 256 log2(e) / temperature: 2^(y / 256) with y =
-// k + r, |r| <= 1/2, from a table of 2^(j / 256) and the exponential series to the fourth power of
-// r ln 2 / 256 (the next term is below 2^-54).
-__device__ __forceinline__ unsigned long long fixed_exp(const double* power, double d, double rate, int shift) {
+// exp((x - top) / temperature) as a multiple of 2^-40. Two forms:
+//   exact: 2^(y / 256) with y = 256 log2(e) (x - top) / temperature = k + r, |r| <= 1/2, from a table of
+//     2^(j / 256) and the exponential series to the fourth power of r ln 2 / 256 (the next term is below 2^-54);
+//   short, for weights below 2^-10, i.e. most ids, in ~25 instructions: 2^(y / 1024) with y = c x - c top,
+//     c = 1024 log2(e) / temperature as a sum of two floats and c top as an integer and a float; r is an fma of
+//     an exact product (|r| <= 1, off by 2^-23), the series goes to its square in fp32 and is multiplied with
+//     the table's 30 bits in integers: off by about 2^-31 of the weight, so by 2^-41.
+// Which form an id takes depends on its logit alone, so equal logits weigh the same.
+struct Scale {
+    double rate;         // 256 log2(e) / temperature
+    float hi, lo;        // 1,024 log2(e) / temperature as a sum of two floats; hi NaN: no short form
+    float top_f;         // c top - top_i
+    int top_i;
+};
+__device__ __forceinline__ Scale scale_of(double temperature, float top) {
+    constexpr double kLog2e = 1.4426950408889634074;
+    Scale c;
+    c.rate = 256.0 * kLog2e / temperature;
+    const double ten = 4.0 * c.rate, at = ten * top;
+    c.hi = static_cast<float>(ten);
+    c.lo = static_cast<float>(ten - static_cast<double>(c.hi));
+    if (fabs(at) < 2097152.0) {   // 2^21: products c x that matter stay below 2^22, where their integers are exact
+        c.top_i = __double2int_rn(at);
+        c.top_f = static_cast<float>(at - c.top_i);
+    } else {
+        c.hi = __int_as_float(0x7FC00000);
+        c.lo = c.top_f = 0.0f;
+        c.top_i = 0;
+    }
+    return c;
+}
+__device__ __noinline__ unsigned long long exact_exp(const double* power, double d, double rate) {
     constexpr double kLn = 0.69314718055994530942 / 256.0;
     const double y = d * rate;
-    if (!(y > -16000.0)) return 0;   // below 2^-62
+    if (!(y > -256.0 * 42)) return 0;   // below half of 2^-41; also x = -infinity
     const double t = y + 6755399441055744.0;   // 1.5 * 2^52: the nearest integer in the low word
     const int k = __double2loint(t);
     const double r = y - (t - 6755399441055744.0);
     double p = fma(r, kLn * kLn * kLn * kLn / 24.0, kLn * kLn * kLn / 6.0);
     p = fma(p, r, kLn * kLn / 2.0);
     p = fma(p, r, kLn);
-    p = fma(p, r, 1.0);
-    const unsigned long long m = (static_cast<unsigned long long>(__double_as_longlong(p * power[k & 255])) & kMantissa) | (1ull << 52);
-    // p * power is within [1, 2) except for a rounding to just below 1 or to 2, where the exponent moves by one
-    const int e = static_cast<int>(static_cast<unsigned>(__double2hiint(p * power[k & 255])) >> 20) - 1023;
-    const int s = 52 - shift - (k >> 8) - e;
-    if (s > 60) return 0;
-    return s > 0 ? (m + (1ull << (s - 1))) >> s : m << -s;
+    p = fma(p, r, 1.0) * power[k & 255];   // [1, 2), or just beside it by a rounding
+    const unsigned long long m = (static_cast<unsigned long long>(__double_as_longlong(p)) & kMantissa) | (1ull << 52);
+    const int s = 52 - kShift - (k >> 8) - (static_cast<int>(static_cast<unsigned>(__double2hiint(p)) >> 20) - 1023);
+    return (m + (1ull << (s - 1))) >> s;   // 11 <= s <= 55
 }
+// The short form where it holds; else `big` is set (x = -infinity, and whatever is below 2^-42, among them).
+__device__ __forceinline__ uint32_t short_exp(const Shared& sh, float x, const Scale& c, bool& big) {
+    const float t = __fmaf_rn(x, c.hi, 12582912.0f);   // 1.5 * 2^23: the nearest integer in the low bits
+    const int k = __float_as_int(t) - 0x4B400000 - c.top_i;
+    big = static_cast<uint32_t>(k + 42 * 1024) >= 32u * 1024;   // a t beyond its range gives a k beyond this one
+    float r = __fmaf_rn(x, c.hi, -__fsub_rn(t, 12582912.0f));
+    r = __fsub_rn(__fmaf_rn(x, c.lo, r), c.top_f);
+    constexpr float kLn = 0.69314718055994530942f / 1024.0f;
+    // (z + z^2 / 2) * 2^32 with z = r kLn, to the nearest integer (below 2^22 in magnitude)
+    const float g = __fmaf_rn(r, 0.5f * kLn * kLn * 4294967296.0f, kLn * 4294967296.0f);
+    const int p = __float_as_int(__fmaf_rn(r, g, 12582912.0f)) - 0x4B400000;
+    const int m = sh.power10[k & 1023];
+    const uint32_t w = static_cast<uint32_t>(m + __mulhi(m, p)) >> ((-11 - (k >> 10)) & 31);   // twice the weight
+    return big ? 0u : (w + 1) >> 1;
+}
+__device__ __forceinline__ unsigned long long fixed_exp(const Shared& sh, float x, float top, const Scale& c) {
+    bool big;
+    const uint32_t w = short_exp(sh, x, c, big);
+    return big ? exact_exp(sh.power, static_cast<double>(x) - static_cast<double>(top), c.rate) : w;
+}
+// Sums weights with the exact forms put off: they are few, and a warp that stops for each holds up the others.
+struct Summer {
+    unsigned long long sum = 0;
+    float put_off = -INFINITY;
+    __device__ __forceinline__ void add(const Shared& sh, float x, float top, const Scale& c) {
+        bool big;
+        sum += short_exp(sh, x, c, big);
+        if (big && x > -INFINITY) {
+            if (put_off > -INFINITY) sum += exact_exp(sh.power, static_cast<double>(put_off) - static_cast<double>(top), c.rate);
+            put_off = x;
+        }
+    }
+    __device__ __forceinline__ unsigned long long total(const Shared& sh, float top, const Scale& c) {
+        if (put_off > -INFINITY) sum += exact_exp(sh.power, static_cast<double>(put_off) - static_cast<double>(top), c.rate);
+        put_off = -INFINITY;
+        return sum;
+    }
+};
 
 __device__ __forceinline__ unsigned long long warp_sum(unsigned long long x) {
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
@@ -132,6 +195,8 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
     auto logit = [&](uint32_t i) { return a.resident ? slice_s[i] : as_logit(__ldg(src + base + i)); };
 
     // ---- 1: the largest logit and its lowest id
+    if (tid < 256) sh.power[tid] = exp2(tid * (1.0 / 256.0));
+    sh.power10[tid] = __double2int_rn(exp2(tid * (1.0 / 1024.0)) * 1073741824.0);
     unsigned long long best = 0;
     auto look = [&](uint32_t i, float x) {
         x = i < n ? as_logit(x) : -INFINITY;
@@ -140,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
         return x;
     };
     if (a.resident && a.vec) {
-        constexpr int U = 4;   // loads in flight per thread
+        constexpr int U = 8;   // loads in flight per thread
         for (uint32_t i0 = tid * 4; i0 < n4; i0 += kThreads * 4 * U) {
             float4 x[U];
 #pragma unroll
@@ -167,7 +232,6 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
             if (a.resident) slice_s[i] = x;
         }
     }
-    if (tid < 256) sh.power[tid] = exp2(tid * (1.0 / 256.0));
     for (int i = tid; i < kLevels; i += kThreads) sh.count[i] = 0;
     if (tid == 0) sh.first = kLevels, sh.last = kLevels, sh.by_count = kLevels, sh.gathered = 0, sh.pick = kLevels;
     for (int o = 16; o > 0; o >>= 1) {
@@ -202,14 +266,23 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
         cluster.sync();   // no CTA leaves while another may read its shared memory
         return;
     }
-    constexpr double kRate = 256.0 * 1.4426950408889634074;
+    const Scale one = scale_of(1.0, top);
     const double top_d = top;
-    auto weight = [&](float x) { return fixed_exp(sh.power, static_cast<double>(x) - top_d, kRate, a.shift); };
-    auto level = [&](float x) { return static_cast<uint32_t>(fminf((top - x) * 64.0f, kLevels - 1.0f)); };
+    auto weight = [&](float x) { return fixed_exp(sh, x, top, one); };
+    // the nearest level, in the low bits of a float of 2^23 or more
+    auto level = [&](float x) { return __float_as_uint(fminf(fmaf(top - x, kPerNat, 8388608.0f), 8388607.0f + kLevels)) - 0x4B000000u; };
     const bool greedy = !(rule.temperature > 0.0f);
     const bool cut_p = !greedy && rule.top_p < 1.0f, cut_k = !greedy && rule.top_k > 0 && static_cast<uint32_t>(rule.top_k) < a.vocab;
-    // ids with p below min_p of the largest are out of the draw
-    const double floor_d = !greedy && rule.min_p > 0.0f ? log(static_cast<double>(rule.min_p)) : -INFINITY;
+    // ids with a key below `border` are out: at first those without a finite logit, and those with p below
+    // min_p of the largest, by the least logit that is not
+    unsigned long long border = static_cast<unsigned long long>(ordered(-3.402823466e38f)) << 32;
+    if (!greedy && rule.min_p > 0.0f) {
+        const double floor_d = log(static_cast<double>(rule.min_p));
+        uint32_t o = ordered(static_cast<float>(top_d + floor_d));
+        while (o < ordered(top) && !(static_cast<double>(from_ordered(o)) - top_d >= floor_d)) ++o;
+        while (o > ordered(-3.402823466e38f) && static_cast<double>(from_ordered(o - 1)) - top_d >= floor_d) --o;
+        border = static_cast<unsigned long long>(o) << 32;
+    }
 
     // ---- 2a: counts per level, and the bracket
     uint32_t first = kLevels, last = kLevels;
@@ -234,33 +307,34 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
         // two levels per thread: counts and bounds of the mass down to and including each
         static_assert(kLevels == 2 * kThreads, "");
         const uint32_t c0 = sh.count[2 * tid], c1 = sh.count[2 * tid + 1];
-        // a level's edges are off by the rounding of (max - l) * 64 and by the weights' own: 2^-12 covers both
-        const double q0 = exp(-(2 * tid) / 64.0) * (1 + 0x1p-12), q1 = exp(-(2 * tid + 1) / 64.0), q2 = exp(-(2 * tid + 2) / 64.0) * (1 - 0x1p-12);
-        double lo0 = c0 * q1 * (1 - 0x1p-12), hi0 = c0 * q0, lo1 = tid == kThreads - 1 ? 0.0 : c1 * q2, hi1 = c1 * q1 * (1 + 0x1p-12);
+        // a level's edges are off by the rounding of (max - l) * 128, its mass by fp32 sums and exponentials: 2^-12
+        // covers them all
+        constexpr float kMore = 1.0f + 0x1p-12f, kLess = 1.0f - 0x1p-12f;
+        const float q0 = expf((0.5f - 2.0f * tid) / kPerNat), q1 = expf((-0.5f - 2.0f * tid) / kPerNat), q2 = expf((-1.5f - 2.0f * tid) / kPerNat);
+        const float lo0 = c0 * q1 * kLess, hi0 = c0 * q0 * kMore, lo1 = tid == kThreads - 1 ? 0.0f : c1 * q2 * kLess, hi1 = c1 * q1 * kMore;
         uint32_t pc = c0 + c1;
-        double pl = lo0 + lo1, ph = hi0 + hi1;
+        float pl = lo0 + lo1, ph = hi0 + hi1;
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t uc = __shfl_up_sync(0xffffffffu, pc, o);
-            const double ul = __shfl_up_sync(0xffffffffu, pl, o), uh = __shfl_up_sync(0xffffffffu, ph, o);
+            const float ul = __shfl_up_sync(0xffffffffu, pl, o), uh = __shfl_up_sync(0xffffffffu, ph, o);
             if (lane >= o) pc += uc, pl += ul, ph += uh;
         }
         if (lane == 31) sh.warp_count[warp] = pc, sh.warp_lo[warp] = pl, sh.warp_hi[warp] = ph;
         __syncthreads();
         uint32_t bc = 0;
-        double bl = 0.0, bh = 0.0, all_lo = 0.0, all_hi = 0.0;
+        float bl = 0.0f, bh = 0.0f, all_lo = 0.0f, all_hi = 0.0f;
         for (int w = 0; w < kWarps; ++w) {
             if (w < warp) bc += sh.warp_count[w], bl += sh.warp_lo[w], bh += sh.warp_hi[w];
             all_lo += sh.warp_lo[w], all_hi += sh.warp_hi[w];
         }
-        const double p = rule.top_p;
         const uint32_t cum1 = bc + pc, cum0 = cum1 - c1;
-        const double l1 = bl + pl, l0 = l1 - lo1, h1 = bh + ph, h0 = h1 - hi1;
-        if (cut_p) {   // sums of doubles are off by far less than 2^-20
-            const double low = p * all_lo * (1 - 0x1p-20), high = p * all_hi * (1 + 0x1p-20);
-            if (c0 && h0 >= low) atomicMin(&sh.first, 2 * tid);
-            if (c1 && h1 >= low) atomicMin(&sh.first, 2 * tid + 1);
-            if (c0 && l0 >= high) atomicMin(&sh.last, 2 * tid);
-            if (c1 && l1 >= high) atomicMin(&sh.last, 2 * tid + 1);
+        const float l1 = bl + pl, l0 = bl + (pl - lo1), h1 = bh + ph, h0 = bh + (ph - hi1);
+        if (cut_p) {
+            const float low = rule.top_p * all_lo * kLess, high = rule.top_p * all_hi * kMore;
+            if (c0 && h0 * kMore >= low) atomicMin(&sh.first, 2 * tid);
+            if (c1 && h1 * kMore >= low) atomicMin(&sh.first, 2 * tid + 1);
+            if (c0 && l0 * kLess >= high) atomicMin(&sh.last, 2 * tid);
+            if (c1 && l1 * kLess >= high) atomicMin(&sh.last, 2 * tid + 1);
         }
         if (cut_k) {
             if (c0 && cum0 >= static_cast<uint32_t>(rule.top_k)) atomicMin(&sh.by_count, 2 * tid);
@@ -280,23 +354,29 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
     // ---- 2b: exact sums: the whole distribution, the levels above the bracket, each level in it
     unsigned long long whole = 0, above_mass = 0;
     {
-        unsigned long long sum = 0, up = 0;
+        Summer every, over;
+        // below every id of the bracket
+        const float low = !(bracket && cut_p) ? INFINITY : last == kLevels - 1u ? -3.402823466e38f : top - (static_cast<float>(last) + 1.0f) / kPerNat;
         for (uint32_t i = tid * 4; i < n; i += kThreads * 4) {
             const float4 x4 = four(i);
             const float x[4] = {x4.x, x4.y, x4.z, x4.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const unsigned long long w = x[j] > -INFINITY ? weight(x[j]) : 0ull;
-                sum += w;
-                if (cut_p && w) {
+            for (int j = 0; j < 4; ++j) every.add(sh, x[j], top, one);
+            const float most = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+            if (most >= low) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
                     const uint32_t lev = level(x[j]);
-                    if (lev < first)
-                        up += w;
-                    else if (lev <= last)
-                        atomicAdd(&sh.mass[lev - first], w);
+                    if (x[j] >= low && lev <= last) {
+                        if (lev < first)
+                            over.add(sh, x[j], top, one);
+                        else
+                            atomicAdd(&sh.mass[lev - first], weight(x[j]));
+                    }
                 }
             }
         }
+        unsigned long long sum = every.total(sh, top, one), up = over.total(sh, top, one);
         sum = warp_sum(sum), up = warp_sum(up);
         if (lane == 0) sh.warp_mass[warp] = sum, sh.warp_mass2[warp] = up;
         __syncthreads();
@@ -311,8 +391,8 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
         }
     }
     uint32_t above = 0, border_level = kLevels, ties = 0xFFFFFFFFu;
-    unsigned long long need = 0, border = 0;   // ids with a key below `border` are out
-    bool tied = false;                         // and of those with the border's logit only the first `ties` stay
+    unsigned long long need = 0;
+    bool tied = false;   // of the ids with the border's logit only the first `ties` stay
     if (bracket) {
         need = cut_p ? static_cast<unsigned long long>(ceil(static_cast<double>(rule.top_p) * static_cast<double>(whole))) : ~0ull;
         above = sh.pick_count;
@@ -375,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
                 __syncthreads();
             }
             cluster.sync();
-            border = *cluster.map_shared_rank(&sh.border_key, 0);
+            border = max(border, *cluster.map_shared_rank(&sh.border_key, 0));
         } else {
             uint32_t lo = 0, bits = 32;   // the border's logit has these high bits
             for (int pass = 0; pass < 3; ++pass) {
@@ -443,8 +523,8 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
                         const unsigned long long t = (need - above_mass + w - 1) / w;
                         ties = t < ties ? static_cast<uint32_t>(t) : ties;
                     }
-                    border = static_cast<unsigned long long>(lo) << 32;
-                    tied = true;
+                    tied = static_cast<unsigned long long>(lo) << 32 >= border;   // else min_p leaves fewer
+                    border = max(border, static_cast<unsigned long long>(lo) << 32);
                 }
                 __syncthreads();
             }
@@ -453,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
 
     // ---- 3: the draw
     if (!greedy) {
-        const double rate = kRate / static_cast<double>(rule.temperature);
+        const Scale heat = scale_of(rule.temperature, top);
         const uint32_t edge = static_cast<uint32_t>(border >> 32);
         const uint32_t run = a.slice / kWarps;   // a warp's run of ids, a multiple of 32
         const uint32_t r0 = min(n, warp * run), r1 = min(n, r0 + run);
@@ -474,10 +554,12 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
             for (int w = 0; w < warp; ++w) ties_before += sh.warp_count[w];
             cluster.sync();
         }
-        auto in_cuts = [&](float x, uint32_t i) {
-            return x > -INFINITY && key_of(x, base + i) >= border && static_cast<double>(x) - top_d >= floor_d;
+        const float edge_x = from_ordered(edge);
+        const uint32_t least = static_cast<uint32_t>(border);
+        auto in_cuts = [&](float x, uint32_t i) {   // key_of(x, base + i) >= border
+            return x > edge_x || (x == edge_x && ~(base + i) >= least);
         };
-        auto mass = [&](float x) { return fixed_exp(sh.power, static_cast<double>(x) - top_d, rate, a.shift); };
+        auto mass = [&](float x) { return fixed_exp(sh, x, top, heat); };
         // lane's id of the 32 from i0 on: whether it is kept; `seen` counts the ties so far (the whole warp calls it)
         auto keep_tied = [&](uint32_t i0, uint32_t& seen) {
             const uint32_t i = i0 + lane;
@@ -488,15 +570,26 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
             seen += __popc(vote);
             return keep;
         };
-        unsigned long long sum = 0;
+        Summer draw;
         uint32_t count = 0, seen = ties_before;
-        for (uint32_t i0 = r0; i0 < r1; i0 += 32) {
-            const uint32_t i = i0 + lane;
-            const float x = i < r1 ? logit(i) : -INFINITY;
-            const bool keep = tied ? keep_tied(i0, seen) : in_cuts(x, i);
-            if (keep) sum += mass(x), ++count;
+        if (tied) {
+            for (uint32_t i0 = r0; i0 < r1; i0 += 32) {
+                const uint32_t i = i0 + lane;
+                if (keep_tied(i0, seen)) draw.add(sh, logit(i), top, heat), ++count;
+            }
+        } else {
+            for (uint32_t i0 = r0; i0 < r1; i0 += 128) {
+                const uint32_t i = i0 + 4 * lane;
+                const float4 x4 = i < r1 ? four(i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                const float x[4] = {x4.x, x4.y, x4.z, x4.w};
+                const float most = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                if (!__any_sync(0xffffffffu, most >= edge_x)) continue;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (in_cuts(x[j], i + j)) draw.add(sh, x[j], top, heat), ++count;
+            }
         }
-        sum = warp_sum(sum);
+        const unsigned long long sum = warp_sum(draw.total(sh, top, heat));
         for (int o = 16; o > 0; o >>= 1) count += __shfl_xor_sync(0xffffffffu, count, o);
         if (lane == 0) sh.warp_mass[warp] = sum, sh.warp_count[warp] = count;
         __syncthreads();
@@ -537,12 +630,13 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
                 }
             } else {
                 for (uint32_t g0 = r0; g0 < r1; g0 += 1024) {
-                    unsigned long long s = 0;
+                    Summer part;
                     for (int j = 0; j < 32; ++j) {
                         const uint32_t i = g0 + lane * 32 + ((j + lane) & 31);
                         const float x = i < r1 ? logit(i) : -INFINITY;
-                        if (in_cuts(x, i)) s += mass(x);
+                        if (in_cuts(x, i)) part.add(sh, x, top, heat);
                     }
+                    const unsigned long long s = part.total(sh, top, heat);
                     unsigned long long p = s;
                     for (int o = 1; o < 32; o <<= 1) {
                         const unsigned long long up = __shfl_up_sync(0xffffffffu, p, o);
@@ -571,8 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
                 a.token[row] = base + i;
                 if (a.kept) a.kept[row] = kept;
                 if (a.logprob) {
-                    const double unit = __hiloint2double((1023 + a.shift) << 20, 0);
-                    a.logprob[row] = static_cast<float>(static_cast<double>(x) - top_d - log(static_cast<double>(whole) / unit));
+                    a.logprob[row] = static_cast<float>(static_cast<double>(x) - top_d - log(static_cast<double>(whole) * 0x1p-40));
                 }
             }
         }
@@ -580,8 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
         a.token[row] = top_id;
         if (a.kept) a.kept[row] = 1;
         if (a.logprob) {
-            const double unit = __hiloint2double((1023 + a.shift) << 20, 0);
-            a.logprob[row] = static_cast<float>(-log(static_cast<double>(whole) / unit));
+            a.logprob[row] = static_cast<float>(-log(static_cast<double>(whole) * 0x1p-40));
         }
     }
     cluster.sync();   // no CTA leaves while another may read its shared memory
@@ -644,9 +736,6 @@ extern "C" GTM_API int gtm_sample_rows(const float* logits, uint32_t n, uint32_t
     a.logits = logits, a.row_stride = row_stride, a.uniform = uniform;
     a.token = token, a.kept = kept, a.logprob = logprob;
     a.vocab = vocab;
-    int bits = 0;
-    while ((1u << bits) < vocab) ++bits;
-    a.shift = std::min(52, 62 - bits);
     a.vec = aligned(logits, 16) && (n == 1 || row_stride % 4 == 0);
     const cudaError_t e = getenv("CL16") ? launch<16>(a, r, n, static_cast<cudaStream_t>(stream)) : launch<8>(a, r, n, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) {
