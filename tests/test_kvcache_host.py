@@ -169,7 +169,7 @@ def test_python_wrappers_check_shapes_and_types():
             c.write(args.pop("q"), args.pop("k"), args.pop("v"), args.pop("q_out"), args.pop("positions"), args.pop("seqs"), **args)
     a = np.arange(3, dtype=np.uint32)
     p, owner = _u32(a, 3)
-    assert p.value == a.ctypes.data and owner is a
+    assert p == a.ctypes.data and owner is a
     s = RowSampler(10, 2, device="cpu")
     with pytest.raises(gtmoe.GtmError):
         s(torch.zeros(3, 10), [RowParams()] * 3)

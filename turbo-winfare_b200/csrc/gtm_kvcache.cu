@@ -216,13 +216,15 @@ __global__ void __launch_bounds__(kWriteWarps * 32) kv_write(const __grid_consta
     }
 }
 
-// kv_read: 16 codes a thread, 16 bytes in and 64 out; blockIdx.y: keys or values.
+// kv_read: a CTA reads kReadRows positions of the keys or of the values (blockIdx.y), four codes a thread and
+// load: a warp takes 128 bytes in and 512 out, the loads of all its rows before the first store.
+constexpr int kReadRows = 8;
 struct ReadArgs {
     const uint8_t* codes[2];
     const float* scale[2];
     float* out[2];
-    uint64_t chunks;            // 16-code pieces of one output
-    uint32_t start, capacity, kv_heads, per_vec;   // ring row of the first position; pieces of a vector
+    uint32_t count, start, capacity, words, shift;   // start: ring row of the first position; words
+                                                               // of four codes in a row, 2^shift of them a vector
 };
 
 template <int FMT>
@@ -239,20 +241,26 @@ __device__ __forceinline__ float2 code_pair(uint32_t two) {   // the low 16 bits
 template <int FMT>
 __global__ void __launch_bounds__(256) kv_read(const __grid_constant__ ReadArgs a) {
     const int which = a.out[0] && blockIdx.y == 0 ? 0 : 1;
-    const uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (i >= a.chunks) return;
-    const uint32_t per_row = a.per_vec * a.kv_heads;
-    const uint32_t t = static_cast<uint32_t>(i / per_row), c = static_cast<uint32_t>(i % per_row);
-    uint64_t slot = static_cast<uint64_t>(a.start) + t;
-    if (slot >= a.capacity) slot -= a.capacity;
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(a.codes[which]) + slot * per_row + c);
-    const float s = __ldg(a.scale[which] + static_cast<size_t>(c / a.per_vec) * a.capacity + slot);
-    float4* o = reinterpret_cast<float4*>(a.out[which]) + i * 4;
-    const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(a.codes[which]);
+    float4* out = reinterpret_cast<float4*>(a.out[which]);
+    const uint32_t t0 = blockIdx.x * kReadRows;
+    for (uint32_t w = threadIdx.x; w < a.words; w += 256) {
+        const float* scale = a.scale[which] + static_cast<size_t>(w >> a.shift) * a.capacity;
+        uint32_t word[kReadRows];
+        float s[kReadRows];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float2 lo = code_pair<FMT>(wd[j]), hi = code_pair<FMT>(wd[j] >> 16);
-        o[j] = make_float4(lo.x * s, lo.y * s, hi.x * s, hi.y * s);
+        for (int r = 0; r < kReadRows; ++r) {
+            uint64_t slot = static_cast<uint64_t>(a.start) + min(t0 + r, a.count - 1);
+            if (slot >= a.capacity) slot -= a.capacity;
+            word[r] = __ldg(codes + slot * a.words + w);
+            s[r] = __ldg(scale + slot);
+        }
+#pragma unroll
+        for (int r = 0; r < kReadRows; ++r) {
+            const float2 lo = code_pair<FMT>(word[r]), hi = code_pair<FMT>(word[r] >> 16);
+            if (t0 + r < a.count)
+                __stcs(out + static_cast<size_t>(t0 + r) * a.words + w, make_float4(lo.x * s[r], lo.y * s[r], hi.x * s[r], hi.y * s[r]));
+        }
     }
 }
 
@@ -305,8 +313,7 @@ GTM_API int gtm_qkv_cache_rows(const GtmKvCache* c, uint32_t q_heads, uint32_t n
     }
     if (n > kMaxBatchRows) return set_error(GTM_ERR_INVALID, "%s: n=%u rows (at most %u)", fn, n, kMaxBatchRows);
     if (!q || !k || !v || !q_out || !positions || !seqs) return set_error(GTM_ERR_INVALID, "%s: null pointer", fn);
-    if (q_heads == 0 || q_heads > 65535u || c->kv_heads > 65535u)
-        return set_error(GTM_ERR_UNSUPPORTED, "%s: q_heads=%u kv_heads=%u (1..65535)", fn, q_heads, c->kv_heads);
+    if (q_heads == 0 || q_heads > 65535u) return set_error(GTM_ERR_UNSUPPORTED, "%s: q_heads=%u (1..65535)", fn, q_heads);
     const uint64_t q_width = static_cast<uint64_t>(q_heads) * c->head_dim, kv_width = static_cast<uint64_t>(c->kv_heads) * c->head_dim;
     if (n > 1 && (q_stride < q_width || k_stride < kv_width || v_stride < kv_width))
         return set_error(GTM_ERR_INVALID, "%s: row strides %llu, %llu, %llu below the rows' widths", fn,
@@ -377,14 +384,12 @@ GTM_API int gtm_kv_read(const GtmKvCache* c, uint32_t seq, uint32_t first, uint3
     a.codes[0] = static_cast<const uint8_t*>(c->k_dev) + codes, a.codes[1] = static_cast<const uint8_t*>(c->v_dev) + codes;
     a.scale[0] = c->k_scale_dev + scales, a.scale[1] = c->v_scale_dev + scales;
     a.out[0] = k_out, a.out[1] = v_out;
-    a.per_vec = c->head_dim / 16;
-    a.kv_heads = c->kv_heads;
-    a.chunks = static_cast<uint64_t>(count) * c->kv_heads * a.per_vec;
+    a.words = c->kv_heads * (c->head_dim / 4);
+    a.shift = c->head_dim == 128 ? 5 : c->head_dim == 256 ? 6 : 7;
+    a.count = count;
     a.start = first % c->capacity;
     a.capacity = c->capacity;
-    const uint64_t blocks = (a.chunks + 255) / 256;
-    if (blocks > 0x7FFFFFFFull) return set_error(GTM_ERR_UNSUPPORTED, "%s: %u positions of %u heads", fn, count, c->kv_heads);
-    const dim3 grid(static_cast<uint32_t>(blocks), k_out && v_out ? 2 : 1);
+    const dim3 grid((count - 1) / kReadRows + 1, k_out && v_out ? 2 : 1);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (c->format == GTM_KV_INT8)
         kv_read<GTM_KV_INT8><<<grid, 256, 0, st>>>(a);

@@ -31,6 +31,7 @@ inline int check_kv(const char* fn, const char* what, const GtmKvCache* c) {
     if (c->num_seqs == 0 || c->capacity == 0 || c->kv_heads == 0 || c->reserved != 0)
         return set_error(GTM_ERR_INVALID, "%s: %s of %u sequences, %u positions, %u heads, reserved %u", fn, what,
                          c->num_seqs, c->capacity, c->kv_heads, c->reserved);
+    if (c->kv_heads > 65535u) return set_error(GTM_ERR_UNSUPPORTED, "%s: %s of %u heads (at most 65535)", fn, what, c->kv_heads);
     if (!ptr_aligned(c->k_dev, 16) || !ptr_aligned(c->v_dev, 16) || !ptr_aligned(c->k_scale_dev, 4) ||
         !ptr_aligned(c->v_scale_dev, 4))
         return set_error(GTM_ERR_MISALIGNED, "%s: %s codes need 16-byte alignment, scales 4", fn, what);

@@ -6,10 +6,10 @@
 //   1 the largest logit, and its lowest id;
 //   2 the cuts. Ranked by logit, every cut keeps a run from the top, so the kept set is the ids whose
 //     key (logit, then lower id) is at least a border's. Ids are counted per level of max - logit,
-//     1/128 wide; a level's weights agree within 0.8%, so the counts alone bracket the nucleus' border
-//     to a few levels. One pass then sums the exact weights (all, above the bracket, per level in
-//     it), and the ids of the level that holds the border are gathered and ranked. More ids than the
-//     gather holds (equal or nearly equal logits) are narrowed by the logit's ordered bits instead;
+//     1/128 wide where it counts; a level's weights agree within 0.8%, so the counts alone bracket the
+//     nucleus' border to a few levels. One pass sums the exact weights (all of them, and those above the bracket) and
+//     gathers the bracket's ids, among which one CTA finds the border by halves. A bracket of more than 4,096 ids (nearly equal
+//     logits) is narrowed by its levels' masses and then by the logit's ordered bits instead;
 //   3 the draw: sums of the kept weights per warp's run of ids, CTA and cluster, then one warp finds
 //     the id in the run that the target falls in.
 // Weights exp(l - max) are rounded to multiples of 2^-40 and summed as 64-bit integers: the sums cannot
@@ -20,7 +20,6 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
-#include <cstdlib>
 
 #include "gtm_internal.h"
 #include "gtmoe_sampling.h"
@@ -33,11 +32,38 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kLevels = 2048;
-constexpr float kPerNat = 128.0f;      // levels of max - logit: 16 and more is the last
-constexpr int kGather = 1024;          // ids of the border's level that are ranked at once
+// Levels of max - logit: 1/128 wide up to 8, then three times as wide; 32 and more is the last.
+constexpr float kFine = 128.0f, kCoarse = 128.0f / 3.0f, kOne = 8388608.0f;   // 2^23: a float's integers from here on
+// The nearest level, in the low bits of a float; monotone in d.
+__device__ __forceinline__ float near_level(float d) {
+    return fminf(fmaf(d, kFine, kOne), fmaf(d, kCoarse, kOne + 2048.0f / 3.0f));
+}
+__device__ __forceinline__ float level_middle(int level) { return level <= 1024 ? level / kFine : 8.0f + (level - 1024) / kCoarse; }
+constexpr uint32_t kGather = 4096;     // ids of a bracket that are gathered
 constexpr uint32_t kSmemIds = 40960;   // ids of a share that stay in shared memory
-constexpr uint64_t kMantissa = (1ull << 52) - 1;
-constexpr int kShift = 40;             // weights are multiples of 2^-40: 2^22 of them stay below 2^63
+constexpr int kGroups = 10;            // parts of a warp's run of ids in the draw (128 ids of a share in shared memory)
+
+// 2^(j / 1024) in units of 2^-62, from the exponential series in 64-bit arithmetic at compile time.
+struct PowerTable {
+    unsigned long long v[1024];
+    constexpr PowerTable() : v() {
+        for (int j = 0; j < 1024; ++j) {
+            // 2^(j / 1024) = e^z, z < 0.7, as 1 + z (1 + z / 2 (1 + z / 3 (...))) in units of 2^-62
+            constexpr unsigned long long kLn2 = 3196577161300663914ull;   // ln 2 in units of 2^-62
+            const unsigned long long z = kLn2 / 1024 * j + kLn2 % 1024 * j / 1024;
+            unsigned long long sum = 1ull << 62;
+            for (int i = 24; i > 0; --i) sum = (1ull << 62) + mul62(z, sum) / i;
+            v[j] = sum;
+        }
+    }
+    static constexpr unsigned long long mul62(unsigned long long a, unsigned long long b) {   // a b / 2^62
+        const unsigned long long ah = a >> 32, al = a & 0xFFFFFFFFu, bh = b >> 32, bl = b & 0xFFFFFFFFu;
+        const unsigned long long mid = (al * bl >> 32) + (ah * bl & 0xFFFFFFFFu) + (al * bh & 0xFFFFFFFFu);
+        const unsigned long long hi = ah * bh + (ah * bl >> 32) + (al * bh >> 32) + (mid >> 32);
+        return (hi << 2) | (mid >> 30 & 3u);
+    }
+};
+__device__ const PowerTable kPowers;
 
 struct Rows {
     GtmSamplingRow v[GTM_SAMPLE_MAX_ROWS];
@@ -66,107 +92,128 @@ __device__ __forceinline__ unsigned long long key_of(float x, uint32_t id) {
     return (static_cast<unsigned long long>(ordered(x)) << 32) | static_cast<uint32_t>(~id);
 }
 
-struct Shared {
-    double power[256];                  // 2^(j / 256)
-    int power10[1024];                  // 2^(j / 1024) in units of 2^-30
-    unsigned long long mass[kLevels];   // also the gathered keys
+struct __align__(16) Shared {
+    unsigned long long power62[1024];   // 2^(j / 1024) in units of 2^-62
+    int power30[1024];                  // and of 2^-30
+    unsigned long long mass[kGather];   // masses of levels, or the gathered ids' keys
     uint32_t count[kLevels];
-    unsigned long long warp_mass[kWarps], warp_mass2[kWarps];
-    float warp_lo[kWarps], warp_hi[kWarps];
+    unsigned long long key_lo, key_hi;  // of the gathered ids
+    uint3 half[2][kWarps];
+    unsigned long long warp_mass[kWarps], warp_mass2[kWarps], group_mass[kWarps][kGroups];
+    float warp_near[kWarps], warp_var[kWarps];
     uint32_t warp_count[kWarps];
     unsigned long long cta_key, cta_mass, cta_mass2, draw_mass, border_key;   // each read by the peers: none is reused
-    uint32_t tie_count, draw_count, gathered;
+    double floor_d;                     // log(min_p)
+    float scale[3];                     // 1,024 log2(e) / temperature as a sum
+    uint32_t tie_count, draw_count, gathered, members, border_at;
     uint32_t first, last, by_count;     // the bracket's levels; the level that holds the top_k-th id
     uint32_t pick;                      // the level that holds the border
     unsigned long long pick_mass;       // mass and count of the levels above it
     uint32_t pick_count;
 };
 
-// exp((x - top) / temperature) as a multiple of 2^-40. Two forms:
-//   exact: 2^(y / 256) with y = 256 log2(e) (x - top) / temperature = k + r, |r| <= 1/2, from a table of
-//     2^(j / 256) and the exponential series to the fourth power of r ln 2 / 256 (the next term is below 2^-54);
-//   short, for weights below 2^-10, i.e. most ids, in ~25 instructions: 2^(y / 1024) with y = c x - c top,
-//     c = 1024 log2(e) / temperature as a sum of two floats and c top as an integer and a float; r is an fma of
-//     an exact product (|r| <= 1, off by 2^-23), the series goes to its square in fp32 and is multiplied with
-//     the table's 30 bits in integers: off by about 2^-31 of the weight, so by 2^-41.
+// exp((x - top) / temperature) as a multiple of 2^-40, without double precision, of which this GPU does little.
+// With c = 1024 log2(e) / temperature as a sum of three floats it is 2^(y / 1024), y = c (x - top), in two forms:
+//   short, for weights below 2^-10, i.e. most ids, in ~25 instructions: y = c x - c top, c top as an integer and a
+//     float; y = k + r with r an fma of an exact product (|r| <= 1, off by 2^-23); the series of 2^(r / 1024)
+//     goes to its square in fp32 and is multiplied with 30 bits of a table of 2^(j / 1024): off by about 2^-31
+//     of the weight, so by 2^-41;
+//   exact: x - top as a sum of two floats, the products as sums of two floats each, added as 64-bit integers in
+//     units of 2^-40; the series to its cube (the next term is below 2^-46) and the table's 62 bits in integers.
 // Which form an id takes depends on its logit alone, so equal logits weigh the same.
 struct Scale {
-    double rate;         // 256 log2(e) / temperature
-    float hi, lo;        // 1,024 log2(e) / temperature as a sum of two floats; hi NaN: no short form
+    float hi, lo, lo2;   // c
     float top_f;         // c top - top_i
     int top_i;
+    bool brief;          // the short form may be used
 };
-__device__ __forceinline__ Scale scale_of(double temperature, float top) {
-    constexpr double kLog2e = 1.4426950408889634074;
+__device__ __forceinline__ Scale scale_of(float hi, float lo, float lo2, float top) {
     Scale c;
-    c.rate = 256.0 * kLog2e / temperature;
-    const double ten = 4.0 * c.rate, at = ten * top;
-    c.hi = static_cast<float>(ten);
-    c.lo = static_cast<float>(ten - static_cast<double>(c.hi));
-    if (fabs(at) < 2097152.0) {   // 2^21: products c x that matter stay below 2^22, where their integers are exact
-        c.top_i = __double2int_rn(at);
-        c.top_f = static_cast<float>(at - c.top_i);
-    } else {
-        c.hi = __int_as_float(0x7FC00000);
-        c.lo = c.top_f = 0.0f;
-        c.top_i = 0;
-    }
+    c.hi = hi, c.lo = lo, c.lo2 = lo2;
+    const float p = __fmul_rn(hi, top);
+    c.brief = fabsf(p) < 2097152.0f;   // 2^21: products c x that matter stay below 2^22, where their integers are exact
+    const float n = rintf(p);
+    c.top_i = c.brief ? static_cast<int>(n) : 0;
+    c.top_f = __fadd_rn(__fsub_rn(p, n), __fmaf_rn(lo, top, __fmaf_rn(hi, top, -p)));
     return c;
 }
-__device__ __noinline__ unsigned long long exact_exp(const double* power, double d, double rate) {
-    constexpr double kLn = 0.69314718055994530942 / 256.0;
-    const double y = d * rate;
-    if (!(y > -256.0 * 42)) return 0;   // below half of 2^-41; also x = -infinity
-    const double t = y + 6755399441055744.0;   // 1.5 * 2^52: the nearest integer in the low word
-    const int k = __double2loint(t);
-    const double r = y - (t - 6755399441055744.0);
-    double p = fma(r, kLn * kLn * kLn * kLn / 24.0, kLn * kLn * kLn / 6.0);
-    p = fma(p, r, kLn * kLn / 2.0);
-    p = fma(p, r, kLn);
-    p = fma(p, r, 1.0) * power[k & 255];   // [1, 2), or just beside it by a rounding
-    const unsigned long long m = (static_cast<unsigned long long>(__double_as_longlong(p)) & kMantissa) | (1ull << 52);
-    const int s = 52 - kShift - (k >> 8) - (static_cast<int>(static_cast<unsigned>(__double2hiint(p)) >> 20) - 1023);
-    return (m + (1ull << (s - 1))) >> s;   // 11 <= s <= 55
+__device__ __noinline__ unsigned long long exact_exp(const Shared& sh, float x, float top, float hi, float lo, float lo2) {
+    const float d = __fsub_rn(x, top), b = __fsub_rn(d, x);
+    if (d == 0.0f) return 1ull << 40;
+    const float y = __fmul_rn(d, hi);
+    if (!(y > -42.0f * 1024.0f)) return 0;   // below half of 2^-41
+    const float e = __fsub_rn(__fsub_rn(x, __fsub_rn(d, b)), __fadd_rn(top, b));   // what the difference was rounded by
+    const float q = __fmul_rn(d, lo);
+    constexpr float kUnit = 1099511627776.0f;   // 2^40
+    long long v = __float2ll_rn(y * kUnit) + __float2ll_rn(__fmaf_rn(d, hi, -y) * kUnit);
+    v += __float2ll_rn(q * kUnit) + __float2ll_rn(__fmaf_rn(d, lo, -q) * kUnit);
+    v += __float2ll_rn(__fmaf_rn(d, lo2, __fmaf_rn(e, hi, e * lo)) * kUnit);
+    v = v > 0 ? 0 : v;
+    const int k = static_cast<int>(v >> 40);
+    const unsigned long long r = static_cast<unsigned long long>(v) << 24;              // in units of 2^-64
+    const unsigned long long z = __umul64hi(r, 12486629536330718ull);                   // times ln 2 / 1024
+    const unsigned long long z2 = __umul64hi(z, z) >> 1, z3 = __umul64hi(__umul64hi(z2, z), 6148914691236517205ull);   // / 3
+    const unsigned long long m = sh.power62[k & 1023];
+    const unsigned long long w = m + __umul64hi(m, z + z2 + z3);
+    const int s = 22 - (k >> 10);
+    return (w + (1ull << (s - 1))) >> s;
 }
 // The short form where it holds; else `big` is set (x = -infinity, and whatever is below 2^-42, among them).
 __device__ __forceinline__ uint32_t short_exp(const Shared& sh, float x, const Scale& c, bool& big) {
     const float t = __fmaf_rn(x, c.hi, 12582912.0f);   // 1.5 * 2^23: the nearest integer in the low bits
     const int k = __float_as_int(t) - 0x4B400000 - c.top_i;
-    big = static_cast<uint32_t>(k + 42 * 1024) >= 32u * 1024;   // a t beyond its range gives a k beyond this one
+    big = static_cast<uint32_t>(k + 42 * 1024) >= 32u * 1024 || !c.brief;   // a t beyond its range gives a k beyond this one
     float r = __fmaf_rn(x, c.hi, -__fsub_rn(t, 12582912.0f));
     r = __fsub_rn(__fmaf_rn(x, c.lo, r), c.top_f);
     constexpr float kLn = 0.69314718055994530942f / 1024.0f;
     // (z + z^2 / 2) * 2^32 with z = r kLn, to the nearest integer (below 2^22 in magnitude)
     const float g = __fmaf_rn(r, 0.5f * kLn * kLn * 4294967296.0f, kLn * 4294967296.0f);
     const int p = __float_as_int(__fmaf_rn(r, g, 12582912.0f)) - 0x4B400000;
-    const int m = sh.power10[k & 1023];
+    const int m = sh.power30[k & 1023];
     const uint32_t w = static_cast<uint32_t>(m + __mulhi(m, p)) >> ((-11 - (k >> 10)) & 31);   // twice the weight
     return big ? 0u : (w + 1) >> 1;
 }
 __device__ __forceinline__ unsigned long long fixed_exp(const Shared& sh, float x, float top, const Scale& c) {
     bool big;
     const uint32_t w = short_exp(sh, x, c, big);
-    return big ? exact_exp(sh.power, static_cast<double>(x) - static_cast<double>(top), c.rate) : w;
+    return big ? exact_exp(sh, x, top, c.hi, c.lo, c.lo2) : w;
 }
-// Sums weights with the exact forms put off: they are few, and a warp that stops for each holds up the others.
-struct Summer {
-    unsigned long long sum = 0;
-    float put_off = -INFINITY;
-    __device__ __forceinline__ void add(const Shared& sh, float x, float top, const Scale& c) {
-        bool big;
-        sum += short_exp(sh, x, c, big);
-        if (big && x > -INFINITY) {
-            if (put_off > -INFINITY) sum += exact_exp(sh.power, static_cast<double>(put_off) - static_cast<double>(top), c.rate);
-            put_off = x;
-        }
+// The weights of four ids, those of `in`: short forms in one straight run (below 2^-10, so four fit 32 bits); the
+// exact ones, which are few, stay behind in `big`.
+__device__ __forceinline__ uint32_t short_four(const Shared& sh, const float (&x)[4], const bool (&in)[4], const Scale& c, uint32_t (&w)[4], uint32_t& big) {
+    uint32_t sum = 0;
+    big = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        bool b;
+        w[j] = short_exp(sh, x[j], c, b);
+        w[j] = in[j] ? w[j] : 0u;
+        big |= b && in[j] ? 1u << j : 0u;
+        sum += w[j];
     }
-    __device__ __forceinline__ unsigned long long total(const Shared& sh, float top, const Scale& c) {
-        if (put_off > -INFINITY) sum += exact_exp(sh.power, static_cast<double>(put_off) - static_cast<double>(top), c.rate);
-        put_off = -INFINITY;
-        return sum;
-    }
-};
+    return sum;
+}
+__device__ __forceinline__ float pick(const float (&x)[4], int j) { return j & 2 ? (j & 1 ? x[3] : x[2]) : (j & 1 ? x[1] : x[0]); }
 
+// ceil(p x) for 0 < p < 1, in integers.
+__device__ __forceinline__ unsigned long long product_up(float p, unsigned long long x) {
+    const uint32_t bits = __float_as_uint(p), e = bits >> 23;
+    const unsigned long long m = e ? (bits & 0x7FFFFFu) | 0x800000u : bits & 0x7FFFFFu;   // p = m 2^-q
+    const int q = 150 - static_cast<int>(e ? e : 1);                                       // 24 or more
+    unsigned long long lo = m * x, hi = __umul64hi(m, x);
+    if (q >= 88) return 1;
+    if (q >= 64) return (hi >> (q - 64)) + ((lo | (hi & ((1ull << (q - 64)) - 1))) ? 1 : 0);
+    return (hi << (64 - q)) + (lo >> q) + ((lo & ((1ull << q) - 1)) ? 1 : 0);
+}
+// floor(u x) for 0 <= u < 1, in integers (u to 64 bits).
+__device__ __forceinline__ unsigned long long product_down(double u, unsigned long long x) {
+    const unsigned long long bits = static_cast<unsigned long long>(__double_as_longlong(u));
+    const int e = static_cast<int>(bits >> 52);   // u = m 2^(e - 1075)
+    const int s = 1011 + 0 - e;                   // to units of 2^-64: m 2^(e - 1011)
+    if (e == 0 || s >= 53) return 0;
+    const unsigned long long m = (bits & ((1ull << 52) - 1)) | (1ull << 52);
+    return __umul64hi(s >= 0 ? m >> s : m << -s, x);
+}
 __device__ __forceinline__ unsigned long long warp_sum(unsigned long long x) {
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
@@ -174,8 +221,9 @@ __device__ __forceinline__ unsigned long long warp_sum(unsigned long long x) {
 
 template <int CL>
 __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ SampleArgs a, const __grid_constant__ Rows rows) {
-    extern __shared__ __align__(16) float slice_s[];
-    __shared__ Shared sh;
+    extern __shared__ __align__(16) unsigned char smem[];
+    Shared& sh = *reinterpret_cast<Shared*>(smem);
+    float* slice_s = reinterpret_cast<float*>(smem + sizeof(Shared));
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = cluster.block_rank(), row = blockIdx.x / CL;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -195,13 +243,22 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
     auto logit = [&](uint32_t i) { return a.resident ? slice_s[i] : as_logit(__ldg(src + base + i)); };
 
     // ---- 1: the largest logit and its lowest id
-    if (tid < 256) sh.power[tid] = exp2(tid * (1.0 / 256.0));
-    sh.power10[tid] = __double2int_rn(exp2(tid * (1.0 / 1024.0)) * 1073741824.0);
-    unsigned long long best = 0;
-    auto look = [&](uint32_t i, float x) {
+    sh.power62[tid] = kPowers.v[tid];
+    sh.power30[tid] = static_cast<int>((kPowers.v[tid] + (1ull << 31)) >> 32);
+    if (tid == kThreads - 1) {   // what takes double precision, on one thread beside the loads
+        const double c = 1477.3197218702985291 / static_cast<double>(rule.temperature);   // 1024 log2(e)
+        const float hi = static_cast<float>(c), lo = static_cast<float>(c - hi);
+        sh.scale[0] = hi;
+        sh.scale[1] = isinf(hi) ? 0.0f : lo;
+        sh.scale[2] = isinf(hi) ? 0.0f : static_cast<float>(c - hi - lo);
+    } else if (tid == kThreads - 33 && rule.min_p > 0.0f) {
+        sh.floor_d = log(static_cast<double>(rule.min_p));
+    }
+    float most = -INFINITY;
+    uint32_t most_id = base;
+    auto look = [&](uint32_t i, float x) {   // a thread's ids come in rising order
         x = i < n ? as_logit(x) : -INFINITY;
-        const unsigned long long key = i < n ? key_of(x, base + i) : 0;
-        best = key > best ? key : best;
+        if (x > most) most = x, most_id = base + i;
         return x;
     };
     if (a.resident && a.vec) {
@@ -234,6 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
     }
     for (int i = tid; i < kLevels; i += kThreads) sh.count[i] = 0;
     if (tid == 0) sh.first = kLevels, sh.last = kLevels, sh.by_count = kLevels, sh.gathered = 0, sh.pick = kLevels;
+    unsigned long long best = key_of(most, most_id);
     for (int o = 16; o > 0; o >>= 1) {
         const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
         best = other > best ? other : best;
@@ -266,22 +324,28 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
         cluster.sync();   // no CTA leaves while another may read its shared memory
         return;
     }
-    const Scale one = scale_of(1.0, top);
-    const double top_d = top;
+    // 1,024 log2(e) as a sum of three floats
+    constexpr double kC = 1477.3197218702985291;
+    constexpr float kHi = static_cast<float>(kC), kLo = static_cast<float>(kC - kHi), kLo2 = static_cast<float>(kC - kHi - kLo);
+    const Scale one = scale_of(kHi, kLo, kLo2, top);
     auto weight = [&](float x) { return fixed_exp(sh, x, top, one); };
-    // the nearest level, in the low bits of a float of 2^23 or more
-    auto level = [&](float x) { return __float_as_uint(fminf(fmaf(top - x, kPerNat, 8388608.0f), 8388607.0f + kLevels)) - 0x4B000000u; };
+    auto level = [&](float x) { return __float_as_uint(fminf(near_level(top - x), kOne - 1.0f + kLevels)) - 0x4B000000u; };
     const bool greedy = !(rule.temperature > 0.0f);
     const bool cut_p = !greedy && rule.top_p < 1.0f, cut_k = !greedy && rule.top_k > 0 && static_cast<uint32_t>(rule.top_k) < a.vocab;
     // ids with a key below `border` are out: at first those without a finite logit, and those with p below
     // min_p of the largest, by the least logit that is not
     unsigned long long border = static_cast<unsigned long long>(ordered(-3.402823466e38f)) << 32;
     if (!greedy && rule.min_p > 0.0f) {
-        const double floor_d = log(static_cast<double>(rule.min_p));
-        uint32_t o = ordered(static_cast<float>(top_d + floor_d));
-        while (o < ordered(top) && !(static_cast<double>(from_ordered(o)) - top_d >= floor_d)) ++o;
-        while (o > ordered(-3.402823466e38f) && static_cast<double>(from_ordered(o - 1)) - top_d >= floor_d) --o;
-        border = static_cast<unsigned long long>(o) << 32;
+        if (tid == 0) {
+            const double floor_d = sh.floor_d, top_d = top;
+            uint32_t o = ordered(static_cast<float>(top_d + floor_d));
+            while (o < ordered(top) && !(static_cast<double>(from_ordered(o)) - top_d >= floor_d)) ++o;
+            while (o > ordered(-3.402823466e38f) && static_cast<double>(from_ordered(o - 1)) - top_d >= floor_d) --o;
+            sh.border_key = static_cast<unsigned long long>(o) << 32;
+        }
+        __syncthreads();
+        border = sh.border_key;
+        __syncthreads();
     }
 
     // ---- 2a: counts per level, and the bracket
@@ -304,79 +368,98 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
         if (tid < kPart)
             for (int r = 0; r < CL; ++r) *cluster.map_shared_rank(&sh.count[mine], r) = c;
         cluster.sync();
-        // two levels per thread: counts and bounds of the mass down to and including each
+        // two levels per thread: counts, and the mass down to and including each, near enough
         static_assert(kLevels == 2 * kThreads, "");
         const uint32_t c0 = sh.count[2 * tid], c1 = sh.count[2 * tid + 1];
-        // a level's edges are off by the rounding of (max - l) * 128, its mass by fp32 sums and exponentials: 2^-12
-        // covers them all
-        constexpr float kMore = 1.0f + 0x1p-12f, kLess = 1.0f - 0x1p-12f;
-        const float q0 = expf((0.5f - 2.0f * tid) / kPerNat), q1 = expf((-0.5f - 2.0f * tid) / kPerNat), q2 = expf((-1.5f - 2.0f * tid) / kPerNat);
-        const float lo0 = c0 * q1 * kLess, hi0 = c0 * q0 * kMore, lo1 = tid == kThreads - 1 ? 0.0f : c1 * q2 * kLess, hi1 = c1 * q1 * kMore;
+        const float e0 = c0 * expf(-level_middle(2 * tid)), e1 = c1 * expf(-level_middle(2 * tid + 1));
         uint32_t pc = c0 + c1;
-        float pl = lo0 + lo1, ph = hi0 + hi1;
+        float pe = e0 + e1, var = (c0 && !(tid == 0 && c0 == 1) ? e0 * e0 / c0 : 0.0f) + (c1 ? e1 * e1 / c1 : 0.0f);   // a lone largest id weighs 1
+        if (tid >= kThreads / 2) var *= 9.0f;
+        for (int o = 16; o > 0; o >>= 1) var += __shfl_xor_sync(0xffffffffu, var, o);
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t uc = __shfl_up_sync(0xffffffffu, pc, o);
-            const float ul = __shfl_up_sync(0xffffffffu, pl, o), uh = __shfl_up_sync(0xffffffffu, ph, o);
-            if (lane >= o) pc += uc, pl += ul, ph += uh;
+            const float ue = __shfl_up_sync(0xffffffffu, pe, o);
+            if (lane >= o) pc += uc, pe += ue;
         }
-        if (lane == 31) sh.warp_count[warp] = pc, sh.warp_lo[warp] = pl, sh.warp_hi[warp] = ph;
+        if (lane == 31) sh.warp_count[warp] = pc, sh.warp_near[warp] = pe, sh.warp_var[warp] = var;
         __syncthreads();
         uint32_t bc = 0;
-        float bl = 0.0f, bh = 0.0f, all_lo = 0.0f, all_hi = 0.0f;
+        float be = 0.0f, all = 0.0f;
+        var = 0.0f;
         for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) bc += sh.warp_count[w], bl += sh.warp_lo[w], bh += sh.warp_hi[w];
-            all_lo += sh.warp_lo[w], all_hi += sh.warp_hi[w];
+            if (w < warp) bc += sh.warp_count[w], be += sh.warp_near[w];
+            all += sh.warp_near[w], var += sh.warp_var[w];
         }
         const uint32_t cum1 = bc + pc, cum0 = cum1 - c1;
-        const float l1 = bl + pl, l0 = bl + (pl - lo1), h1 = bh + ph, h0 = bh + (ph - hi1);
         if (cut_p) {
-            const float low = rule.top_p * all_lo * kLess, high = rule.top_p * all_hi * kMore;
-            if (c0 && h0 * kMore >= low) atomicMin(&sh.first, 2 * tid);
-            if (c1 && h1 * kMore >= low) atomicMin(&sh.first, 2 * tid + 1);
-            if (c0 && l0 * kLess >= high) atomicMin(&sh.last, 2 * tid);
-            if (c1 && l1 * kLess >= high) atomicMin(&sh.last, 2 * tid + 1);
+            // an id's weight is off by up to 1/256 of itself, evenly spread in a level: 3.5 standard deviations of the
+            // sum (and 2^-13 of it for the rest) to either side, mostly a level or two
+            const float slack = 3.5f * (1.0f / 256.0f) * 0.57735f * sqrtf(var) + all * 0x1p-13f;
+            const float m1 = be + pe, m0 = be + (pe - e1), low = rule.top_p * all - slack, high = rule.top_p * all + slack;
+            if (c0 && m0 >= low) atomicMin(&sh.first, 2 * tid);
+            if (c1 && m1 >= low) atomicMin(&sh.first, 2 * tid + 1);
+            if (c0 && m0 >= high) atomicMin(&sh.last, 2 * tid);
+            if (c1 && m1 >= high) atomicMin(&sh.last, 2 * tid + 1);
         }
         if (cut_k) {
             if (c0 && cum0 >= static_cast<uint32_t>(rule.top_k)) atomicMin(&sh.by_count, 2 * tid);
             if (c1 && cum1 >= static_cast<uint32_t>(rule.top_k)) atomicMin(&sh.by_count, 2 * tid + 1);
         }
         __syncthreads();
-        first = cut_p ? min(sh.first, sh.by_count) : sh.by_count;
+        first = cut_p ? min(min(sh.first, sh.by_count), kLevels - 1u) : sh.by_count;
         last = cut_p ? min(min(sh.last, sh.by_count), kLevels - 1u) : sh.by_count;
-        // counts of the levels above the bracket
+        // ids above the bracket, and ids in it
         if (2 * tid == first) sh.pick_count = cum0 - c0;
         if (2 * tid + 1 == first) sh.pick_count = cum1 - c1;
-        for (int i = tid; i < kLevels; i += kThreads) sh.mass[i] = 0;
+        if (2 * tid == last) sh.members = cum0;
+        if (2 * tid + 1 == last) sh.members = cum1;
         __syncthreads();
     }
     const bool bracket = first < kLevels;   // else every id is kept
+    uint32_t above = bracket ? sh.pick_count : 0;
+    const uint32_t members = bracket ? sh.members - above : 0;
+    const bool gather = members <= kGather;
 
     // ---- 2b: exact sums: the whole distribution, the levels above the bracket, each level in it
     unsigned long long whole = 0, above_mass = 0;
     {
-        Summer every, over;
-        // below every id of the bracket
-        const float low = !(bracket && cut_p) ? INFINITY : last == kLevels - 1u ? -3.402823466e38f : top - (static_cast<float>(last) + 1.0f) / kPerNat;
+        unsigned long long sum = 0, up = 0;
+        float put_off = -INFINITY;   // an id whose exact form waits, so that no warp stops for each
+        auto exact = [&](float x) {
+            const unsigned long long w = exact_exp(sh, x, top, one.hi, one.lo, one.lo2);
+            sum += w;
+            if (level(x) < first) up += w;
+        };
+        // level(x) < first is near < before_first, level(x) <= last near <= to_last
+        const bool collect = bracket && gather;
+        const float before_first = kOne + (bracket ? first : 0);
+        const float to_last = collect ? (last == kLevels - 1u ? INFINITY : kOne + last) : -1.0f;
         for (uint32_t i = tid * 4; i < n; i += kThreads * 4) {
             const float4 x4 = four(i);
             const float x[4] = {x4.x, x4.y, x4.z, x4.w};
+            constexpr bool kAll[4] = {true, true, true, true};
+            uint32_t w[4], big;
+            sum += short_four(sh, x, kAll, one, w, big);
+            uint32_t above4 = 0, inside = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) every.add(sh, x[j], top, one);
-            const float most = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-            if (most >= low) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t lev = level(x[j]);
-                    if (x[j] >= low && lev <= last) {
-                        if (lev < first)
-                            over.add(sh, x[j], top, one);
-                        else
-                            atomicAdd(&sh.mass[lev - first], weight(x[j]));
-                    }
+            for (int j = 0; j < 4; ++j) {
+                const float near = near_level(top - x[j]);
+                above4 += near < before_first ? w[j] : 0u;
+                inside |= near >= before_first && near <= to_last ? 1u << j : 0u;
+            }
+            up += above4;
+            for (uint32_t left = inside | big; left; left &= left - 1) {
+                const int j = __ffs(left) - 1;
+                const float y = pick(x, j);
+                if (!(y > -INFINITY)) continue;
+                if (inside >> j & 1) sh.mass[atomicAdd(&sh.gathered, 1u)] = key_of(y, base + i + j);
+                if (big >> j & 1) {
+                    if (put_off > -INFINITY) exact(put_off);
+                    put_off = y;
                 }
             }
         }
-        unsigned long long sum = every.total(sh, top, one), up = over.total(sh, top, one);
+        if (put_off > -INFINITY) exact(put_off);
         sum = warp_sum(sum), up = warp_sum(up);
         if (lane == 0) sh.warp_mass[warp] = sum, sh.warp_mass2[warp] = up;
         __syncthreads();
@@ -390,13 +473,90 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
             above_mass += *cluster.map_shared_rank(&sh.cta_mass2, r);
         }
     }
-    uint32_t above = 0, border_level = kLevels, ties = 0xFFFFFFFFu;
+    uint32_t border_level = kLevels, ties = 0xFFFFFFFFu;
     unsigned long long need = 0;
     bool tied = false;   // of the ids with the border's logit only the first `ties` stay
-    if (bracket) {
-        need = cut_p ? static_cast<unsigned long long>(ceil(static_cast<double>(rule.top_p) * static_cast<double>(whole))) : ~0ull;
-        above = sh.pick_count;
-        if (warp == 0) {   // walk the bracket's levels, 32 at a time; masses of the whole cluster
+    if (bracket) need = cut_p ? product_up(rule.top_p, whole) : ~0ull;
+    bool sought = bracket;
+    if (bracket && gather && above_mass < need) {   // else the bracket begins too low
+        // ---- 2c: the bracket's ids, to the cluster's first CTA, sorted; the border is the first that reaches a cut
+        if (rank != 0) {
+            if (tid == 0) sh.border_at = atomicAdd(cluster.map_shared_rank(&sh.gathered, 0), sh.gathered);
+            __syncthreads();
+            unsigned long long* list = cluster.map_shared_rank(sh.mass, 0) + sh.border_at;
+            for (uint32_t i = tid; i < sh.gathered; i += kThreads) list[i] = sh.mass[i];
+        }
+        cluster.sync();
+        if (rank == 0) {
+            // four ids per thread; the border is the largest key with which those from it on reach a cut: halves of
+            // the range [lo, hi) that holds it, until one id is left
+            if (tid == 0) sh.border_key = 0, sh.key_lo = ~0ull, sh.key_hi = 0;
+            __syncthreads();
+            constexpr int kMine = kGather / kThreads;
+            unsigned long long key[kMine], w[kMine];
+#pragma unroll
+            for (int j = 0; j < kMine; ++j) {
+                const uint32_t i = tid + j * kThreads;
+                key[j] = i < members ? sh.mass[i] : 0;
+                w[j] = key[j] ? weight(from_ordered(static_cast<uint32_t>(key[j] >> 32))) : 0;
+                if (key[j]) {
+                    atomicMin(&sh.key_lo, key[j]);
+                    atomicMax(&sh.key_hi, key[j]);
+                }
+            }
+            __syncthreads();
+            unsigned long long lo = sh.key_lo, hi = sh.key_hi + 1;
+            // ids from `from` on, and their mass (24 and 17 bits apart: 4,096 weights of 2^40 at most)
+            int turn = 0;
+            auto down_to = [&](unsigned long long from, uint32_t& count) {
+                uint32_t c = 0, wl = 0, wh = 0;
+#pragma unroll
+                for (int j = 0; j < kMine; ++j)
+                    if (key[j] >= from) ++c, wl += static_cast<uint32_t>(w[j]) & 0xFFFFFFu, wh += static_cast<uint32_t>(w[j] >> 24);
+                c = __reduce_add_sync(0xffffffffu, c), wl = __reduce_add_sync(0xffffffffu, wl), wh = __reduce_add_sync(0xffffffffu, wh);
+                if (lane == 0) sh.half[turn][warp] = make_uint3(c, wl, wh);
+                __syncthreads();
+                const uint3 v = sh.half[turn][lane];
+                turn ^= 1;
+                count = __reduce_add_sync(0xffffffffu, v.x);
+                const unsigned long long l = __reduce_add_sync(0xffffffffu, v.y & 0xFFFFu), h = __reduce_add_sync(0xffffffffu, v.y >> 16);
+                return l + (h << 16) + (static_cast<unsigned long long>(__reduce_add_sync(0xffffffffu, v.z)) << 24);
+            };
+            const auto reached = [&](unsigned long long mass, uint32_t count) {
+                return (cut_p && above_mass + mass >= need) || (cut_k && above + count >= static_cast<uint32_t>(rule.top_k));
+            };
+            uint32_t at_lo, at_hi = 0, c;
+            const bool any = reached(down_to(lo, at_lo), at_lo);
+            while (any && at_lo - at_hi > 1) {
+                const unsigned long long mid = lo + (hi - lo) / 2;
+                if (reached(down_to(mid, c), c))
+                    lo = mid, at_lo = c;
+                else
+                    hi = mid, at_hi = c;
+            }
+#pragma unroll
+            for (int j = 0; j < kMine; ++j)
+                if (any && key[j] >= lo && key[j] < hi) sh.border_key = key[j];
+            __syncthreads();
+        }
+        cluster.sync();
+        const unsigned long long key = *cluster.map_shared_rank(&sh.border_key, 0);
+        sought = key == 0;   // the bracket ends too high
+        border = max(border, key);
+        cluster.sync();      // the peers have read the key
+    }
+    if (sought) {
+        // ---- 2c otherwise (many nearly equal logits, or a border that the counts misjudged): the exact masses of all
+        // levels, and then of the parts of the border's by the bits of the logit
+        first = 0, last = kLevels - 1, above = 0, above_mass = 0;
+        for (int i = tid; i < kLevels; i += kThreads) sh.mass[i] = 0;
+        __syncthreads();
+        for (uint32_t i = tid; i < n && cut_p; i += kThreads) {
+            const float x = logit(i);
+            if (x > -INFINITY) atomicAdd(&sh.mass[level(x)], weight(x));
+        }
+        cluster.sync();
+        if (warp == 0) {   // walk the levels, 32 at a time; masses of the whole cluster
             unsigned long long run = above_mass;
             uint32_t run_c = above;
             for (uint32_t i = first; i <= last; i += 32) {
@@ -426,37 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
         above = sh.pick_count, above_mass = sh.pick_mass;
     }
     if (border_level < kLevels) {
-        // ---- 2c: the border within its level
-        const uint32_t members = sh.count[border_level];
-        if (members <= kGather) {
-            unsigned long long* list = cluster.map_shared_rank(sh.mass, 0);
-            uint32_t* next = cluster.map_shared_rank(&sh.gathered, 0);
-            for (uint32_t i = tid * 4; i < n; i += kThreads * 4) {
-                const float4 x4 = four(i);
-                const float x[4] = {x4.x, x4.y, x4.z, x4.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (x[j] > -INFINITY && level(x[j]) == border_level) list[atomicAdd(next, 1u)] = key_of(x[j], base + i + j);
-            }
-            cluster.sync();
-            if (rank == 0) {   // each member's rank and the mass above it; the border is the first that reaches a cut
-                if (tid == 0) sh.border_key = 0;
-                unsigned long long* weights = sh.mass + kGather;
-                const unsigned long long key = tid < members ? sh.mass[tid] : 0;
-                if (tid < members) weights[tid] = weight(from_ordered(static_cast<uint32_t>(key >> 32)));
-                __syncthreads();
-                if (tid < members) {
-                    unsigned long long m = above_mass + weights[tid];
-                    uint32_t c = above + 1;
-                    for (uint32_t j = 0; j < members; ++j)
-                        if (sh.mass[j] > key) m += weights[j], ++c;
-                    if ((cut_p && m >= need) || (cut_k && c >= static_cast<uint32_t>(rule.top_k))) atomicMax(&sh.border_key, key);
-                }
-                __syncthreads();
-            }
-            cluster.sync();
-            border = max(border, *cluster.map_shared_rank(&sh.border_key, 0));
-        } else {
+        {
             uint32_t lo = 0, bits = 32;   // the border's logit has these high bits
             for (int pass = 0; pass < 3; ++pass) {
                 for (int i = tid; i < kLevels; i += kThreads) sh.mass[i] = 0, sh.count[i] = 0;
@@ -533,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
 
     // ---- 3: the draw
     if (!greedy) {
-        const Scale heat = scale_of(rule.temperature, top);
+        const Scale heat = scale_of(sh.scale[0], sh.scale[1], sh.scale[2], top);
         const uint32_t edge = static_cast<uint32_t>(border >> 32);
         const uint32_t run = a.slice / kWarps;   // a warp's run of ids, a multiple of 32
         const uint32_t r0 = min(n, warp * run), r1 = min(n, r0 + run);
@@ -570,26 +700,61 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
             seen += __popc(vote);
             return keep;
         };
-        Summer draw;
+        unsigned long long sum = 0;
         uint32_t count = 0, seen = ties_before;
+        // ids of a group: 128 at a time
+        const uint32_t per_group = (run + kGroups * 128 - 1) / (kGroups * 128) * 128;
+        // this lane's share of the 128 ids from i0 on (its four, in id order)
+        auto of_four = [&](uint32_t i0, float (&x)[4], bool (&in)[4]) {
+            const uint32_t i = i0 + 4 * lane;
+            const float4 x4 = i < r1 ? four(i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            x[0] = x4.x, x[1] = x4.y, x[2] = x4.z, x[3] = x4.w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) in[j] = in_cuts(x[j], i + j);
+        };
+        auto exact_mass = [&](float x) { return exact_exp(sh, x, top, heat.hi, heat.lo, heat.lo2); };
+        auto mass_of_four = [&](const float (&x)[4], const bool (&in)[4]) {
+            uint32_t w[4], big;
+            unsigned long long m = short_four(sh, x, in, heat, w, big);
+            for (; big; big &= big - 1) m += exact_mass(pick(x, __ffs(big) - 1));
+            return m;
+        };
         if (tied) {
             for (uint32_t i0 = r0; i0 < r1; i0 += 32) {
                 const uint32_t i = i0 + lane;
-                if (keep_tied(i0, seen)) draw.add(sh, logit(i), top, heat), ++count;
+                if (keep_tied(i0, seen)) sum += mass(logit(i)), ++count;
             }
         } else {
-            for (uint32_t i0 = r0; i0 < r1; i0 += 128) {
-                const uint32_t i = i0 + 4 * lane;
-                const float4 x4 = i < r1 ? four(i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                const float x[4] = {x4.x, x4.y, x4.z, x4.w};
-                const float most = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                if (!__any_sync(0xffffffffu, most >= edge_x)) continue;
+            float put_off = -INFINITY;   // as above
+            int put_off_group = 0;
+            for (int g = 0; g < kGroups; ++g) {
+                unsigned long long m = 0;
+                for (uint32_t i0 = r0 + g * per_group; i0 < min(r1, r0 + (g + 1) * per_group); i0 += 128) {
+                    float x[4];
+                    bool in[4];
+                    of_four(i0, x, in);
+                    if (!__any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3])) continue;
+                    uint32_t w[4], big;
+                    m += short_four(sh, x, in, heat, w, big);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (in_cuts(x[j], i + j)) draw.add(sh, x[j], top, heat), ++count;
+                    for (int j = 0; j < 4; ++j) count += in[j];
+                    for (; big; big &= big - 1) {
+                        if (put_off > -INFINITY) m += exact_mass(pick(x, __ffs(big) - 1));
+                        else put_off = pick(x, __ffs(big) - 1), put_off_group = g;
+                    }
+                }
+                m = warp_sum(m);
+                if (lane == 0) sh.group_mass[warp][g] = m;
+                sum += lane == 0 ? m : 0ull;
+            }
+            __syncwarp();
+            if (put_off > -INFINITY) {
+                const unsigned long long m = exact_mass(put_off);
+                sum += m;
+                atomicAdd(&sh.group_mass[warp][put_off_group], m);
             }
         }
-        const unsigned long long sum = warp_sum(draw.total(sh, top, heat));
+        sum = warp_sum(sum);
         for (int o = 16; o > 0; o >>= 1) count += __shfl_xor_sync(0xffffffffu, count, o);
         if (lane == 0) sh.warp_mass[warp] = sum, sh.warp_count[warp] = count;
         __syncthreads();
@@ -608,16 +773,16 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
             all += s;
             kept += *cluster.map_shared_rank(&sh.draw_count, r);
         }
-        double u = a.uniform[row];
-        u = u >= 0.0 ? fmin(u, 1.0) : 0.0;   // NaN and negative values to 0
-        unsigned long long target = static_cast<unsigned long long>(u * static_cast<double>(all));
-        if (target >= all) target = all - 1;
+        const double u = a.uniform[row];   // NaN and negative values stand for 0
+        const unsigned long long target = !(u > 0.0) ? 0 : u < 1.0 ? min(product_down(u, all), all - 1) : all - 1;
         for (int w = 0; w < warp; ++w) before += sh.warp_mass[w];
         if (target >= before && target < before + sum) {   // this warp's run holds the token
-            // the 32 ids that hold it: sums of 32 groups at a time, a group per lane (its ids taken in turn from
-            // a place of its own: 32 different banks), or group after group where ties need their order
+            // the group that holds it, the 128 ids in that, and the id; where ties need their order, 32 ids at a time
             unsigned long long at = before;
             uint32_t group = r0, seen_at = ties_before;
+            uint32_t id = 0;
+            float x = -INFINITY;
+            bool mine = false;
             if (tied) {
                 for (uint32_t i0 = r0; i0 < r1; i0 += 32) {
                     uint32_t seen_now = seen_at;
@@ -628,44 +793,58 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
                     at += s;
                     seen_at = seen_now;
                 }
+                const uint32_t i = group + lane;
+                x = i < r1 ? logit(i) : -INFINITY;
+                const bool keep = keep_tied(group, seen_at);
+                unsigned long long p = keep ? mass(x) : 0ull;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned long long up = __shfl_up_sync(0xffffffffu, p, o);
+                    if (lane >= o) p += up;
+                }
+                const uint32_t vote = __ballot_sync(0xffffffffu, at + p > target);
+                mine = vote && lane == __ffs(vote) - 1;
+                id = base + i;
             } else {
-                for (uint32_t g0 = r0; g0 < r1; g0 += 1024) {
-                    Summer part;
-                    for (int j = 0; j < 32; ++j) {
-                        const uint32_t i = g0 + lane * 32 + ((j + lane) & 31);
-                        const float x = i < r1 ? logit(i) : -INFINITY;
-                        if (in_cuts(x, i)) part.add(sh, x, top, heat);
-                    }
-                    const unsigned long long s = part.total(sh, top, heat);
-                    unsigned long long p = s;
+                __syncwarp();   // lane 0's group sums
+                int g = 0;
+                for (; g < kGroups - 1 && at + sh.group_mass[warp][g] <= target; ++g) at += sh.group_mass[warp][g];
+                for (uint32_t i0 = r0 + g * per_group; i0 < r1; i0 += 128) {
+                    float y[4];
+                    bool in[4];
+                    of_four(i0, y, in);
+                    const unsigned long long m = mass_of_four(y, in);
+                    unsigned long long p = m;
                     for (int o = 1; o < 32; o <<= 1) {
                         const unsigned long long up = __shfl_up_sync(0xffffffffu, p, o);
                         if (lane >= o) p += up;
                     }
                     const uint32_t vote = __ballot_sync(0xffffffffu, at + p > target);
                     if (vote) {
-                        const int f = __ffs(vote) - 1;
-                        group = g0 + f * 32;
-                        at += __shfl_sync(0xffffffffu, p - s, f);
+                        mine = lane == __ffs(vote) - 1;
+                        if (mine) {
+                            unsigned long long run_m = at + p - m;
+                            for (int j = 0; j < 4; ++j) {
+                                const float z = pick(y, j);
+                                const bool keep = j & 2 ? (j & 1 ? in[3] : in[2]) : (j & 1 ? in[1] : in[0]);
+                                if (!keep) continue;
+                                run_m += mass(z);
+                                if (run_m > target) {
+                                    x = z;
+                                    id = base + i0 + 4 * lane + j;
+                                    break;
+                                }
+                            }
+                        }
                         break;
                     }
                     at += __shfl_sync(0xffffffffu, p, 31);
                 }
             }
-            const uint32_t i = group + lane;
-            const float x = i < r1 ? logit(i) : -INFINITY;
-            const bool keep = tied ? keep_tied(group, seen_at) : in_cuts(x, i);
-            unsigned long long p = keep ? mass(x) : 0ull;
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned long long up = __shfl_up_sync(0xffffffffu, p, o);
-                if (lane >= o) p += up;
-            }
-            const uint32_t vote = __ballot_sync(0xffffffffu, at + p > target);
-            if (vote && lane == __ffs(vote) - 1) {
-                a.token[row] = base + i;
+            if (mine) {
+                a.token[row] = id;
                 if (a.kept) a.kept[row] = kept;
                 if (a.logprob) {
-                    a.logprob[row] = static_cast<float>(static_cast<double>(x) - top_d - log(static_cast<double>(whole) * 0x1p-40));
+                    a.logprob[row] = static_cast<float>(static_cast<double>(x) - static_cast<double>(top) - log(static_cast<double>(whole) * 0x1p-40));
                 }
             }
         }
@@ -684,13 +863,13 @@ cudaError_t launch(SampleArgs& a, const Rows& r, uint32_t n, cudaStream_t st) {
     const uint32_t per = (a.vocab + CL - 1) / CL;
     a.slice = (per + 1023) / 1024 * 1024;
     a.resident = a.slice <= kSmemIds;
-    cudaError_t e = cudaFuncSetAttribute(smp_rows<CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemIds * sizeof(float));
+    cudaError_t e = cudaFuncSetAttribute(smp_rows<CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared) + kSmemIds * sizeof(float));
     if (e == cudaSuccess && CL > 8) e = cudaFuncSetAttribute(smp_rows<CL>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(n * CL);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = a.resident ? a.slice * sizeof(float) : 0;
+    cfg.dynamicSmemBytes = sizeof(Shared) + (a.resident ? a.slice * sizeof(float) : 0);
     cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -737,7 +916,10 @@ extern "C" GTM_API int gtm_sample_rows(const float* logits, uint32_t n, uint32_t
     a.token = token, a.kept = kept, a.logprob = logprob;
     a.vocab = vocab;
     a.vec = aligned(logits, 16) && (n == 1 || row_stride % 4 == 0);
-    const cudaError_t e = getenv("CL16") ? launch<16>(a, r, n, static_cast<cudaStream_t>(stream)) : launch<8>(a, r, n, static_cast<cudaStream_t>(stream));
+    // Sixteen CTAs a row while they all fit the SMs at once (one row of 262,144 ids: 45 us against 54 with
+    // eight); beyond that eight, whose rows finish in fewer rounds (64 rows: 240 us against 340).
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const cudaError_t e = n <= 8 ? launch<16>(a, r, n, st) : launch<8>(a, r, n, st);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return set_cuda_error(fn, e);

@@ -7,44 +7,63 @@ from __future__ import annotations
 
 import ctypes as C
 
-from . import ERR_INVALID, ERR_UNSUPPORTED, GtmError, KvCacheDesc, _stream, check, lib, ptr
+from . import ERR_INVALID, ERR_UNSUPPORTED, GtmError, KvCacheDesc, check, lib
 
 INT8, E4M3 = 0, 1
 FORMATS = {"int8": INT8, "e4m3": E4M3}
 
 
 def _u32(vals, n: int | None = None):
-    """(pointer, owner) of a host array of uint32; n: the length it must have."""
+    """(address, owner) of a host array of uint32; n: the length it must have."""
     import numpy as np
-    if not (isinstance(vals, np.ndarray) and vals.dtype == np.uint32 and vals.flags.c_contiguous):
+    if not (type(vals) is np.ndarray and vals.dtype == np.uint32 and vals.flags.c_contiguous):
         vals = np.asarray(vals)
         if vals.size and (vals.dtype.kind not in "iu" or vals.min() < 0 or vals.max() > 0xFFFFFFFF):
             raise GtmError(ERR_INVALID, "positions and sequence indices are integers in [0, 2^32)")
         vals = np.ascontiguousarray(vals, dtype=np.uint32)
     if n is not None and vals.size != n:
         raise GtmError(ERR_INVALID, f"{vals.size} positions or sequence indices for {n} rows")
-    return C.c_void_p(vals.ctypes.data), vals
+    return vals.ctypes.data, vals
 
 
-def _f32(t, name: str, device, shape=None) -> None:
-    """The checks a raw pointer cannot make."""
+def _raw_stream(stream, device):
+    """The stream to launch on, as an integer: the caller's, or torch's current one on the tensors' device,
+    which has to be the current device."""
     import torch
-    if t.dtype != torch.float32 or t.device != device:
+    if device.type == "cuda" and torch.cuda.current_device() != device.index:
+        raise GtmError(ERR_INVALID, f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    if stream is not None:
+        return stream.cuda_stream
+    return torch.cuda.current_stream().cuda_stream if device.type == "cuda" else None
+
+
+def _f32(t, name: str, device, shape=None) -> int:
+    """The checks a raw pointer cannot make, and the pointer."""
+    import torch
+    if t.dtype is not torch.float32 or t.device != device:
         raise GtmError(ERR_INVALID, f"{name} must be float32 on {device}, not {t.dtype} on {t.device}")
-    if shape is not None and (tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
+    if shape is not None and (t.shape != shape or not t.is_contiguous()):
         raise GtmError(ERR_INVALID, f"{name} must be contiguous {tuple(shape)}, not {tuple(t.shape)}")
+    return t.data_ptr()
 
 
-def _row_stride(t, name: str, device, n: int, width: int) -> int:
-    _f32(t, name, device)
-    if t.dim() != 2 or t.shape[0] != n or t.shape[1] != width or t.stride(1) != 1:
-        raise GtmError(ERR_INVALID, f"{name} must be [{n}, {width}] with contiguous rows, not {tuple(t.shape)}")
-    return width if n <= 1 else t.stride(0)
+def _rows(t, name: str, device, n: int, width: int):
+    """(pointer, row stride) of n rows of `width` floats."""
+    p = _f32(t, name, device)
+    if t.shape != (n, width):
+        raise GtmError(ERR_INVALID, f"{name} must be [{n}, {width}], not {tuple(t.shape)}")
+    stride = t.stride()
+    if stride[1] != 1:
+        raise GtmError(ERR_INVALID, f"{name} must have contiguous rows")
+    return p, width if n <= 1 else stride[0]
 
 
-def _bf16(t, name: str, device, n: int) -> None:
-    if t is not None and (t.element_size() != 2 or t.numel() != n or not t.is_contiguous() or t.device != device):
+def _bf16(t, name: str, device, n: int):
+    if t is None:
+        return None
+    if t.element_size() != 2 or t.numel() != n or not t.is_contiguous() or t.device != device:
         raise GtmError(ERR_INVALID, f"{name} must be {n} contiguous bf16 values on {device}")
+    return t.data_ptr()
 
 
 class KvCache:
@@ -83,35 +102,36 @@ class KvCache:
         self.fmt = "int8" if k.dtype == torch.int8 else "e4m3"
         self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), FORMATS[self.fmt], num_seqs,
                                 capacity, kv_heads, head_dim, 0)
+        self._ref = C.byref(self.desc)
 
     def write(self, q, k, v, q_out, positions, seqs, *, q_w=None, k_w=None, eps: float = 1e-6, rotated_pairs: int = 0,
               theta: float = 10000.0, stream=None) -> None:
         """gtm_qkv_cache_rows: q [n, q_heads * head_dim], k and v [n, kv_heads * head_dim] (rows may be
         strided, v may be k); q_out contiguous like q, or q itself; q_w, k_w bf16 [head_dim] or None."""
-        n, width = q.shape[0], self.kv_heads * self.head_dim
         if q.dim() != 2 or q.shape[1] % self.head_dim:
             raise GtmError(ERR_INVALID, f"q must be [n, q_heads * {self.head_dim}], not {tuple(q.shape)}")
-        qs = _row_stride(q, "q", self.device, n, q.shape[1])
-        ks, vs = (_row_stride(t, name, self.device, n, width) for name, t in (("k", k), ("v", v)))
-        _f32(q_out, "q_out", self.device, (n, q.shape[1]))
-        _bf16(q_w, "q_w", self.device, self.head_dim)
-        _bf16(k_w, "k_w", self.device, self.head_dim)
+        shape, dev, width = q.shape, self.device, self.kv_heads * self.head_dim
+        n = shape[0]
+        qp, qs = _rows(q, "q", dev, n, shape[1])
+        kp, ks = _rows(k, "k", dev, n, width)
+        vp, vs = _rows(v, "v", dev, n, width)
+        out = _f32(q_out, "q_out", dev, shape)
+        qw, kw = _bf16(q_w, "q_w", dev, self.head_dim), _bf16(k_w, "k_w", dev, self.head_dim)
         pos, _p = _u32(positions, n)
         sq, _s = _u32(seqs, n)
-        check(lib().gtm_qkv_cache_rows(C.byref(self.desc), q.shape[1] // self.head_dim, n, ptr(q), ptr(k), ptr(v), qs, ks, vs,
-                                       ptr(q_w), ptr(k_w), eps, rotated_pairs, theta, pos, sq, ptr(q_out), _stream(stream)))
+        check(lib().gtm_qkv_cache_rows(self._ref, shape[1] // self.head_dim, n, qp, kp, vp, qs, ks, vs, qw, kw, eps,
+                                       rotated_pairs, theta, pos, sq, out, _raw_stream(stream, dev)))
 
     def read(self, seq: int, first: int, count: int, k_out=None, v_out=None, stream=None):
         """gtm_kv_read: positions [first, first + count) of `seq` as fp32 [count, kv_heads * head_dim];
         (k_out, v_out), allocated where both are None."""
-        import torch
         shape = (count, self.kv_heads * self.head_dim)
         if k_out is None and v_out is None:
+            import torch
             k_out, v_out = (torch.empty(shape, dtype=torch.float32, device=self.device) for _ in range(2))
-        for name, t in (("k_out", k_out), ("v_out", v_out)):
-            if t is not None:
-                _f32(t, name, self.device, shape)
-        check(lib().gtm_kv_read(C.byref(self.desc), seq, first, count, ptr(k_out), ptr(v_out), _stream(stream)))
+        kp = None if k_out is None else _f32(k_out, "k_out", self.device, shape)
+        vp = None if v_out is None else _f32(v_out, "v_out", self.device, shape)
+        check(lib().gtm_kv_read(self._ref, seq, first, count, kp, vp, _raw_stream(stream, self.device)))
         return k_out, v_out
 
 
@@ -126,19 +146,18 @@ class KvAttention:
         if n == 0:
             raise GtmError(ERR_UNSUPPORTED, f"attention of {q_heads} / {kv_heads} heads of {head_dim}, {max_rows} rows")
         self.workspace = torch.empty(n, dtype=torch.uint8, device=device)
-        self.ws_ptr, self.ws_bytes = C.c_void_p(self.workspace.data_ptr()), n
+        self.ws_ptr, self.ws_bytes, self.device = self.workspace.data_ptr(), n, self.workspace.device
 
     def __call__(self, q, cache: KvCache, seqs, positions, ctx, *, window: int = 0, prefix: KvCache | None = None,
                  prefix_seq: int = 0, prefix_len: int = 0, stream=None) -> None:
-        n, width = q.shape[0], self.q_heads * self.head_dim
-        _f32(q, "q", cache.device, (n, width))
-        _f32(ctx, "ctx", cache.device, (n, width))
-        if (cache.kv_heads, cache.head_dim) != (self.kv_heads, self.head_dim) or self.workspace.device != cache.device:
+        dev, shape = cache.device, (q.shape[0], self.q_heads * self.head_dim)
+        n = shape[0]
+        qp, out = _f32(q, "q", dev, shape), _f32(ctx, "ctx", dev, shape)
+        if cache.kv_heads != self.kv_heads or cache.head_dim != self.head_dim or self.device != dev:
             raise GtmError(ERR_INVALID, "the cache's heads or device are not the attention's")
-        if prefix is not None and prefix.device != cache.device:
+        if prefix is not None and prefix.device != dev:
             raise GtmError(ERR_INVALID, "cache and prefix must be on one device")
         pos, _p = _u32(positions, n)
         sq, _s = _u32(seqs, n)
-        check(lib().gtm_attention_kv_rows(C.byref(cache.desc), C.byref(prefix.desc) if prefix is not None else None, prefix_seq,
-                                          prefix_len, self.q_heads, n, window, ptr(q), sq, pos, ptr(ctx), self.ws_ptr,
-                                          self.ws_bytes, _stream(stream)))
+        check(lib().gtm_attention_kv_rows(cache._ref, None if prefix is None else prefix._ref, prefix_seq, prefix_len, self.q_heads, n,
+                                          window, qp, sq, pos, out, self.ws_ptr, self.ws_bytes, _raw_stream(stream, dev)))

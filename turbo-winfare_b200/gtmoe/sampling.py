@@ -115,27 +115,30 @@ class RowSampler:
         self.vocab, self.max_rows = vocab, max_rows
         self.tokens, self.kept = (torch.zeros(max_rows, dtype=torch.int32, device=device) for _ in range(2))
         self.logprobs = torch.zeros(max_rows, dtype=torch.float32, device=device)
+        self._out = tuple(t.data_ptr() for t in (self.tokens, self.kept, self.logprobs))
 
     def __call__(self, logits, rows, uniforms=None, stream=None) -> RowTokens:
         """logits: fp32 [n, vocab], rows contiguous but possibly strided; rows: sampling_rows(...) or a
         list of RowParams, n of them; uniforms: float64 [n] on the device, None where every row is greedy."""
         import torch
-        n = logits.shape[0]
-        if logits.dim() != 2 or logits.shape[1] != self.vocab or logits.dtype != torch.float32 or logits.stride(1) != 1 or \
-                logits.device != self.tokens.device:
-            raise GtmError(ERR_INVALID, f"logits must be float32 [n, {self.vocab}] on {self.tokens.device} with contiguous rows")
+        from .kvcache import _raw_stream
+        dev, shape, stride = self.tokens.device, logits.shape, logits.stride()
+        if len(shape) != 2 or shape[1] != self.vocab or logits.dtype is not torch.float32 or stride[1] != 1 or logits.device != dev:
+            raise GtmError(ERR_INVALID, f"logits must be float32 [n, {self.vocab}] on {dev} with contiguous rows")
+        n = shape[0]
         if n > self.max_rows:
             raise GtmError(ERR_INVALID, f"{n} rows for a sampler of {self.max_rows}")
-        if uniforms is not None and (uniforms.dtype != torch.float64 or uniforms.numel() != n or not uniforms.is_contiguous() or
-                                     uniforms.device != logits.device):
-            raise GtmError(ERR_INVALID, f"uniforms must be {n} contiguous float64 values on {logits.device}")
+        u = None
+        if uniforms is not None:
+            if uniforms.dtype is not torch.float64 or uniforms.numel() != n or not uniforms.is_contiguous() or uniforms.device != dev:
+                raise GtmError(ERR_INVALID, f"uniforms must be {n} contiguous float64 values on {dev}")
+            u = uniforms.data_ptr()
         if isinstance(rows, (list, tuple)):
             if len(rows) != n:
                 raise GtmError(ERR_INVALID, f"{len(rows)} settings for {n} rows")
             rows = sampling_rows(rows)
         elif len(rows) < n:
             raise GtmError(ERR_INVALID, f"{len(rows)} settings for {n} rows")
-        stride = self.vocab if n <= 1 else logits.stride(0)
-        check(lib().gtm_sample_rows(ptr(logits), n, self.vocab, stride, rows, ptr(uniforms), ptr(self.tokens), ptr(self.kept),
-                                    ptr(self.logprobs), _stream(stream)))
+        check(lib().gtm_sample_rows(logits.data_ptr(), n, self.vocab, self.vocab if n <= 1 else stride[0], rows, u, *self._out,
+                                    _raw_stream(stream, dev)))
         return RowTokens(self.tokens[:n], self.kept[:n], self.logprobs[:n])
