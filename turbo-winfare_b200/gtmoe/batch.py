@@ -16,8 +16,14 @@ row i being one sequence's token,
               one GPU, or expert parallel over NVLink peer memory (gtmoe.ep.ep_layer_peer) with the
               sequences split over the ranks;
 
-then the greedy LM head (gtm_lm_head_greedy) for every sequence past its prompt. Only the step's
-token ids come back to the host. Under expert parallelism every rank takes part in every layer's
+then the greedy LM head (gtm_lm_head_greedy) for every sequence past its prompt, or, sampled, the
+softcapped logits of those rows and gtm_sample_rows. Only the step's token ids come back to the
+host.
+
+With `kv_format` ("int8" or "e4m3") the caches are one-byte rings (gtmoe.kvcache): one launch norms,
+rotates and stores a step's queries, keys and values, and gtm_attention_kv_rows attends. A prompt
+that all sequences begin with can then be run and held once (`set_prefix`): its tokens go through
+the layers max_seqs at a time, and every later step reads its keys and values once for all rows. Under expert parallelism every rank takes part in every layer's
 exchange until all ranks' sequences are done (a rank whose sequences finished joins with none).
 """
 from __future__ import annotations
@@ -65,13 +71,15 @@ class BatchDecoder:
     attn_layers: gtmoe.decoder.AttnLayerWeights (weights only; the caches live here, one K and one
     V tensor per layer laid out [max_seqs][capacity][kv_heads * head_dim]); moe: LocalMoe or
     PeerEpMoe; embed: the tied embedding dict (w, s, b, rows, in_dim); final_norm: bf16 bits
-    [hidden]; max_pos: the longest prompt + generated tokens any sequence reaches."""
+    [hidden]; max_pos: the longest prompt + generated tokens any sequence reaches (a prefix included);
+    kv_format: None for fp32 caches, else the one-byte format of gtmoe.kvcache.KvCache."""
 
     SOFTCAP = 30.0
 
     def __init__(self, attn_layers, moe, embed: dict, final_norm, max_pos: int, max_seqs: int,
-                 eps: float = 1e-6, device: str = "cuda", dist=None):
+                 eps: float = 1e-6, device: str = "cuda", dist=None, kv_format: str | None = None):
         import torch
+        from .kvcache import KvAttention, KvCache
         self.attn, self.moe, self.embed, self.final_norm, self.eps = attn_layers, moe, embed, final_norm, eps
         self.max_pos, self.max_seqs, self.dist = max_pos, max_seqs, dist
         f32 = dict(dtype=torch.float32, device=device)
@@ -81,13 +89,23 @@ class BatchDecoder:
         self.attn_out = torch.zeros(max_seqs, HIDDEN, **f32)
         self.tokens = torch.zeros(max_seqs, dtype=torch.int32, device=device)
         self.lm = LmHead(embed["rows"], device=device)
-        self.caches = []    # [layer] -> (k, v), each [max_seqs][capacity][kv_heads * head_dim]
+        self.kv_format, self.device = kv_format, device
+        self.prefix_len, self.prefixes = 0, None   # the common prompt's positions, and its caches by layer
+        self.logits = None
+        self.caches = []    # [layer] -> (k, v), each [max_seqs][capacity][kv_heads * head_dim], or a KvCache
+        self.kv_ops = {}    # KvAttention by (query heads, kv heads, head_dim)
         qn = max(a.num_heads * a.head_dim for a in attn_layers)
         kn = max(a.kv_heads * a.head_dim for a in attn_layers)
         ws = 0
         for a in attn_layers:
             cap = self.capacity(a)
             row = a.kv_heads * a.head_dim
+            if kv_format is not None:
+                self.caches.append(KvCache(max_seqs, cap, a.kv_heads, a.head_dim, kv_format, device=device))
+                key = (a.num_heads, a.kv_heads, a.head_dim)
+                if key not in self.kv_ops:
+                    self.kv_ops[key] = KvAttention(*key, max_seqs, device=device)
+                continue
             self.caches.append((torch.zeros(max_seqs, cap, row, **f32), torch.zeros(max_seqs, cap, row, **f32)))
             ws = max(ws, lib().gtm_attention_rows_workspace_bytes(a.num_heads, a.head_dim, cap, max_seqs))
         # flat scratch, viewed [n, width] with each layer's widths (sliding and full layers differ)
@@ -110,7 +128,17 @@ class BatchDecoder:
         check(lib().gtm_gemv_q4_rows(m["rows"], m["in_dim"], n, ptr(m["w"]), ptr(m["s"]), ptr(m["b"]), ptr(x), ptr(out),
                                      st))
 
-    def _attention(self, l: int, n: int, seqs, pos, st) -> None:
+    def _attention_kv(self, l: int, n: int, seqs, pos, q, k, v, ctx, prefill: bool) -> None:
+        """Layer l's attention over one-byte caches: the sequences' own behind the prefix, or, while the
+        prefix itself is run, the prefix's rows among themselves."""
+        a = self.attn[l]
+        cache = self.prefixes[l] if prefill else self.caches[l]
+        cache.write(q, k, v, q, pos, seqs, q_w=a.q_norm, k_w=a.k_norm, eps=self.eps, rotated_pairs=a.rotated_pairs,
+                    theta=a.theta)
+        prefix, plen = (cache, int(pos[n - 1]) + 1) if prefill else (self.prefixes[l], self.prefix_len) if self.prefix_len else (None, 0)
+        self.kv_ops[a.num_heads, a.kv_heads, a.head_dim](q, cache, seqs, pos, ctx, window=a.window, prefix=prefix, prefix_len=plen)
+
+    def _attention(self, l: int, n: int, seqs, pos, st, prefill: bool = False) -> None:
         """Layer l's attention for the step's n rows: hidden[:n] -> mid[:n]."""
         L = lib()
         a = self.attn[l]
@@ -123,6 +151,17 @@ class BatchDecoder:
         if a.v is not None:
             self._gemv(a.v, n, self.normed, v, st)
         v_src = v if a.v is not None else k   # full layers: V is k_proj's output
+        if self.kv_format is not None:
+            self._attention_kv(l, n, seqs, pos, q, k, v_src, ctx, prefill)
+        else:
+            self._attention_f32(l, n, seqs, pos, q, k, v_src, ctx, st)
+        self._gemv(a.o, n, ctx, self.attn_out, st)
+        check(L.gtm_post_attn_rows(n, HIDDEN, ptr(self.attn_out), ptr(self.hidden), ptr(a.post_attn_norm), None, None,
+                                   self.eps, ptr(self.mid), None, None, None, st))
+
+    def _attention_f32(self, l: int, n: int, seqs, pos, q, k, v_src, ctx, st) -> None:
+        L = lib()
+        a = self.attn[l]
         cap = self.capacity(a)
         kc, vc = self.caches[l]
         S = self.max_seqs
@@ -135,13 +174,20 @@ class BatchDecoder:
         check(L.gtm_attention_decode_rows(a.num_heads, a.kv_heads, a.head_dim, n, a.window, cap, ptr(q), ptr(kc),
                                           ptr(vc), seqs, S, pos, ptr(ctx), C.c_void_p(self.workspace.data_ptr()),
                                           self.ws_bytes, st))
-        self._gemv(a.o, n, ctx, self.attn_out, st)
-        check(L.gtm_post_attn_rows(n, HIDDEN, ptr(self.attn_out), ptr(self.hidden), ptr(a.post_attn_norm), None, None,
-                                   self.eps, ptr(self.mid), None, None, None, st))
 
-    def step(self, seqs, toks, positions, heads) -> None:
+    def step(self, seqs, toks, positions, heads, prefill: bool = False) -> None:
         """One step: row i carries sequence seqs[i]'s token toks[i] at positions[i]; rows in
-        `heads` (the sequences past their prompt) get their greedy next token in self.tokens."""
+        `heads` (the sequences past their prompt) get their greedy next token in self.tokens.
+        prefill: the rows are consecutive tokens of the prefix (seqs all 0)."""
+        self._layers(seqs, toks, positions, prefill)
+        st = _stream()
+        n, e = len(seqs), self.embed
+        if heads:
+            check(lib().gtm_rmsnorm_rows(n, HIDDEN, ptr(self.hidden), ptr(self.final_norm), self.eps, ptr(self.normed), st))
+        for i in heads:
+            self.lm(e["w"], e["s"], e["b"], self.normed[i], self.tokens[i:i + 1])
+
+    def _layers(self, seqs, toks, positions, prefill: bool) -> None:
         st = _stream()
         L = lib()
         e = self.embed
@@ -149,15 +195,37 @@ class BatchDecoder:
         if n:
             check(L.gtm_embed_lookup_rows(e["rows"], e["in_dim"], ptr(e["w"]), ptr(e["s"]), ptr(e["b"]), self._u32(toks),
                                           n, self.scale, ptr(self.hidden), st))
-        sq, ps = self._u32(seqs), self._u32(positions)
+        if self.kv_format is not None:
+            import numpy as np
+            sq, ps = np.asarray(seqs, dtype=np.uint32), np.asarray(positions, dtype=np.uint32)
+        else:
+            sq, ps = self._u32(seqs), self._u32(positions)
         for l in range(len(self.attn)):
             if n:
-                self._attention(l, n, sq, ps, st)
+                self._attention(l, n, sq, ps, st, prefill)
             self.moe(l, self.mid[:n], self.hidden[:n])
-        if heads:
-            check(L.gtm_rmsnorm_rows(n, HIDDEN, ptr(self.hidden), ptr(self.final_norm), self.eps, ptr(self.normed), st))
-        for i in heads:
-            self.lm(e["w"], e["s"], e["b"], self.normed[i], self.tokens[i:i + 1])
+
+    def set_prefix(self, tokens) -> None:
+        """Runs `tokens`, which every later prompt is taken to begin with, and keeps their keys and values
+        once for all sequences (kv_format caches only; [] takes the prefix away). The tokens go through the
+        layers max_seqs at a time."""
+        from .kvcache import KvCache
+        if self.kv_format is None:
+            raise ValueError("a shared prefix needs kv_format")
+        if self.dist is not None and self.dist.get_world_size() > 1:
+            raise ValueError("a shared prefix is run on one rank")
+        if len(tokens) >= self.max_pos:
+            raise ValueError(f"a prefix of {len(tokens)} tokens leaves no position of {self.max_pos}")
+        self.prefix_len, self.prefixes = 0, None
+        if len(tokens) == 0:
+            return
+        # a sliding layer's rows of one step reach back window - 1 positions from the first of them
+        self.prefixes = [KvCache(1, min(len(tokens), a.window + self.max_seqs - 1) if a.window > 0 else len(tokens), a.kv_heads,
+                                 a.head_dim, self.kv_format, device=self.device) for a in self.attn]
+        for p in range(0, len(tokens), self.max_seqs):
+            part = [int(t) for t in tokens[p:p + self.max_seqs]]
+            self.step([0] * len(part), part, list(range(p, p + len(part))), [], prefill=True)
+        self.prefix_len = len(tokens)
 
     def _all_done(self, done: bool) -> bool:
         if self.dist is None:
@@ -169,17 +237,54 @@ class BatchDecoder:
 
     def greedy(self, prompts, max_tokens: int, stops=(1, 106, 50), on_step=None) -> list[list[int]]:
         """CpuReference::generate's greedy loop for every prompt, advanced together: sequence i
-        prefills prompts[i] at positions 0.., then feeds back its argmax token until it has
-        max_tokens tokens or meets a stop id. on_step(step) is called after every step."""
+        prefills prompts[i] at positions 0.. (behind the prefix, where one is set), then feeds back its
+        argmax token until it has max_tokens tokens or meets a stop id. on_step(step) is called after every
+        step."""
+        return self._generate(prompts, max_tokens, stops, on_step, None)
+
+    def sample(self, prompts, max_tokens: int, params, generator=None, stops=(1, 106, 50), on_step=None) -> list[list[int]]:
+        """The same loop with sampled tokens: params is one gtmoe.sampling.RowParams or a list of one per
+        prompt; each step draws one uniform per sequence, in order, from `generator` (a torch.Generator on
+        the device; None: torch's default), whether or not the sequence is past its prompt, so a sequence's
+        tokens do not depend on the others' lengths. Logits are softcapped as in DeviceDecoder.sample."""
+        import torch
+        from .sampling import RowSampler
+        if not isinstance(params, (list, tuple)):
+            params = [params] * len(prompts)
+        if len(params) != len(prompts):
+            raise ValueError(f"{len(params)} settings for {len(prompts)} prompts")
+        if self.logits is None:
+            self.logits = torch.zeros(self.max_seqs, self.embed["rows"], dtype=torch.float32, device=self.device)
+            self.sampler = RowSampler(self.embed["rows"], self.max_seqs, device=self.device)
+        return self._generate(prompts, max_tokens, stops, on_step, (params, generator))
+
+    def _sampled(self, seqs, heads, params, uniforms) -> list[int]:
+        """Tokens of the rows in `heads` after the step's layers."""
+        import torch
+        st, L, e, n = _stream(), lib(), self.embed, len(heads)
+        check(L.gtm_rmsnorm_rows(len(seqs), HIDDEN, ptr(self.hidden), ptr(self.final_norm), self.eps, ptr(self.normed), st))
+        rows = self.normed[:len(seqs)] if n == len(seqs) else self.normed[torch.tensor(heads, device=self.hidden.device)]
+        logits = self.logits[:n]
+        self._gemv(e, n, rows, logits, st)   # tie_word_embeddings
+        check(L.gtm_softcap(logits.numel(), ptr(logits), self.SOFTCAP, ptr(logits), st))
+        own = [seqs[i] for i in heads]
+        u = uniforms[torch.tensor(own, device=uniforms.device)]
+        got = self.sampler(logits, [params[i] for i in own], u).tokens.cpu().tolist()
+        if min(got) < 0:
+            raise RuntimeError("a row without a finite largest logit")
+        return got
+
+    def _generate(self, prompts, max_tokens: int, stops, on_step, sampling) -> list[list[int]]:
         if len(prompts) > self.max_seqs:
             raise ValueError(f"{len(prompts)} prompts > max_seqs {self.max_seqs}")
         if any(len(p) == 0 for p in prompts):
             raise ValueError("empty prompt")   # cpu_reference.cpp:546
-        if any(len(p) + max_tokens > self.max_pos for p in prompts):
+        if any(self.prefix_len + len(p) + max_tokens > self.max_pos for p in prompts):
             raise ValueError(f"a prompt plus {max_tokens} tokens exceeds max_pos {self.max_pos}")
-        for kc, vc in self.caches:
-            kc.zero_()
-            vc.zero_()
+        if self.kv_format is None:
+            for kc, vc in self.caches:
+                kc.zero_()
+                vc.zero_()
         out = [[] for _ in prompts]
         live = [max_tokens > 0 for _ in prompts]
         step = 0
@@ -196,19 +301,25 @@ class BatchDecoder:
                     heads.append(len(seqs))
                 seqs.append(i)
                 toks.append(t)
-                pos.append(step)
-            self.step(seqs, toks, pos, heads)
-            if heads:
-                got = self.tokens[:len(seqs)].cpu().tolist()
-                for r in heads:
-                    i = seqs[r]
-                    nxt = int(got[r])
-                    if nxt in stops:
-                        live[i] = False
-                        continue
-                    out[i].append(nxt)
-                    if len(out[i]) >= max_tokens:
-                        live[i] = False
+                pos.append(self.prefix_len + step)
+            if sampling is None:
+                self.step(seqs, toks, pos, heads)
+                got = dict(zip(range(len(seqs)), self.tokens[:len(seqs)].cpu().tolist())) if heads else {}
+            else:
+                import torch
+                params, generator = sampling
+                uniforms = torch.rand(len(prompts), dtype=torch.float64, device=self.hidden.device, generator=generator)
+                self.step(seqs, toks, pos, [])
+                got = dict(zip(heads, self._sampled(seqs, heads, params, uniforms))) if heads else {}
+            for r in heads:
+                i = seqs[r]
+                nxt = int(got[r])
+                if nxt in stops:
+                    live[i] = False
+                    continue
+                out[i].append(nxt)
+                if len(out[i]) >= max_tokens:
+                    live[i] = False
             if on_step is not None:
                 on_step(step)
             step += 1
