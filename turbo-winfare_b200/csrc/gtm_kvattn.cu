@@ -45,33 +45,44 @@ struct Starts {
 
 template <int HD>
 struct RowsShape {
-    static constexpr int kWarps = HD == 128 ? 4 : 8;
+    static constexpr int kWarps = HD == 512 ? 8 : 4;   // of each kind
     static constexpr int kTile = 16 * kWarps;
     static constexpr int kDims = HD / kWarps;   // V dims of a warp
     static constexpr int kD = kDims / 8;        // contiguous V codes of a thread: 8 or 4
     static constexpr int kChunks = HD / 64;
+    static constexpr int kThreads = 2 * kWarps * 32;
 };
 
-// A tile: each warp scores 16 positions (A = K: 16 positions x 16 dims; B = q: 16 dims x 8 heads),
-// the CTA agrees on the heads' maxima, and each warp adds all the tile's positions to its share of
-// the dims (A = V^T: 16 dims x 16 positions; B = p). The order of dims and positions inside a
-// product is free, so threads read contiguous codes: 16 of a K vector, kD of a V vector. Codes of
-// the next tile are loaded into the registers that the products have just emptied.
+// Barriers among part of the CTA's warps: a full wait, and an arrival that does not wait.
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" :: "r"(id), "r"(threads) : "memory"); }
+
+// A tile's two products are made by two kinds of warps, so that both run at once: the first half of the
+// CTA scores 16 positions a warp (A = K: 16 positions x 16 dims; B = q: 16 dims x 8 heads), agrees on
+// the heads' maxima and leaves the weights in one of two buffers; the second half adds all of the tile's
+// positions to a warp's share of the dims (A = V^T: 16 dims x 16 positions; B = p). The order of dims and
+// positions inside a product is free, so threads read contiguous codes: 16 of a K vector, kD of a V
+// vector. Codes of the next tile are loaded into the registers that the products have just emptied.
 template <int HD, int FMT>
-__global__ void __launch_bounds__(RowsShape<HD>::kWarps * 32, HD == 512 ? 1 : 2)
+__global__ void __launch_bounds__(RowsShape<HD>::kThreads, HD == 512 ? 1 : 2)
     kv_rows(const __grid_constant__ RowsArgs a, const __grid_constant__ Starts starts, const __grid_constant__ RowU32 pos,
             const __grid_constant__ RowU32 seq) {
     using S = RowsShape<HD>;
-    constexpr int T = S::kTile, W = S::kWarps, D = S::kD, C = S::kChunks;
+    constexpr int T = S::kTile, W = S::kWarps, D = S::kD, C = S::kChunks, kHalf = W * 32, kAll = S::kThreads;
     constexpr int kPad = T + 8;   // halves per head row of P
-    __shared__ uint4 qf_s[C][2][2][32];               // [64-dim chunk][limb][half][lane]: B fragments of q
-    __shared__ __align__(16) __half p_s[2][8][kPad];  // [limb][head][position]
-    __shared__ __align__(16) uint64_t kaddr[2][T], vaddr[2][T];
-    __shared__ float2 sc_s[2][T];                     // ks, vs
-    __shared__ float wmax[W][8], qscale[8], lsum[W][8];
+    constexpr int kScorers = 1, kFull = 2, kEmpty = 4;   // barriers; a buffer's number is added to the last two
+    __shared__ uint4 qf_s[C][2][2][32];                  // [64-dim chunk][limb][half][lane]: B fragments of q
+    __shared__ __align__(16) __half p_s[2][2][8][kPad];  // [buffer][limb][head][position]
+    __shared__ float f_s[2][8];                          // what the sums so far are multiplied by
+    // addresses of the codes of four tiles: the scorers are two tiles ahead at most, and each looks one further
+    __shared__ __align__(16) uint64_t kaddr[4][T], vaddr[4][T];
+    __shared__ float2 sc_s[2][T];                        // ks, vs
+    __shared__ float wmax[2][W][8], qscale[8], lsum[W][8], m_s[8];
 
     const uint32_t item = blockIdx.x, kvh = blockIdx.y;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane & 3, oct = lane >> 2;
+    const bool scorer = warp < W;
+    const int part = scorer ? warp : warp - W;   // the warp among its kind
     uint32_t row = 0;
     for (uint32_t step = 256; step; step >>= 1)
         if (row + step < a.n && starts.v[row + step] <= item) row += step;
@@ -83,36 +94,32 @@ __global__ void __launch_bounds__(RowsShape<HD>::kWarps * 32, HD == 512 ? 1 : 2)
     if (!a.list_prefix) sp.pn = 0;
     const uint32_t total = sp.pn + sp.on;
     const uint32_t j0 = (item - starts.v[row]) * a.chunk, j1 = min(total, j0 + a.chunk);
+    const uint32_t tiles = (j1 - j0 + T - 1) / T;
     const uint32_t pslot = sp.pn ? sp.pa % a.pre.capacity : 0, oslot = sp.oa % a.own.capacity;
     const uint64_t own_vec = static_cast<uint64_t>(seq.v[row]) * a.own.capacity * a.kv_heads + kvh;
     const uint64_t own_sc = (static_cast<uint64_t>(seq.v[row]) * a.kv_heads + kvh) * a.own.capacity;
 
-    // list position j: addresses of its K and V codes, and its scales
-    auto place = [&](uint32_t j, uint64_t& ka, uint64_t& va, float2& s) {
+    // Entry tid of tile t: addresses of its K and V codes, and its scales. The last position stands in for those
+    // past the run (their weight is 0).
+    auto write_places = [&](uint32_t t, float2& sc) {
+        if (tid >= T) return;
+        const uint32_t j = min(j0 + t * T + tid, j1 - 1);
         const bool p = j < sp.pn;
         const uint32_t cap = p ? a.pre.capacity : a.own.capacity;
         uint64_t slot = p ? static_cast<uint64_t>(pslot) + j : static_cast<uint64_t>(oslot) + (j - sp.pn);
         if (slot >= cap) slot -= cap;
         const uint64_t vec = ((p ? kvh : own_vec) + slot * a.kv_heads) * HD;
-        const uint64_t sc = (p ? static_cast<uint64_t>(kvh) * cap : own_sc) + slot;
-        ka = reinterpret_cast<uint64_t>((p ? a.pre.k : a.own.k) + vec);
-        va = reinterpret_cast<uint64_t>((p ? a.pre.v : a.own.v) + vec);
-        s = make_float2(__ldg((p ? a.pre.ks : a.own.ks) + sc), __ldg((p ? a.pre.vs : a.own.vs) + sc));
-    };
-    // entry tid of tile t: the last position stands in for those past the run (their weight is 0)
-    auto write_places = [&](uint32_t t, float2& s) {
-        if (tid < T) {
-            uint64_t ka, va;
-            place(min(j0 + t * T + tid, j1 - 1), ka, va, s);
-            kaddr[t & 1][tid] = ka, vaddr[t & 1][tid] = va;
-        }
+        const uint64_t at = (p ? static_cast<uint64_t>(kvh) * cap : own_sc) + slot;
+        kaddr[t & 3][tid] = reinterpret_cast<uint64_t>((p ? a.pre.k : a.own.k) + vec);
+        vaddr[t & 3][tid] = reinterpret_cast<uint64_t>((p ? a.pre.v : a.own.v) + vec);
+        sc = make_float2(__ldg((p ? a.pre.ks : a.own.ks) + at), __ldg((p ? a.pre.vs : a.own.vs) + at));
     };
 
     float2 sc_next = make_float2(0.0f, 0.0f);
     write_places(0, sc_next);
     if (tid < T) sc_s[0][tid] = sc_next;
     // q of head h: scaled by a power of two into [1, 2), then high and low fp16 parts
-    for (int h = warp; h < 8; h += W) {
+    for (int h = warp; h < 8; h += 2 * W) {
         const float* src = a.q + (static_cast<size_t>(row) * a.q_heads + static_cast<size_t>(kvh) * grp + h) * HD;
         float x[HD / 32], top = 0.0f;
 #pragma unroll
@@ -144,21 +151,115 @@ __global__ void __launch_bounds__(RowsShape<HD>::kWarps * 32, HD == 512 ? 1 : 2)
     }
     __syncthreads();
 
-    uint4 kr[2][C];
-    uint32_t vr[T / 16][4][D / 4];
-    auto load_k = [&](uint32_t t) {
+    if (scorer) {
+        uint4 kr[2][C];
+        auto load_k = [&](uint32_t t) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const uint4* p = reinterpret_cast<const uint4*>(kaddr[t & 1][warp * 16 + oct + 8 * r]) + quad;
+            for (int r = 0; r < 2; ++r) {
+                const uint4* p = reinterpret_cast<const uint4*>(kaddr[t & 3][part * 16 + oct + 8 * r]) + quad;
 #pragma unroll
-            for (int c = 0; c < C; ++c) kr[r][c] = __ldg(p + 4 * c);
+                for (int c = 0; c < C; ++c) kr[r][c] = __ldg(p + 4 * c);
+            }
+        };
+        load_k(0);
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        const float qs[2] = {qscale[2 * quad], qscale[2 * quad + 1]};
+        for (uint32_t t = 0; t < tiles; ++t) {
+            const bool more = t + 1 < tiles;
+            const int buf = t & 1;
+            if (more) write_places(t + 1, sc_next);
+            // four sums per score (limb, half of the dims' runs): short chains, as each product's addition
+            // to the accumulator is cut to fp32 rather than rounded, and four products in flight
+            float part4[4][4] = {};
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const uint32_t w0[4] = {kr[0][c].x, kr[0][c].y, kr[0][c].z, kr[0][c].w};
+                const uint32_t w1[4] = {kr[1][c].x, kr[1][c].y, kr[1][c].z, kr[1][c].w};
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint4 hi = qf_s[c][0][half][lane], lo = qf_s[c][1][half][lane];
+                    const uint32_t bh[4] = {hi.x, hi.y, hi.z, hi.w}, bl[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t b0 = bias_codes<FMT>(w0[2 * half + j]), b1 = bias_codes<FMT>(w1[2 * half + j]);
+                        const uint32_t a0 = pair_in_word<FMT, 0>(b0), a2 = pair_in_word<FMT, 1>(b0);
+                        const uint32_t a1 = pair_in_word<FMT, 0>(b1), a3 = pair_in_word<FMT, 1>(b1);
+                        mma16816(part4[j], a0, a1, a2, a3, bh[2 * j], bh[2 * j + 1]);
+                        mma16816(part4[2 + j], a0, a1, a2, a3, bl[2 * j], bl[2 * j + 1]);
+                    }
+                }
+            }
+            float s[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] = (part4[0][i] + part4[1][i]) + (part4[2][i] + part4[3][i]);
+            // s: positions oct and oct + 8 of the warp's 16, heads 2 quad and 2 quad + 1
+            float vs[2], top[2] = {-INFINITY, -INFINITY};
+            bool valid[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int p = part * 16 + oct + 8 * r;
+                const float2 sc = sc_s[buf][p];
+                valid[r] = j0 + t * T + p < j1;
+                vs[r] = sc.y;
+                const float lg = log2f(fmaxf(sc.y, kKvTiny));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    s[2 * r + h] = valid[r] ? s[2 * r + h] * sc.x * qs[h] : -INFINITY;
+                    top[h] = fmaxf(top[h], s[2 * r + h] + (valid[r] ? lg : 0.0f));
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                for (int x = 4; x < 32; x <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], x));
+            }
+            if (oct == 0) *reinterpret_cast<float2*>(&wmax[buf][part][2 * quad]) = make_float2(top[0], top[1]);
+            if (more && tid < T) sc_s[buf ^ 1][tid] = sc_next;
+            bar_sync(kScorers, kHalf);
+            if (more) load_k(t + 1);
+            float mn[2] = {m[0], m[1]};
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float2 x = *reinterpret_cast<const float2*>(&wmax[buf][w][2 * quad]);
+                mn[0] = fmaxf(mn[0], x.x), mn[1] = fmaxf(mn[1], x.y);
+            }
+            if (t >= 2) bar_sync(kEmpty + buf, kAll);   // the sums of tile t - 2 have used the buffer
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float f = m[h] == mn[h] ? 1.0f : ex2(m[h] - mn[h]);
+                m[h] = mn[h];
+                l[h] *= f;
+                if (part == 0 && oct == 0) f_s[buf][2 * quad + h] = f;
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float e = valid[r] ? ex2(s[2 * r + h] - mn[h]) : 0.0f;
+                    l[h] += e;
+                    const float p = valid[r] ? e * vs[r] : 0.0f;
+                    const __half hi = __float2half_rn(p);
+                    const int at = part * 16 + oct + 8 * r;
+                    p_s[buf][0][2 * quad + h][at] = hi;
+                    p_s[buf][1][2 * quad + h][at] = __float2half_rn(p - __half2float(hi));
+                }
+            }
+            bar_arrive(kFull + buf, kAll);
         }
-    };
-    const uint64_t vdim = static_cast<uint64_t>(warp * S::kDims + oct * D);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            for (int x = 4; x < 32; x <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], x);
+        }
+        if (oct == 0) {
+            lsum[part][2 * quad] = l[0], lsum[part][2 * quad + 1] = l[1];
+            if (part == 0) m_s[2 * quad] = m[0], m_s[2 * quad + 1] = m[1];
+        }
+        __syncthreads();
+        return;
+    }
+
+    uint32_t vr[T / 16][4][D / 4];
+    const uint64_t vdim = static_cast<uint64_t>(part * S::kDims + oct * D);
     auto load_v = [&](uint32_t t, int ks) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const uint64_t p = vaddr[t & 1][16 * ks + 4 * quad + r] + vdim;
+            const uint64_t p = vaddr[t & 3][16 * ks + 4 * quad + r] + vdim;
             if constexpr (D == 8) {
                 const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
                 vr[ks][r][0] = w.x, vr[ks][r][1] = w.y;
@@ -167,99 +268,23 @@ __global__ void __launch_bounds__(RowsShape<HD>::kWarps * 32, HD == 512 ? 1 : 2)
             }
         }
     };
-    const uint32_t tiles = (j1 - j0 + T - 1) / T;
-    load_k(0);
 #pragma unroll
     for (int ks = 0; ks < T / 16; ++ks) load_v(0, ks);
-
     float o[D / 2][4];
 #pragma unroll
     for (int i = 0; i < D / 2; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    const float qs[2] = {qscale[2 * quad], qscale[2 * quad + 1]};
     for (uint32_t t = 0; t < tiles; ++t) {
         const bool more = t + 1 < tiles;
-        if (more) write_places(t + 1, sc_next);
-        // four sums per score (limb, half of the dims' runs): short chains, as each product's addition
-        // to the accumulator is cut to fp32 rather than rounded, and four products in flight
-        float part[4][4] = {};
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const uint32_t w0[4] = {kr[0][c].x, kr[0][c].y, kr[0][c].z, kr[0][c].w};
-            const uint32_t w1[4] = {kr[1][c].x, kr[1][c].y, kr[1][c].z, kr[1][c].w};
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint4 hi = qf_s[c][0][half][lane], lo = qf_s[c][1][half][lane];
-                const uint32_t bh[4] = {hi.x, hi.y, hi.z, hi.w}, bl[4] = {lo.x, lo.y, lo.z, lo.w};
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint32_t b0 = bias_codes<FMT>(w0[2 * half + j]), b1 = bias_codes<FMT>(w1[2 * half + j]);
-                    const uint32_t a0 = pair_in_word<FMT, 0>(b0), a2 = pair_in_word<FMT, 1>(b0);
-                    const uint32_t a1 = pair_in_word<FMT, 0>(b1), a3 = pair_in_word<FMT, 1>(b1);
-                    mma16816(part[j], a0, a1, a2, a3, bh[2 * j], bh[2 * j + 1]);
-                    mma16816(part[2 + j], a0, a1, a2, a3, bl[2 * j], bl[2 * j + 1]);
-                }
-            }
-        }
-        float s[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = (part[0][i] + part[1][i]) + (part[2][i] + part[3][i]);
-        // s: positions oct and oct + 8 of the warp's 16, heads 2 quad and 2 quad + 1
-        float vs[2], top[2] = {-INFINITY, -INFINITY};
-        bool valid[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int p = warp * 16 + oct + 8 * r;
-            const float2 sc = sc_s[t & 1][p];
-            valid[r] = j0 + t * T + p < j1;
-            vs[r] = sc.y;
-            const float lg = log2f(fmaxf(sc.y, kKvTiny));
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                s[2 * r + h] = valid[r] ? s[2 * r + h] * sc.x * qs[h] : -INFINITY;
-                top[h] = fmaxf(top[h], s[2 * r + h] + (valid[r] ? lg : 0.0f));
-            }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            for (int x = 4; x < 32; x <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], x));
-        }
-        if (oct == 0) *reinterpret_cast<float2*>(&wmax[warp][2 * quad]) = make_float2(top[0], top[1]);
-        __syncthreads();
-        if (more) {
-            load_k(t + 1);
-            if (tid < T) sc_s[(t + 1) & 1][tid] = sc_next;
-        }
-        float mn[2] = {m[0], m[1]}, fs[2];
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float2 x = *reinterpret_cast<const float2*>(&wmax[w][2 * quad]);
-            mn[0] = fmaxf(mn[0], x.x), mn[1] = fmaxf(mn[1], x.y);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            fs[h] = m[h] == mn[h] ? 1.0f : ex2(m[h] - mn[h]);
-            m[h] = mn[h];
-            l[h] *= fs[h];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const float e = valid[r] ? ex2(s[2 * r + h] - mn[h]) : 0.0f;
-                l[h] += e;
-                const float p = valid[r] ? e * vs[r] : 0.0f;
-                const __half hi = __float2half_rn(p);
-                const int at = warp * 16 + oct + 8 * r;
-                p_s[0][2 * quad + h][at] = hi;
-                p_s[1][2 * quad + h][at] = __float2half_rn(p - __half2float(hi));
-            }
-        }
-        __syncthreads();
+        const int buf = t & 1;
+        bar_sync(kFull + buf, kAll);   // the weights, and the addresses of the next tile
+        const float fs[2] = {f_s[buf][2 * quad], f_s[buf][2 * quad + 1]};
         float add[D / 2][4] = {};   // this tile's share, added to o in fp32 (see above)
 #pragma unroll
         for (int ks = 0; ks < T / 16; ++ks) {
-            const uint2 bh = *reinterpret_cast<const uint2*>(&p_s[0][oct][16 * ks + 4 * quad]);
-            const uint2 bl = *reinterpret_cast<const uint2*>(&p_s[1][oct][16 * ks + 4 * quad]);
+            const uint2 bh = *reinterpret_cast<const uint2*>(&p_s[buf][0][oct][16 * ks + 4 * quad]);
+            const uint2 bl = *reinterpret_cast<const uint2*>(&p_s[buf][1][oct][16 * ks + 4 * quad]);
 #pragma unroll
             for (int wd = 0; wd < D / 4; ++wd) {
                 uint32_t w[4];
@@ -275,35 +300,28 @@ __global__ void __launch_bounds__(RowsShape<HD>::kWarps * 32, HD == 512 ? 1 : 2)
             }
             if (more) load_v(t + 1, ks);
         }
+        if (t + 2 < tiles) bar_arrive(kEmpty + buf, kAll);
 #pragma unroll
         for (int i = 0; i < D / 2; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[i][j] = o[i][j] * fs[j & 1] + add[i][j];
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        for (int x = 4; x < 32; x <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], x);
-    }
-    if (oct == 0) lsum[warp][2 * quad] = l[0], lsum[warp][2 * quad + 1] = l[1];
     __syncthreads();
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        l[h] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) l[h] += lsum[w][2 * quad + h];
-    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int head = 2 * quad + h;
         if (head >= grp) continue;
-        const float f = (FMT == GTM_KV_E4M3 ? 256.0f : 1.0f) / (direct ? l[h] : 1.0f);
+        float l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) l += lsum[w][head];
+        const float f = (FMT == GTM_KV_E4M3 ? 256.0f : 1.0f) / (direct ? l : 1.0f);
         const size_t at = (static_cast<size_t>(item) * a.kv_heads + kvh) * grp + head;
         float* dst = direct ? a.ctx + (static_cast<size_t>(row) * a.q_heads + static_cast<size_t>(kvh) * grp + head) * HD : a.part + at * HD;
 #pragma unroll
         for (int i = 0; i < D / 4; ++i)
             *reinterpret_cast<float4*>(dst + vdim + 4 * i) =
                 make_float4(o[2 * i][h] * f, o[2 * i][h + 2] * f, o[2 * i + 1][h] * f, o[2 * i + 1][h + 2] * f);
-        if (!direct && warp == 0 && oct == 0) a.ml[at] = make_float2(m[h], l[h]);
+        if (!direct && part == 0 && oct == 0) a.ml[at] = make_float2(m_s[head], l);
     }
 }
 
@@ -374,9 +392,9 @@ int launch_rows(RowsArgs& a, Starts& starts, const RowU32& pos, const RowU32& se
     const dim3 grid(items, a.kv_heads);
     if (items) {
         if (fmt == GTM_KV_INT8)
-            kv_rows<HD, GTM_KV_INT8><<<grid, S::kWarps * 32, 0, st>>>(a, starts, pos, seq);
+            kv_rows<HD, GTM_KV_INT8><<<grid, S::kThreads, 0, st>>>(a, starts, pos, seq);
         else
-            kv_rows<HD, GTM_KV_E4M3><<<grid, S::kWarps * 32, 0, st>>>(a, starts, pos, seq);
+            kv_rows<HD, GTM_KV_E4M3><<<grid, S::kThreads, 0, st>>>(a, starts, pos, seq);
     }
     if (merge) kv_combine<HD><<<dim3(a.q_heads, a.n), HD / 4, 0, st>>>(a, starts, pos, sh);
     return GTM_OK;
