@@ -300,8 +300,29 @@ def test_attention(case, fmt):
     check_attention(cache, queries(n, H, hd), seqs, [P + m - 1 for m in lens], window, prefix, 1, P)
 
 
+# Prefixes long enough, over the rows together, to be computed once for all (98,304 positions x kv heads)
+SHARED = [  # as above
+    (3, 8, 8, 128, 0, 5000, 5000, [1, 2, 3]),
+    (40, 16, 8, 256, 0, 400, 400, list(range(1, 121, 3))),
+    (64, 16, 2, 512, 0, 1000, 1000, [1 + (i * 5) % 70 for i in range(64)]),
+    (33, 8, 1, 128, 0, 3100, 4000, [5] * 33),                           # ring larger than the prefix
+    (37, 14, 2, 256, 0, 1400, 1400, [1] * 37),                          # groups of 7 across units of 64
+    (64, 8, 4, 256, 700, 4000, 900, [1 + i for i in range(64)]),        # a wrapped ring, spans that move
+    (64, 4, 4, 128, 700, 4096, 768, [1 + i for i in range(64)]),        # a ring of whole tiles
+    (200, 16, 8, 128, 300, 2000, 2000, [1 + 3 * i for i in range(200)]),  # half of the rows past the prefix
+    (512, 3, 3, 512, 0, 65, 65, [2] * 512),
+    (100, 8, 8, 128, 0, 129, 129, [1] * 100),
+]
+
+
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
-@pytest.mark.parametrize("n,H,KV,hd,start,window", [(2, 16, 8, 256, 0, 0), (130, 16, 2, 512, 77, 0), (200, 6, 2, 128, 1000, 333),
+@pytest.mark.parametrize("case", SHARED)
+def test_attention_over_a_prefix_computed_once(case, fmt):
+    test_attention(case, fmt)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("n,H,KV,hd,start,window", [(300, 16, 2, 512, 200, 0), (400, 8, 2, 256, 1000, 333), (2, 16, 8, 256, 0, 0), (130, 16, 2, 512, 77, 0), (200, 6, 2, 128, 1000, 333),
                                                     (300, 8, 4, 256, 3, 17), (512, 2, 1, 128, 0, 0)])
 def test_attention_causal_rows_of_one_sequence(fmt, n, H, KV, hd, start, window):
     from gtmoe.kvcache import KvCache
@@ -329,17 +350,17 @@ def test_attention_uneven_scales(spread):
     import torch
     cache.v_scale.mul_(torch.from_numpy(f).cuda())
     check_attention(cache, queries(2, 8, 128), [1, 0], [199, 100])
-    prefix = cache
-    check_attention(cache, queries(30, 8, 128), [0] * 30, [150] * 30, 0, prefix, 1, 151)
+    for n in (30, 400):   # row by row, and once for all
+        check_attention(cache, queries(n, 8, 128), [0] * n, [150] * n, 0, cache, 1, 151)
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
-@pytest.mark.parametrize("many", [1, 40])
+@pytest.mark.parametrize("many", [1, 40, 400])
 def test_masked_rows_of_a_cache_do_not_matter(fmt, many):
     import torch
     from gtmoe.kvcache import KvCache
     P, cap = 100, 64
-    cache, prefix = KvCache(2, cap, 2, 256, fmt), KvCache(1, 128, 2, 256, fmt)
+    cache, prefix = KvCache(2, cap, 4, 256, fmt), KvCache(1, 128, 4, 256, fmt)
     fill(cache, 51)
     fill(prefix, 52)
     pos = [P + 20] * many
@@ -359,19 +380,22 @@ def test_masked_rows_of_a_cache_do_not_matter(fmt, many):
     assert torch.equal(run_attention(cache, q, seqs, pos, 90, prefix, 0, P), clean)
 
 
-def test_nan_vectors_reach_the_rows_that_attend_them_only():
+@pytest.mark.parametrize("repeat", [1, 45])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_nan_vectors_reach_the_rows_that_attend_them_only(repeat, which):
     import torch
     from gtmoe.kvcache import KvCache
-    cache = KvCache(1, 64, 2, 128)
+    cache = KvCache(1, 64, 8, 128)
     fill(cache, 61)
-    q = queries(12, 4, 128)
-    pos = list(range(20, 32))
-    clean = run_attention(cache, q, [0] * 12, pos, 0, cache, 0, 64)
-    cache.v_scale[0, 1, 25] = float("nan")   # kv head 1, position 25
-    got = run_attention(cache, q, [0] * 12, pos, 0, cache, 0, 64).view(12, 4, 128)
-    clean = clean.view(12, 4, 128)
-    assert torch.equal(got[:, :2], clean[:, :2]) and torch.equal(got[:5], clean[:5])
-    assert torch.isnan(got[5:, 2:]).all()
+    n = 11 * repeat
+    q = queries(n, 16, 128)
+    pos = sorted(list(range(20, 31)) * repeat)
+    clean = run_attention(cache, q, [0] * n, pos, 0, cache, 0, 64).view(n, 16, 128)
+    getattr(cache, which + "_scale")[0, 1, 25] = float("nan")   # kv head 1 (query heads 2 and 3), position 25
+    got = run_attention(cache, q, [0] * n, pos, 0, cache, 0, 64).view(n, 16, 128)
+    others = [h for h in range(16) if h not in (2, 3)]
+    assert torch.equal(got[:, others], clean[:, others]) and torch.equal(got[:5 * repeat], clean[:5 * repeat])
+    assert torch.isnan(got[5 * repeat:, 2:4]).all()
 
 
 def test_rows_behind_the_last_stay_and_repeats_are_equal():
@@ -389,21 +413,22 @@ def test_rows_behind_the_last_stay_and_repeats_are_equal():
     assert torch.equal(again, ctx[:3])
 
 
-def test_streams_and_graphs():
+@pytest.mark.parametrize("n", [6, 300])
+def test_streams_and_graphs(n):
     import torch
     from gtmoe.kvcache import KvAttention, KvCache
-    cache = KvCache(2, 128, 2, 256)
+    cache = KvCache(2, 400, 2, 256)
     fill(cache, 81)
-    H, n = 8, 6
+    H = 8
     q, kv = queries(n, H, 256, 1), queries(n, 4, 256, 2)
     k, v = kv[:, :512].contiguous(), kv[:, 512:].contiguous()
-    pos, seqs = [40, 41, 42, 43, 44, 45], [1] * n
+    pos, seqs = list(range(40, 40 + n)), [1] * n
     op = KvAttention(H, 2, 256, n)
     qo, ctx = torch.empty_like(q), torch.empty_like(q)
 
     def step(stream=None):
         cache.write(q, k, v, qo, pos, seqs, rotated_pairs=128, stream=stream)
-        op(qo, cache, seqs, pos, ctx, prefix=cache, prefix_seq=1, prefix_len=46, stream=stream)
+        op(qo, cache, seqs, pos, ctx, prefix=cache, prefix_seq=1, prefix_len=40 + n, stream=stream)
 
     step()
     want = ctx.clone()

@@ -361,6 +361,14 @@ __global__ void __launch_bounds__(HD / 4) kv_combine(const __grid_constant__ Row
         make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
 }
 
+// Prefix positions x kv heads over all rows from which the prefix is computed once for all (three rows or
+// more). kv_shared costs 8 (128 dims) to 25 us (512) however little it does; kv_rows reads the prefix again
+// for every row at 3.3-4.3 TB/s. Whole calls, once for all against row by row, int8: 16 rows x 2,048
+// positions x 2 heads of 512 (65,536) 44 against 42 us, 32 rows (131,072) 46 against 57, 32 rows x 16,384
+// 104 against 261; 4 rows x 2,048 x 8 heads of 256 (65,536) 32 against 28, 16 rows (262,144) 33 against 50,
+// 32 rows x 16,384 66 against 497; 2 rows x 16,384 x 8 heads of 256 (262,144) 59 against 52.
+constexpr uint64_t kSharedFrom = 98304;
+
 // Items of all rows are at most n plus this (a chunk is at least the total / target).
 constexpr uint32_t kTargetCtas = 592;
 uint32_t target_items(uint32_t kv_heads) { return std::max(1u, kTargetCtas / kv_heads); }
@@ -466,8 +474,10 @@ GTM_API int gtm_attention_kv_rows(const GtmKvCache* c, const GtmKvCache* prefix,
     if (!ptr_aligned(q, 16) || !ptr_aligned(ctx, 16) || !ptr_aligned(ws, 16))
         return set_error(GTM_ERR_MISALIGNED, "%s: q, ctx and workspace need 16-byte alignment", fn);
     RowU32 pos, seq;
+    uint64_t in_prefix = 0;
     for (uint32_t i = 0; i < n; ++i) {
         const Span s = row_span(positions[i], window, prefix_len);
+        in_prefix += s.pn;
         if (positions[i] == 0xFFFFFFFFu || seqs[i] >= c->num_seqs || s.on > c->capacity ||
             (s.pn && prefix_len - s.pa > prefix->capacity))
             return set_error(GTM_ERR_INVALID, "%s: row %u (sequence %u of %u, position %u, prefix %u) does not fit the rings", fn,
@@ -496,7 +506,7 @@ GTM_API int gtm_attention_kv_rows(const GtmKvCache* c, const GtmKvCache* prefix,
     SharedPlan plan;
     plan.units = 0;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    a.list_prefix = !(prefix_len && n > 1);
+    a.list_prefix = n < 3 || in_prefix * c->kv_heads < kSharedFrom;
     if (!a.list_prefix) {
         const SharedCall call{prefix, prefix_seq, prefix_len, q_heads, c->kv_heads, c->head_dim, n, window, q};
         plan_shared(call, pos, sms, plan);

@@ -45,7 +45,7 @@ constexpr int TP = 128;              // positions of a tile
 constexpr int kThreads = 640;
 constexpr uint64_t kWaitNs = 1000000000ull;
 constexpr int KA = 4;                // K chunks (64 dims) in tensor memory
-constexpr uint32_t kLongest = 16;    // tiles summed in tensor memory before the result goes to memory
+constexpr uint32_t kLongest = 20;    // tiles summed in tensor memory before the result goes to memory
 
 template <int HD>
 struct Shape {
@@ -188,6 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (tid < N) a.plan.ml[static_cast<size_t>(sg.slot) * N + tid] = make_float2(0.0f, __int_as_float(0x7FC00000));
             return false;
         }
+        if (sg.slot == done_slot) return true;   // the same unit goes on: its q, spans and maxima stay
         // ---- q's limbs and the rows' spans
         for (int r = warp; r < N; r += kThreads / 32) {
             const uint32_t qr = sg.unit * N + r, row = qr / a.grp, h = qr - row * a.grp;
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (lane == 0) {
                 qf_s[r] = __int_as_float((127 + e) << 23) * kLog2e * (FMT == GTM_KV_E4M3 ? 256.0f : 1.0f);
-                if (sg.slot != done_slot) m_s[r] = -INFINITY;   // else this unit's maxima go on
+                m_s[r] = -INFINITY;
                 const Span sp = live ? row_span(pos.v[row], a.window, a.prefix_len) : Span{0, 0, 0, 0};
                 // columns without a row are never read: they need no mask
                 rlo[r] = !live ? 0u : sp.pn ? sp.pa - a.lo[sg.unit] : 1u;
@@ -410,7 +411,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     f_c[p] = f * (FMT == GTM_KV_E4M3 ? 256.0f : 1.0f);
                     g_s[col0 + p] = gold;
                 }
-                tc::named_bar_sync(bar, 128);
+                // scales as they were (mostly): what is there only has to be added to, which needs no answer
+                const bool rescale = any_of_128(bar, merge && p < H && g_s[col0 + p] != 1.0f);
                 for (int c0 = 0; c0 < MT * 2; ++c0) {
                     uint32_t v[16];
                     const int r0 = (c0 & 1) * 16;
@@ -423,14 +425,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     float* dst = part + static_cast<size_t>(r0) * HD + (c0 >> 1) * 128 + p;
                     float old[16];
-                    if (merge) {
+                    if (rescale) {
 #pragma unroll
                         for (int c = 0; c < 16; ++c) old[c] = dst[c * HD];
                     }
 #pragma unroll
                     for (int c = 0; c < 16; ++c) {
                         const float o = __uint_as_float(v[c]) * f_c[r0 + c];
-                        dst[c * HD] = merge ? fmaf(old[c], g_s[col0 + r0 + c], o) : o;
+                        if (merge && !rescale)
+                            asm volatile("red.global.add.f32 [%0], %1;" :: "l"(dst + c * HD), "f"(o) : "memory");
+                        else
+                            dst[c * HD] = rescale ? fmaf(old[c], g_s[col0 + r0 + c], o) : o;
                     }
                 }
                 tc::tc_fence_before();
@@ -480,17 +485,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (; it < end; ++it) {
                 if (!__all_sync(0xffffffffu, tc::mbar_wait(&rv_full[it % RV], (it / RV) & 1, abort_flag, kWaitNs))) break;
                 const uint8_t* raw = sRawV + (it % RV) * 8192 + p * 128;
-                uint4 w[4];
+                uint32_t h[4][8];   // converted while the stage is still being multiplied
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4*>(raw + (((half * 4 + j) ^ (p & 7)) << 4));
+                for (int j = 0; j < 4; ++j) widen<FMT>(*reinterpret_cast<const uint4*>(raw + (((half * 4 + j) ^ (p & 7)) << 4)), h[j]);
                 if (!__all_sync(0xffffffffu, tc::mbar_wait(&v_empty[it % VST], ((it / VST) & 1) ^ 1, abort_flag, kWaitNs))) break;
                 uint8_t* dst = sV + (it % VST) * 16384 + half * 8192 + p * 128;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    uint32_t h[8];
-                    widen<FMT>(w[j], h);
-                    *reinterpret_cast<uint4*>(dst + (((2 * j) ^ (p & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4*>(dst + (((2 * j + 1) ^ (p & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+                    *reinterpret_cast<uint4*>(dst + (((2 * j) ^ (p & 7)) << 4)) = make_uint4(h[j][0], h[j][1], h[j][2], h[j][3]);
+                    *reinterpret_cast<uint4*>(dst + (((2 * j + 1) ^ (p & 7)) << 4)) = make_uint4(h[j][4], h[j][5], h[j][6], h[j][7]);
                 }
                 tc::fence_proxy_async_smem();
                 arrive_warp(&v_full[it % VST], &rv_empty[it % RV]);
