@@ -503,3 +503,72 @@ def test_a_step_of_write_read_and_attend_together():
     assert (np.abs(ctx.cpu().numpy() - want).max(1) <= tol).all()
     kr, _ = cache.read(2, P, 10)
     assert np.array_equal(kr.cpu().numpy(), values(cache, "k")[2][np.arange(P, P + 10) % 20].reshape(10, -1).astype(np.float32))
+
+
+def test_host_tensors_are_refused():
+    """Before any launch: a kernel is never given a host pointer."""
+    import torch
+    import gtmoe
+    from gtmoe.kvcache import KvAttention, KvCache
+    from gtmoe.sampling import RowParams, RowSampler
+    c, q = KvCache(1, 4, 1, 128, device="cpu"), torch.zeros(1, 128)
+    for call in (lambda: c.write(q, q, q, q, [0], [0]), lambda: c.read(0, 0, 1),
+                 lambda: KvAttention(1, 1, 128, 1, device="cpu")(q, c, [0], [0], torch.zeros(1, 128)),
+                 lambda: RowSampler(4, 1, device="cpu")(torch.zeros(1, 4), [RowParams()])):
+        with pytest.raises(gtmoe.GtmError, match="not on a GPU"):
+            call()
+
+
+def test_two_calls_at_once_on_two_streams():
+    """Each with its own workspace, over one cache and prefix: the results of the calls one by one."""
+    import torch
+    from gtmoe.kvcache import KvAttention, KvCache
+    torch.manual_seed(9)
+    n, H, KV, hd, P = 24, 8, 2, 256, 4096
+    pre, own = KvCache(1, P, KV, hd), KvCache(n, 64, KV, hd)
+    for c in (pre, own):
+        for t in (c.k, c.v):
+            t.copy_(torch.randint(-127, 128, t.shape, device="cuda", dtype=torch.int8))
+        for t in (c.k_scale, c.v_scale):
+            t.copy_(torch.rand_like(t) * 0.01 + 0.001)
+    q = [torch.randn(n, H * hd, device="cuda") * 0.1 for _ in range(2)]
+    pos = [P + i for i in range(n)]
+    ops = [KvAttention(H, KV, hd, n) for _ in range(2)]
+    want = [torch.empty_like(x) for x in q]
+    for x, w in zip(q, want):
+        ops[0](x, own, list(range(n)), pos, w, prefix=pre, prefix_len=P)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [torch.zeros_like(x) for x in q]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for i in range(2):
+            ops[i](q[i], own, list(range(n)), pos, got[i], prefix=pre, prefix_len=P, stream=streams[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+@pytest.mark.parametrize("prefix", [False, True])
+def test_a_query_of_nan_spoils_its_own_row_only(prefix):
+    import torch
+    from gtmoe.kvcache import KvAttention, KvCache
+    torch.manual_seed(11)
+    n, H, KV, hd, P = 20, 8, 2, 256, 4096
+    pre, own = KvCache(1, P, KV, hd), KvCache(n, 300, KV, hd)
+    for c in (pre, own):
+        for t in (c.k, c.v):
+            t.copy_(torch.randint(-127, 128, t.shape, device="cuda", dtype=torch.int8))
+        for t in (c.k_scale, c.v_scale):
+            t.fill_(0.004)
+    q = torch.randn(n, H * hd, device="cuda") * 0.1
+    kw = dict(prefix=pre, prefix_len=P) if prefix else {}
+    pos = [(P if prefix else 0) + 10 * i for i in range(n)]
+    op, want, got = KvAttention(H, KV, hd, n), torch.empty_like(q), torch.empty_like(q)
+    op(q, own, list(range(n)), pos, want, **kw)
+    q[7, 2 * hd + 5] = float("nan")
+    op(q, own, list(range(n)), pos, got, **kw)
+    want, got = (t.view(n, H, hd) for t in (want, got))
+    assert got[7, 2].isnan().all()
+    got[7, 2] = want[7, 2]
+    # the stabilisers of the heads beside it may move by other steps: a few roundings of fp32 sums
+    assert float((got - want).abs().max()) <= 1e-5 * float(want.abs().max())

@@ -179,3 +179,22 @@ def test_python_wrappers_check_shapes_and_types():
         s(torch.zeros(2, 11), [RowParams()] * 2)
     with pytest.raises(gtmoe.GtmError):
         s(torch.zeros(2, 10), [RowParams(1.0)] * 2, torch.zeros(2))
+
+
+def test_python_wrappers_refuse_what_a_uint32_would_wrap():
+    import torch
+    from gtmoe.kvcache import KvAttention, KvCache
+    from gtmoe.sampling import RowParams, sampling_rows
+    c, q = KvCache(2, 16, 2, 128, device="cpu"), torch.zeros(1, 512)
+    for args in ((-1, 0, 1), (0, -1, 1), (0, 0, -1), (0, 1 << 32, 1)):
+        with pytest.raises(gtmoe.GtmError, match="2\\^32"):
+            c.read(*args, k_out=torch.zeros(1, 256))
+    with pytest.raises(gtmoe.GtmError, match="rotated_pairs"):
+        c.write(q, q[:, :256], q[:, :256], q, [0], [0], rotated_pairs=-1)
+    att = KvAttention(4, 2, 128, 1, device="cpu")
+    for kw in (dict(window=-1), dict(prefix_len=-1, prefix=c), dict(prefix_seq=1 << 32, prefix=c)):
+        with pytest.raises(gtmoe.GtmError, match="2\\^32"):
+            att(q, c, [0], [0], torch.zeros(1, 512), **kw)
+    for top_k in (-1, 1 << 32):
+        with pytest.raises(gtmoe.GtmError, match="top_k"):
+            sampling_rows([RowParams(1.0, 1.0, 0.0, top_k)])

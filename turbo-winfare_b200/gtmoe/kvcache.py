@@ -27,14 +27,27 @@ def _u32(vals, n: int | None = None):
 
 
 def _raw_stream(stream, device):
-    """The stream to launch on, as an integer: the caller's, or torch's current one on the tensors' device,
-    which has to be the current device."""
+    """The stream to launch on, as an integer: the caller's, or torch's current one, on the tensors' device,
+    which has to be the current device. (Without a GPU the library refuses the call itself.)"""
     import torch
-    if device.type == "cuda" and torch.cuda.current_device() != device.index:
+    if device.type != "cuda":
+        if torch.cuda.is_available():
+            raise GtmError(ERR_INVALID, f"the tensors are on {device}, not on a GPU")
+        return None
+    if torch.cuda.current_device() != device.index:
         raise GtmError(ERR_INVALID, f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
-    if stream is not None:
-        return stream.cuda_stream
-    return torch.cuda.current_stream().cuda_stream if device.type == "cuda" else None
+    if stream is None:
+        return torch.cuda.current_stream().cuda_stream
+    if stream.device_index != device.index:
+        raise GtmError(ERR_INVALID, f"the tensors are on {device}, the stream on cuda:{stream.device_index}")
+    return stream.cuda_stream
+
+
+def _uint(**vals) -> None:
+    """Refuses what would not survive the way into a uint32."""
+    for name, x in vals.items():
+        if not 0 <= x <= 0xFFFFFFFF:
+            raise GtmError(ERR_INVALID, f"{name} {x} is not in [0, 2^32)")
 
 
 def _f32(t, name: str, device, shape=None) -> int:
@@ -112,6 +125,7 @@ class KvCache:
             raise GtmError(ERR_INVALID, f"q must be [n, q_heads * {self.head_dim}], not {tuple(q.shape)}")
         shape, dev, width = q.shape, self.device, self.kv_heads * self.head_dim
         n = shape[0]
+        _uint(rotated_pairs=rotated_pairs)
         qp, qs = _rows(q, "q", dev, n, shape[1])
         kp, ks = _rows(k, "k", dev, n, width)
         vp, vs = _rows(v, "v", dev, n, width)
@@ -125,6 +139,7 @@ class KvCache:
     def read(self, seq: int, first: int, count: int, k_out=None, v_out=None, stream=None):
         """gtm_kv_read: positions [first, first + count) of `seq` as fp32 [count, kv_heads * head_dim];
         (k_out, v_out), allocated where both are None."""
+        _uint(seq=seq, first=first, count=count)
         shape = (count, self.kv_heads * self.head_dim)
         if k_out is None and v_out is None:
             import torch
@@ -152,6 +167,7 @@ class KvAttention:
                  prefix_seq: int = 0, prefix_len: int = 0, stream=None) -> None:
         dev, shape = cache.device, (q.shape[0], self.q_heads * self.head_dim)
         n = shape[0]
+        _uint(window=window, prefix_seq=prefix_seq, prefix_len=prefix_len)
         qp, out = _f32(q, "q", dev, shape), _f32(ctx, "ctx", dev, shape)
         if cache.kv_heads != self.kv_heads or cache.head_dim != self.head_dim or self.device != dev:
             raise GtmError(ERR_INVALID, "the cache's heads or device are not the attention's")

@@ -96,6 +96,9 @@ class RowParams:
 
 def sampling_rows(params):
     """The rows of a call, from RowParams; kept by a caller whose settings do not change."""
+    for p in params:
+        if not 0 <= p.top_k <= 0x7FFFFFFF:
+            raise GtmError(ERR_INVALID, f"top_k {p.top_k} is not in [0, 2^31)")
     return (SamplingRow * max(1, len(params)))(*[SamplingRow(p.temperature, p.top_p, p.min_p, p.top_k) for p in params])
 
 
