@@ -86,6 +86,14 @@ def test_a_step_of_512_rows():
     check(z, [RULES[i % len(RULES)] for i in range(512)], u)
 
 
+@pytest.mark.parametrize("n,V", [(8, 700001), (9, 5000), (9, 70003), (20, 262144), (33, 70000), (40, 262147), (34, 600001), (129, 66001),
+                                 (130, 20000)])
+def test_numbers_of_rows(n, V):
+    """On either side of every change of the CTAs per row."""
+    z, u = rows_of(n, V, n + V)
+    check(z, [RULES[(5 * i + 2) % len(RULES)] for i in range(n)], u)
+
+
 @pytest.mark.parametrize("scale", [1e-5, 1.0, 1e4, 1e30])
 def test_ranges_of_logits(scale):
     r = np.random.default_rng(7)

@@ -1,14 +1,16 @@
 // Sampling a batch's rows (gtm_sample_rows, include/gtmoe_sampling.h).
 //
 // One cluster of CTAs per row: each keeps its share of the row's logits in shared memory (larger
-// vocabularies are read from L2 again), so HBM is read once and every later pass runs on chip, with no
-// workspace and one launch.
+// shares are read from L2 again), so HBM is read once and every later pass runs on chip, with no
+// workspace and one launch. Instructions bound it, ~25 for an id's weight, as many for the counts and the
+// bracket's test, and ten cluster barriers a row: one row of 262,144 ids takes 46 us, 64 rows under mixed
+// rules 162-178, 512 rows 871 (1.7 each); the bytes of 64 are 10.4 us.
 //   1 the largest logit, and its lowest id;
 //   2 the cuts. Ranked by logit, every cut keeps a run from the top, so the kept set is the ids whose
 //     key (logit, then lower id) is at least a border's. Ids are counted per level of max - logit,
 //     1/128 wide where it counts; a level's weights agree within 0.8%, so the counts alone bracket the
 //     nucleus' border to a few levels. One pass sums the exact weights (all of them, and those above the bracket) and
-//     gathers the bracket's ids, among which one CTA finds the border by halves. A bracket of more than 4,096 ids (nearly equal
+//     gathers the bracket's ids, among which one CTA finds the border by halves. A bracket of more than 3,072 ids (nearly equal
 //     logits) is narrowed by its levels' masses and then by the logit's ordered bits instead;
 //   3 the draw: sums of the kept weights per warp's run of ids, CTA and cluster, then one warp finds
 //     the id in the run that the target falls in.
@@ -29,17 +31,16 @@ namespace cg = cooperative_groups;
 namespace gtm {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWarps = kThreads / 32;
 constexpr int kLevels = 2048;
-// Levels of max - logit: 1/128 wide up to 8, then three times as wide; 32 and more is the last.
+// Levels of max - logit: 1/128 wide up to 8 (1,024 of them), then three times as wide; 32 and more is the last.
 constexpr float kFine = 128.0f, kCoarse = 128.0f / 3.0f, kOne = 8388608.0f;   // 2^23: a float's integers from here on
 // The nearest level, in the low bits of a float; monotone in d.
 __device__ __forceinline__ float near_level(float d) {
-    return fminf(fmaf(d, kFine, kOne), fmaf(d, kCoarse, kOne + 2048.0f / 3.0f));
+    return fminf(fmaf(d, kFine, kOne), fmaf(d, kCoarse, kOne + 683.0f));
 }
-__device__ __forceinline__ float level_middle(int level) { return level <= 1024 ? level / kFine : 8.0f + (level - 1024) / kCoarse; }
-constexpr uint32_t kGather = 4096;     // ids of a bracket that are gathered
+__device__ __forceinline__ float level_middle(int level) { return level <= 1024 ? level / kFine : (level - 683) / kCoarse; }
+constexpr uint32_t kGather = 3072;     // ids of a bracket that are gathered
+constexpr uint32_t kHalfIds = 16384;   // or of one that leaves room for a second CTA
 constexpr uint32_t kSmemIds = 40960;   // ids of a share that stay in shared memory
 constexpr int kGroups = 10;            // parts of a warp's run of ids in the draw (128 ids of a share in shared memory)
 
@@ -92,6 +93,7 @@ __device__ __forceinline__ unsigned long long key_of(float x, uint32_t id) {
     return (static_cast<unsigned long long>(ordered(x)) << 32) | static_cast<uint32_t>(~id);
 }
 
+template <int kWarps>
 struct __align__(16) Shared {
     unsigned long long power62[1024];   // 2^(j / 1024) in units of 2^-62
     int power30[1024];                  // and of 2^-30
@@ -137,7 +139,8 @@ __device__ __forceinline__ Scale scale_of(float hi, float lo, float lo2, float t
     c.top_f = __fadd_rn(__fsub_rn(p, n), __fmaf_rn(lo, top, __fmaf_rn(hi, top, -p)));
     return c;
 }
-__device__ __noinline__ unsigned long long exact_exp(const Shared& sh, float x, float top, float hi, float lo, float lo2) {
+template <class Sh>
+__device__ __noinline__ unsigned long long exact_exp(const Sh& sh, float x, float top, float hi, float lo, float lo2) {
     const float d = __fsub_rn(x, top), b = __fsub_rn(d, x);
     if (d == 0.0f) return 1ull << 40;
     const float y = __fmul_rn(d, hi);
@@ -159,7 +162,8 @@ __device__ __noinline__ unsigned long long exact_exp(const Shared& sh, float x, 
     return (w + (1ull << (s - 1))) >> s;
 }
 // The short form where it holds; else `big` is set (x = -infinity, and whatever is below 2^-42, among them).
-__device__ __forceinline__ uint32_t short_exp(const Shared& sh, float x, const Scale& c, bool& big) {
+template <class Sh>
+__device__ __forceinline__ uint32_t short_exp(const Sh& sh, float x, const Scale& c, bool& big) {
     const float t = __fmaf_rn(x, c.hi, 12582912.0f);   // 1.5 * 2^23: the nearest integer in the low bits
     const int k = __float_as_int(t) - 0x4B400000 - c.top_i;
     big = static_cast<uint32_t>(k + 42 * 1024) >= 32u * 1024 || !c.brief;   // a t beyond its range gives a k beyond this one
@@ -173,14 +177,16 @@ __device__ __forceinline__ uint32_t short_exp(const Shared& sh, float x, const S
     const uint32_t w = static_cast<uint32_t>(m + __mulhi(m, p)) >> ((-11 - (k >> 10)) & 31);   // twice the weight
     return big ? 0u : (w + 1) >> 1;
 }
-__device__ __forceinline__ unsigned long long fixed_exp(const Shared& sh, float x, float top, const Scale& c) {
+template <class Sh>
+__device__ __forceinline__ unsigned long long fixed_exp(const Sh& sh, float x, float top, const Scale& c) {
     bool big;
     const uint32_t w = short_exp(sh, x, c, big);
     return big ? exact_exp(sh, x, top, c.hi, c.lo, c.lo2) : w;
 }
 // The weights of four ids, those of `in`: short forms in one straight run (below 2^-10, so four fit 32 bits); the
 // exact ones, which are few, stay behind in `big`.
-__device__ __forceinline__ uint32_t short_four(const Shared& sh, const float (&x)[4], const bool (&in)[4], const Scale& c, uint32_t (&w)[4], uint32_t& big) {
+template <class Sh>
+__device__ __forceinline__ uint32_t short_four(const Sh& sh, const float (&x)[4], const bool (&in)[4], const Scale& c, uint32_t (&w)[4], uint32_t& big) {
     uint32_t sum = 0;
     big = 0;
 #pragma unroll
@@ -219,11 +225,12 @@ __device__ __forceinline__ unsigned long long warp_sum(unsigned long long x) {
     return x;
 }
 
-template <int CL>
-__global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ SampleArgs a, const __grid_constant__ Rows rows) {
+template <int CL, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) smp_rows(const __grid_constant__ SampleArgs a, const __grid_constant__ Rows rows) {
     extern __shared__ __align__(16) unsigned char smem[];
-    Shared& sh = *reinterpret_cast<Shared*>(smem);
-    float* slice_s = reinterpret_cast<float*>(smem + sizeof(Shared));
+    constexpr int kWarps = kThreads / 32;
+    Shared<kWarps>& sh = *reinterpret_cast<Shared<kWarps>*>(smem);
+    float* slice_s = reinterpret_cast<float*>(smem + sizeof(sh));
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = cluster.block_rank(), row = blockIdx.x / CL;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -234,6 +241,10 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
     auto four = [&](uint32_t i) -> float4 {
         if (a.resident) return *reinterpret_cast<const float4*>(slice_s + i);
         float4 x;
+        if (a.vec && i + 3 < n) {
+            x = __ldg(reinterpret_cast<const float4*>(src + base + i));
+            return make_float4(as_logit(x.x), as_logit(x.y), as_logit(x.z), as_logit(x.w));
+        }
         x.x = as_logit(__ldg(src + base + i));
         x.y = i + 1 < n ? as_logit(__ldg(src + base + i + 1)) : -INFINITY;
         x.z = i + 2 < n ? as_logit(__ldg(src + base + i + 2)) : -INFINITY;
@@ -243,8 +254,10 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
     auto logit = [&](uint32_t i) { return a.resident ? slice_s[i] : as_logit(__ldg(src + base + i)); };
 
     // ---- 1: the largest logit and its lowest id
-    sh.power62[tid] = kPowers.v[tid];
-    sh.power30[tid] = static_cast<int>((kPowers.v[tid] + (1ull << 31)) >> 32);
+    for (int i = tid; i < 1024; i += kThreads) {
+        sh.power62[i] = kPowers.v[i];
+        sh.power30[i] = static_cast<int>((kPowers.v[i] + (1ull << 31)) >> 32);
+    }
     if (tid == kThreads - 1) {   // what takes double precision, on one thread beside the loads
         const double c = 1477.3197218702985291 / static_cast<double>(rule.temperature);   // 1024 log2(e)
         const float hi = static_cast<float>(c), lo = static_cast<float>(c - hi);
@@ -261,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
         if (x > most) most = x, most_id = base + i;
         return x;
     };
-    if (a.resident && a.vec) {
+    if (a.vec) {
         constexpr int U = 8;   // loads in flight per thread
         for (uint32_t i0 = tid * 4; i0 < n4; i0 += kThreads * 4 * U) {
             float4 x[U];
@@ -280,7 +293,9 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const uint32_t i = i0 + u * kThreads * 4;
-                if (i < n) *reinterpret_cast<float4*>(slice_s + i) = make_float4(look(i, x[u].x), look(i + 1, x[u].y), look(i + 2, x[u].z), look(i + 3, x[u].w));
+                if (i >= n) continue;
+                const float4 y = make_float4(look(i, x[u].x), look(i + 1, x[u].y), look(i + 2, x[u].z), look(i + 3, x[u].w));
+                if (a.resident) *reinterpret_cast<float4*>(slice_s + i) = y;
             }
         }
     } else {
@@ -299,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
     if (lane == 0) sh.warp_mass[warp] = best;
     __syncthreads();
     if (warp == 0) {
-        best = sh.warp_mass[lane];
+        best = lane < kWarps ? sh.warp_mass[lane] : 0;
         for (int o = 16; o > 0; o >>= 1) {
             const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
             best = other > best ? other : best;
@@ -307,10 +322,9 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
         if (lane == 0) sh.cta_key = best;
     }
     cluster.sync();
-    best = 0;
-#pragma unroll
-    for (int r = 0; r < CL; ++r) {
-        const unsigned long long other = *cluster.map_shared_rank(&sh.cta_key, r);
+    best = lane < CL ? *cluster.map_shared_rank(&sh.cta_key, lane) : 0;   // a CTA's value per lane, here and below
+    for (int o = 16; o > 0; o >>= 1) {
+        const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
         best = other > best ? other : best;
     }
     const float top = from_ordered(static_cast<uint32_t>(best >> 32));
@@ -363,18 +377,28 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
         uint32_t c = 0;
         const int mine = rank * kPart + tid;
         if (tid < kPart)
+#pragma unroll 8
             for (int r = 0; r < CL; ++r) c += *cluster.map_shared_rank(&sh.count[mine], r);
         cluster.sync();
         if (tid < kPart)
+#pragma unroll 8
             for (int r = 0; r < CL; ++r) *cluster.map_shared_rank(&sh.count[mine], r) = c;
         cluster.sync();
-        // two levels per thread: counts, and the mass down to and including each, near enough
-        static_assert(kLevels == 2 * kThreads, "");
-        const uint32_t c0 = sh.count[2 * tid], c1 = sh.count[2 * tid + 1];
-        const float e0 = c0 * expf(-level_middle(2 * tid)), e1 = c1 * expf(-level_middle(2 * tid + 1));
-        uint32_t pc = c0 + c1;
-        float pe = e0 + e1, var = (c0 && !(tid == 0 && c0 == 1) ? e0 * e0 / c0 : 0.0f) + (c1 ? e1 * e1 / c1 : 0.0f);   // a lone largest id weighs 1
-        if (tid >= kThreads / 2) var *= 9.0f;
+        // a few levels per thread: counts, and the mass down to and including each, near enough
+        constexpr int kEach = kLevels / kThreads;
+        uint32_t cnt[kEach], pc = 0;
+        float near_mass[kEach], pe = 0.0f, var = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const int i = kEach * tid + j;
+            const uint32_t k = sh.count[i];
+            const float e = k * expf(-level_middle(i)), wide = i > 1024 ? 9.0f : 1.0f;
+            if (k && !(i == 0 && k == 1)) var += wide * e * e / k;   // a lone largest id weighs 1
+            pc += k, pe += e;
+            cnt[j] = pc, near_mass[j] = pe;   // from the thread's first level on
+        }
+        const uint32_t own_c = pc;
+        const float own_e = pe;
         for (int o = 16; o > 0; o >>= 1) var += __shfl_xor_sync(0xffffffffu, var, o);
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t uc = __shfl_up_sync(0xffffffffu, pc, o);
@@ -383,36 +407,36 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
         }
         if (lane == 31) sh.warp_count[warp] = pc, sh.warp_near[warp] = pe, sh.warp_var[warp] = var;
         __syncthreads();
-        uint32_t bc = 0;
-        float be = 0.0f, all = 0.0f;
+        uint32_t bc = pc - own_c;
+        float be = pe - own_e, all = 0.0f;
         var = 0.0f;
         for (int w = 0; w < kWarps; ++w) {
             if (w < warp) bc += sh.warp_count[w], be += sh.warp_near[w];
             all += sh.warp_near[w], var += sh.warp_var[w];
         }
-        const uint32_t cum1 = bc + pc, cum0 = cum1 - c1;
-        if (cut_p) {
-            // an id's weight is off by up to 1/256 of itself, evenly spread in a level: 3.5 standard deviations of the
-            // sum (and 2^-13 of it for the rest) to either side, mostly a level or two
-            const float slack = 3.5f * (1.0f / 256.0f) * 0.57735f * sqrtf(var) + all * 0x1p-13f;
-            const float m1 = be + pe, m0 = be + (pe - e1), low = rule.top_p * all - slack, high = rule.top_p * all + slack;
-            if (c0 && m0 >= low) atomicMin(&sh.first, 2 * tid);
-            if (c1 && m1 >= low) atomicMin(&sh.first, 2 * tid + 1);
-            if (c0 && m0 >= high) atomicMin(&sh.last, 2 * tid);
-            if (c1 && m1 >= high) atomicMin(&sh.last, 2 * tid + 1);
-        }
-        if (cut_k) {
-            if (c0 && cum0 >= static_cast<uint32_t>(rule.top_k)) atomicMin(&sh.by_count, 2 * tid);
-            if (c1 && cum1 >= static_cast<uint32_t>(rule.top_k)) atomicMin(&sh.by_count, 2 * tid + 1);
+        // an id's weight is off by up to 1/256 of itself, evenly spread in a level: 3.5 standard deviations of the
+        // sum (and 2^-13 of it for the rest) to either side, mostly a level or two
+        const float slack = 3.5f * (1.0f / 256.0f) * 0.57735f * sqrtf(var) + all * 0x1p-13f;
+        const float low = rule.top_p * all - slack, high = rule.top_p * all + slack;
+#pragma unroll
+        for (int j = kEach - 1; j >= 0; --j) {
+            if (cnt[j] == (j ? cnt[j - 1] : 0u)) continue;   // no ids
+            const int i = kEach * tid + j;
+            const float m = be + near_mass[j];
+            if (cut_p && m >= low) atomicMin(&sh.first, i);
+            if (cut_p && m >= high) atomicMin(&sh.last, i);
+            if (cut_k && bc + cnt[j] >= static_cast<uint32_t>(rule.top_k)) atomicMin(&sh.by_count, i);
         }
         __syncthreads();
         first = cut_p ? min(min(sh.first, sh.by_count), kLevels - 1u) : sh.by_count;
         last = cut_p ? min(min(sh.last, sh.by_count), kLevels - 1u) : sh.by_count;
-        // ids above the bracket, and ids in it
-        if (2 * tid == first) sh.pick_count = cum0 - c0;
-        if (2 * tid + 1 == first) sh.pick_count = cum1 - c1;
-        if (2 * tid == last) sh.members = cum0;
-        if (2 * tid + 1 == last) sh.members = cum1;
+        // ids above the bracket, and ids down to its end
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const uint32_t i = kEach * tid + j;
+            if (i == first) sh.pick_count = bc + (j ? cnt[j - 1] : 0u);
+            if (i == last) sh.members = bc + cnt[j];
+        }
         __syncthreads();
     }
     const bool bracket = first < kLevels;   // else every id is kept
@@ -464,14 +488,12 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
         if (lane == 0) sh.warp_mass[warp] = sum, sh.warp_mass2[warp] = up;
         __syncthreads();
         if (warp == 0) {
-            sum = warp_sum(sh.warp_mass[lane]), up = warp_sum(sh.warp_mass2[lane]);
+            sum = warp_sum(lane < kWarps ? sh.warp_mass[lane] : 0ull), up = warp_sum(lane < kWarps ? sh.warp_mass2[lane] : 0ull);
             if (lane == 0) sh.cta_mass = sum, sh.cta_mass2 = up;
         }
         cluster.sync();
-        for (int r = 0; r < CL; ++r) {
-            whole += *cluster.map_shared_rank(&sh.cta_mass, r);
-            above_mass += *cluster.map_shared_rank(&sh.cta_mass2, r);
-        }
+        whole = warp_sum(lane < CL ? *cluster.map_shared_rank(&sh.cta_mass, lane) : 0ull);
+        above_mass = warp_sum(lane < CL ? *cluster.map_shared_rank(&sh.cta_mass2, lane) : 0ull);
     }
     uint32_t border_level = kLevels, ties = 0xFFFFFFFFu;
     unsigned long long need = 0;
@@ -488,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
         }
         cluster.sync();
         if (rank == 0) {
-            // four ids per thread; the border is the largest key with which those from it on reach a cut: halves of
+            // a few ids per thread; the border is the largest key with which those from it on reach a cut: halves of
             // the range [lo, hi) that holds it, until one id is left
             if (tid == 0) sh.border_key = 0, sh.key_lo = ~0ull, sh.key_hi = 0;
             __syncthreads();
@@ -506,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
             }
             __syncthreads();
             unsigned long long lo = sh.key_lo, hi = sh.key_hi + 1;
-            // ids from `from` on, and their mass (24 and 17 bits apart: 4,096 weights of 2^40 at most)
+            // ids from `from` on, and their mass (24 and 17 bits apart: 3,072 weights of 2^40 at most)
             int turn = 0;
             auto down_to = [&](unsigned long long from, uint32_t& count) {
                 uint32_t c = 0, wl = 0, wh = 0;
@@ -516,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
                 c = __reduce_add_sync(0xffffffffu, c), wl = __reduce_add_sync(0xffffffffu, wl), wh = __reduce_add_sync(0xffffffffu, wh);
                 if (lane == 0) sh.half[turn][warp] = make_uint3(c, wl, wh);
                 __syncthreads();
-                const uint3 v = sh.half[turn][lane];
+                const uint3 v = lane < kWarps ? sh.half[turn][lane] : make_uint3(0, 0, 0);
                 turn ^= 1;
                 count = __reduce_add_sync(0xffffffffu, v.x);
                 const unsigned long long l = __reduce_add_sync(0xffffffffu, v.y & 0xFFFFu), h = __reduce_add_sync(0xffffffffu, v.y >> 16);
@@ -563,6 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
                 const uint32_t lev = i + lane;
                 unsigned long long own = 0;
                 if (cut_p && lev <= last)
+#pragma unroll 2
                     for (int r = 0; r < CL; ++r) own += *cluster.map_shared_rank(&sh.mass[lev - first], r);
                 uint32_t own_c = lev <= last ? sh.count[lev] : 0, pc = own_c;
                 unsigned long long pm = own;
@@ -607,12 +630,14 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
                 uint32_t c = 0;
                 const int mine = rank * kPart + tid;
                 if (tid < kPart)
+#pragma unroll 2
                     for (int r = 0; r < CL; ++r) {
                         m += *cluster.map_shared_rank(&sh.mass[mine], r);
                         c += *cluster.map_shared_rank(&sh.count[mine], r);
                     }
                 cluster.sync();
                 if (tid < kPart)
+#pragma unroll 2
                     for (int r = 0; r < CL; ++r) {
                         *cluster.map_shared_rank(&sh.mass[mine], r) = m;
                         *cluster.map_shared_rank(&sh.count[mine], r) = c;
@@ -759,20 +784,16 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
         if (lane == 0) sh.warp_mass[warp] = sum, sh.warp_count[warp] = count;
         __syncthreads();
         if (warp == 0) {
-            const unsigned long long s = warp_sum(sh.warp_mass[lane]);
-            uint32_t c = sh.warp_count[lane];
+            const unsigned long long s = warp_sum(lane < kWarps ? sh.warp_mass[lane] : 0ull);
+            uint32_t c = lane < kWarps ? sh.warp_count[lane] : 0u;
             for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
             if (lane == 0) sh.draw_mass = s, sh.draw_count = c;
         }
         cluster.sync();
-        unsigned long long all = 0, before = 0;
-        uint32_t kept = 0;
-        for (uint32_t r = 0; r < CL; ++r) {
-            const unsigned long long s = *cluster.map_shared_rank(&sh.draw_mass, r);
-            if (r < rank) before += s;
-            all += s;
-            kept += *cluster.map_shared_rank(&sh.draw_count, r);
-        }
+        const unsigned long long of_lane = lane < CL ? *cluster.map_shared_rank(&sh.draw_mass, lane) : 0ull;
+        const unsigned long long all = warp_sum(of_lane);
+        unsigned long long before = warp_sum(lane < rank ? of_lane : 0ull);
+        const uint32_t kept = __reduce_add_sync(0xffffffffu, lane < CL ? *cluster.map_shared_rank(&sh.draw_count, lane) : 0u);
         const double u = a.uniform[row];   // NaN and negative values stand for 0
         const unsigned long long target = !(u > 0.0) ? 0 : u < 1.0 ? min(product_down(u, all), all - 1) : all - 1;
         for (int w = 0; w < warp; ++w) before += sh.warp_mass[w];
@@ -858,24 +879,27 @@ __global__ void __launch_bounds__(kThreads, 1) smp_rows(const __grid_constant__ 
     cluster.sync();   // no CTA leaves while another may read its shared memory
 }
 
-template <int CL>
+template <int CL, int T>
 cudaError_t launch(SampleArgs& a, const Rows& r, uint32_t n, cudaStream_t st) {
+    using Sh = Shared<T / 32>;
+    constexpr uint32_t kMost = T == 1024 ? kSmemIds : kHalfIds;
+    static_assert(T == 1024 || 2 * (sizeof(Sh) + kMost * sizeof(float) + 1024) <= 228 * 1024, "two CTAs on an SM");
     const uint32_t per = (a.vocab + CL - 1) / CL;
     a.slice = (per + 1023) / 1024 * 1024;
-    a.resident = a.slice <= kSmemIds;
-    cudaError_t e = cudaFuncSetAttribute(smp_rows<CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared) + kSmemIds * sizeof(float));
-    if (e == cudaSuccess && CL > 8) e = cudaFuncSetAttribute(smp_rows<CL>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    a.resident = a.slice <= kMost;
+    cudaError_t e = cudaFuncSetAttribute(smp_rows<CL, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Sh) + kMost * sizeof(float));
+    if (e == cudaSuccess && CL > 8) e = cudaFuncSetAttribute(smp_rows<CL, T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(n * CL);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = sizeof(Shared) + (a.resident ? a.slice * sizeof(float) : 0);
+    cfg.blockDim = dim3(T);
+    cfg.dynamicSmemBytes = sizeof(Sh) + (a.resident ? a.slice * sizeof(float) : 0);
     cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = CL, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
     cfg.attrs = &attr, cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, smp_rows<CL>, a, r);
+    return cudaLaunchKernelEx(&cfg, smp_rows<CL, T>, a, r);
 }
 
 }  // namespace
@@ -916,10 +940,16 @@ extern "C" GTM_API int gtm_sample_rows(const float* logits, uint32_t n, uint32_t
     a.token = token, a.kept = kept, a.logprob = logprob;
     a.vocab = vocab;
     a.vec = aligned(logits, 16) && (n == 1 || row_stride % 4 == 0);
-    // Sixteen CTAs a row while they all fit the SMs at once (one row of 262,144 ids: 45 us against 54 with
-    // eight); beyond that eight, whose rows finish in fewer rounds (64 rows: 240 us against 340).
+    // Few rows are a matter of latency: sixteen CTAs a row, or eight, keep every SM at work (262,144 ids: 8 rows
+    // 75 us, 12 rows 69 with eight of 1,024 threads against 90 of 512). Many rows are one of throughput: CTAs of
+    // 512 threads, two on an SM, so that one's barriers pass behind the other's work, and as few a row as take
+    // their share into shared memory (four against eight: 64 rows of 32,000 ids 54 against 68 us, of 262,144 198
+    // against 195), or fewer still where the rows alone fill the GPU (512 of 262,144 ids: 871 against 1,027).
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = n <= 8 ? launch<16>(a, r, n, st) : launch<8>(a, r, n, st);
+    const cudaError_t e = n <= 8                                ? launch<16, 1024>(a, r, n, st)
+                          : vocab <= 4 * kHalfIds || n > 128 ? launch<4, 512>(a, r, n, st)
+                          : n <= 32                             ? launch<8, 1024>(a, r, n, st)
+                                                                : launch<8, 512>(a, r, n, st);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return set_cuda_error(fn, e);
