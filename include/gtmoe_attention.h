@@ -105,7 +105,8 @@ typedef struct GtmKvCache {
 
 /* QKVEpilogue of n rows' queries, keys and values in one launch, keys and values going into the
  * cache: row i (n <= 512, i-th row of q_dev, k_dev and v_dev, whose rows are *_stride floats
- * apart) belongs to sequence seqs[i] at positions[i] (HOST arrays, as in the *_rows entries).
+ * apart) belongs to sequence seqs[i] at positions[i] (HOST arrays, as in the *_rows entries: read
+ * during the call, so a captured launch keeps the values it was captured with).
  *   q: RMS norm per head with weight q_w_dev (bf16, NULL = none), rotation -> q_out_dev
  *      [n][q_heads * head_dim] (q_out_dev may be q_dev where q_stride is q_heads * head_dim)
  *   k: RMS norm with k_w_dev, rotation -> cache;   v: RMS norm without a weight -> cache
@@ -124,7 +125,9 @@ GTM_API int gtm_qkv_cache_rows(const GtmKvCache* cache, uint32_t q_heads, uint32
 GTM_API int gtm_kv_read(const GtmKvCache* cache, uint32_t seq, uint32_t first, uint32_t count, float* k_out_dev,
                         float* v_out_dev, void* stream);
 /* Workspace of gtm_attention_kv_rows for at most n rows (0 for unsupported shapes); no
- * initialisation. A workspace serves one stream at a time. */
+ * initialisation. It depends on the current device's number of SMs (a B200's where there is no
+ * device). A workspace serves one stream at a time; two captured graphs may share one if their
+ * replays do not overlap. */
 GTM_API size_t gtm_attention_kv_workspace_bytes(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t n);
 /* Attention of n rows (n <= 512) at positions[i] of sequences seqs[i] (HOST arrays): row i attends
  * [first, positions[i]] with first = max(0, positions[i] + 1 - window) (window 0 = all), scores
@@ -135,7 +138,9 @@ GTM_API size_t gtm_attention_kv_workspace_bytes(uint32_t q_heads, uint32_t kv_he
  * sequence's own cache as the prefix, with prefix_len one past the last row's position.
  * `prefix` has the cache's format, kv_heads and head_dim. A row's span must fit the rings: its
  * own positions within capacity, and prefix_len - first within the prefix's. q_heads a multiple of
- * kv_heads, at most 8 query heads per kv head. q_dev and ctx_dev [n][q_heads * head_dim]. */
+ * kv_heads, at most 8 query heads per kv head. q_dev and ctx_dev [n][q_heads * head_dim], |q| below
+ * 2^100. Infinities, NaN and whatever else the rings hold outside a row's span do not reach it. The
+ * waits on the device are bounded: should one run out (1 s), the rows that it served are NaN. */
 GTM_API int gtm_attention_kv_rows(const GtmKvCache* cache, const GtmKvCache* prefix, uint32_t prefix_seq,
                                   uint32_t prefix_len, uint32_t q_heads, uint32_t n, uint32_t window,
                                   const float* q_dev, const uint32_t* seqs, const uint32_t* positions, float* ctx_dev,
