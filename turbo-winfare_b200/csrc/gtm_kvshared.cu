@@ -30,7 +30,7 @@
 // (512 dims), twice that for O: ~6,000 cycles a tile of 512 dims. A tile takes ~10,000: the hand-overs of
 // K, V, S and p each add a wait, and no role is busy throughout (without any one of conversions, softmax or
 // half the products it took 5 to 20% less). 512 rows (16 / 2 heads of 512) over 32,768 positions: 1.49 ms;
-// 32 rows over 16,384: 78-85 us; 61 windowed rows (8 heads of 256): 18-20 us.
+// 32 rows over 16,384: 71 us; 61 windowed rows (8 heads of 256): 18-20 us.
 // kLongest: 16 tiles 1.63 ms and 5.3e-6 of relative error, 20 1.49 and 6.1e-6, 24 1.47 and 7.0e-6.
 //
 // Roles: warps 0-7 softmax and O (32 of the 64 columns each half of them); 8-11 K; 12-15 V; 16 issues
@@ -78,7 +78,7 @@ struct SharedArgs {
     const float *ks, *vs;          // [kv_heads][capacity]
     const float* q;
     uint32_t q_heads, kv_heads, n, grp, capacity, ring_tiles, window, prefix_len, total;
-    uint32_t lo[kMaxUnitsPerHead], first[kMaxUnitsPerHead];   // a unit's first position and its ring tile
+    uint32_t lo[kMaxUnitsPerHead], first[kMaxUnitsPerHead], tiles[kMaxUnitsPerHead];   // a unit's first position, its ring tile, and its tiles
     SharedPlan plan;
 };
 
@@ -128,6 +128,7 @@ __device__ __forceinline__ void widen(const uint4& w, uint32_t (&o)[8]) {
 
 struct Segment {
     uint32_t kvh, unit, tile, tiles, slot;
+    uint32_t left;   // places of the list until the next one
 };
 __device__ __forceinline__ Segment segment_at(const SharedArgs& a, uint32_t g, uint32_t end) {
     Segment s;
@@ -139,7 +140,9 @@ __device__ __forceinline__ Segment segment_at(const SharedArgs& a, uint32_t g, u
         if (u + step < a.plan.units && a.plan.start[u + step] <= r) u += step;
     s.unit = u;
     s.tile = r - a.plan.start[u];
-    s.tiles = min(min(a.plan.start[u + 1] - r, end - g), kLongest);
+    s.left = min(a.plan.start[u + 1] - r, end - g);
+    s.tiles = min(min(s.left, a.tiles[u] - s.tile), kLongest);
+    if (s.tile + s.tiles < a.tiles[u]) s.left = s.tiles;   // else what fills up the unit's last run goes, too
     s.slot = blockIdx.x + s.kvh * a.plan.units + u;
     return s;
 }
@@ -260,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t *rlo_c = rlo + col0, *rhi_c = rhi + col0;
         for (uint32_t g = g0; g < g1;) {
             const Segment sg = segment_at(a, g, g1);
-            g += sg.tiles;
+            g += sg.left;
             if (!begin(sg)) {
                 done_slot = sg.slot;
                 continue;
@@ -457,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     for (uint32_t g = g0; g < g1;) {
         const Segment sg = segment_at(a, g, g1);
-        g += sg.tiles;
+        g += sg.left;
         const bool good = begin(sg);
         done_slot = sg.slot;
         if (!good) continue;
@@ -656,12 +659,29 @@ size_t shared_slots(uint32_t q_heads, uint32_t kv_heads, uint32_t n, int num_sms
     return units + num_sms;
 }
 
+// The list of tiles is cut into runs of `per`, one for each CTA. A run that touches two units pays for it: q, the
+// first tile's way through every role, the drain and the result, ~20 us together at 512 dims, as much as three or
+// four tiles. So each unit's tiles are filled up to whole runs where that makes runs at most three tiles longer
+// (32 rows over 16,384 positions, 2 heads of 512: 7 tiles a run and 88 us, or 8 and 71).
 void plan_shared(const SharedCall& c, const RowU32& pos, int num_sms, SharedPlan& plan) {
     plan.units = (c.n * (c.q_heads / c.kv_heads) + N - 1) / N;
+    uint32_t tiles[kMaxUnitsPerHead];
+    uint64_t total = 0;
+    for (uint32_t u = 0; u < plan.units; ++u) total += tiles[u] = unit_span(c, pos, u).tiles;
+    total *= c.kv_heads;
+    const uint32_t flat = static_cast<uint32_t>(std::max<uint64_t>(1, (total + num_sms - 1) / num_sms));
+    uint32_t fill = 1;
+    plan.per = flat;
+    for (uint32_t per = flat; per <= flat + 3; ++per) {
+        uint64_t runs = 0;
+        for (uint32_t u = 0; u < plan.units; ++u) runs += (tiles[u] + per - 1) / per;
+        if (runs * c.kv_heads <= static_cast<uint64_t>(num_sms)) {
+            plan.per = fill = per;
+            break;
+        }
+    }
     plan.start[0] = 0;
-    for (uint32_t u = 0; u < plan.units; ++u) plan.start[u + 1] = plan.start[u] + unit_span(c, pos, u).tiles;
-    const uint32_t total = plan.start[plan.units] * c.kv_heads;
-    plan.per = std::max(1u, (total + num_sms - 1) / num_sms);
+    for (uint32_t u = 0; u < plan.units; ++u) plan.start[u + 1] = plan.start[u] + (tiles[u] + fill - 1) / fill * fill;
 }
 
 int launch_shared(const SharedCall& c, const RowU32& pos, const SharedPlan& plan, int num_sms, cudaStream_t st) {
@@ -682,7 +702,7 @@ int launch_shared(const SharedCall& c, const RowU32& pos, const SharedPlan& plan
     a.total = plan.start[plan.units] * c.kv_heads;
     for (uint32_t u = 0; u < plan.units; ++u) {
         const UnitSpan s = unit_span(c, pos, u);
-        a.lo[u] = s.lo, a.first[u] = s.first;
+        a.lo[u] = s.lo, a.first[u] = s.first, a.tiles[u] = s.tiles;
     }
     a.plan = plan;
     const uint32_t ctas = (a.total + plan.per - 1) / plan.per;
