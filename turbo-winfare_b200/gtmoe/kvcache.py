@@ -23,7 +23,8 @@ def _u32(vals, n: int | None = None):
         vals = np.ascontiguousarray(vals, dtype=np.uint32)
     if n is not None and vals.size != n:
         raise GtmError(ERR_INVALID, f"{vals.size} positions or sequence indices for {n} rows")
-    return vals.ctypes.data, vals
+    # the address by the shortest way (a few tenths of a microsecond), which takes writable arrays with elements only
+    return C.addressof(C.c_char.from_buffer(vals)) if vals.size and vals.flags.writeable else vals.ctypes.data, vals
 
 
 def _raw_stream(stream, device):
@@ -37,7 +38,7 @@ def _raw_stream(stream, device):
     if torch.cuda.current_device() != device.index:
         raise GtmError(ERR_INVALID, f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
     if stream is None:
-        return torch.cuda.current_stream().cuda_stream
+        return torch._C._cuda_getCurrentRawStream(device.index)   # current_stream() makes an object: 3 us more a call
     if stream.device_index != device.index:
         raise GtmError(ERR_INVALID, f"the tensors are on {device}, the stream on cuda:{stream.device_index}")
     return stream.cuda_stream
