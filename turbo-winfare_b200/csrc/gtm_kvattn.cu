@@ -57,6 +57,24 @@ struct RowsShape {
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" :: "r"(id), "r"(threads) : "memory"); }
 
+// The second and third kernel of a call are set up while the one before ends (1.5 to 3 us less each), and start
+// here, with all its results in sight. None is let in earlier: kv_combine's CTAs took room from kv_rows' last ones
+// (32 own rows 105.5 -> 107.6 us), and kv_rows beside kv_shared gained on one shape (107.7 -> 101.4) and lost on
+// another (93.2 -> 96.3).
+__device__ __forceinline__ void wait_for_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <class... P, class... Q>
+cudaError_t launch_after(bool early, void (*kernel)(P...), dim3 grid, int threads, cudaStream_t st, const Q&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr, cfg.numAttrs = early ? 1 : 0;   // only behind a kernel of the same call
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // A tile's two products are made by two kinds of warps, so that both run at once: the first half of the
 // CTA scores 16 positions a warp (A = K: 16 positions x 16 dims; B = q: 16 dims x 8 heads), agrees on
 // the heads' maxima and leaves the weights in one of two buffers; the second half adds all of the tile's
@@ -122,6 +140,7 @@ __global__ void __launch_bounds__(RowsShape<HD>::kThreads, HD == 512 ? 1 : 2)
         sc = make_float2(__ldg((p ? a.pre.ks : a.own.ks) + at), __ldg((p ? a.pre.vs : a.own.vs) + at));
     };
 
+    wait_for_kernel_before();
     float2 sc_next = make_float2(0.0f, 0.0f);
     write_places(0, sc_next);
     if (tid < T) sc_s[0][tid] = sc_next;
@@ -333,11 +352,12 @@ __global__ void __launch_bounds__(RowsShape<HD>::kThreads, HD == 512 ? 1 : 2)
 }
 
 // One CTA per (query head, row): the row's partial results merged, its own items' and the shared part's. Latency
-// is all: two dependent rounds of loads, 6 to 10 us behind the other kernels. A factor per thread and eight
+// is all: two dependent rounds of loads, 5 to 9 us behind the other kernels. A factor per thread and eight
 // results in flight, for long lists, gained nothing (6.6 against 5.9 us for one row, 10.3 against 9 for 32).
 template <int HD>
 __global__ void __launch_bounds__(HD / 4) kv_combine(const __grid_constant__ RowsArgs a, const __grid_constant__ Starts starts,
                                                      const __grid_constant__ RowU32 pos, const __grid_constant__ SharedPlan sh) {
+    wait_for_kernel_before();
     const uint32_t head = blockIdx.x, row = blockIdx.y;
     const uint32_t first = starts.v[row], items = starts.v[row + 1] - first;
     const Span sp = row_span(pos.v[row], a.window, a.prefix_len);
@@ -407,13 +427,16 @@ int launch_rows(RowsArgs& a, Starts& starts, const RowU32& pos, const RowU32& se
     const uint32_t items = starts.v[a.n];
     a.ml = reinterpret_cast<float2*>(a.part + static_cast<size_t>(items) * a.q_heads * HD);
     const dim3 grid(items, a.kv_heads);
-    if (items) {
-        if (fmt == GTM_KV_INT8)
-            kv_rows<HD, GTM_KV_INT8><<<grid, S::kThreads, 0, st>>>(a, starts, pos, seq);
-        else
-            kv_rows<HD, GTM_KV_E4M3><<<grid, S::kThreads, 0, st>>>(a, starts, pos, seq);
+    const bool shared = !a.list_prefix && sh.start[sh.units];
+    cudaError_t e = cudaSuccess;
+    if (items)
+        e = launch_after(shared, fmt == GTM_KV_INT8 ? kv_rows<HD, GTM_KV_INT8> : kv_rows<HD, GTM_KV_E4M3>, grid, S::kThreads, st, a, starts, pos, seq);
+    if (e == cudaSuccess && merge)
+        e = launch_after(items || shared, kv_combine<HD>, dim3(a.q_heads, a.n), HD / 4, st, a, starts, pos, sh);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return set_cuda_error("gtm_attention_kv_rows", e);
     }
-    if (merge) kv_combine<HD><<<dim3(a.q_heads, a.n), HD / 4, 0, st>>>(a, starts, pos, sh);
     return GTM_OK;
 }
 
