@@ -10,7 +10,7 @@
 //     key (logit, then lower id) is at least a border's. Ids are counted per level of max - logit,
 //     1/128 wide where it counts; a level's weights agree within 0.8%, so the counts alone bracket the
 //     nucleus' border to a few levels. One pass sums the exact weights (all of them, and those above the bracket) and
-//     gathers the bracket's ids, among which one CTA finds the border by halves. A bracket of more than 3,072 ids (nearly equal
+//     gathers the bracket's ids, among which one CTA finds the border by halves. A bracket of more than 3,200 ids (nearly equal
 //     logits) is narrowed by its levels' masses and then by the logit's ordered bits instead;
 //   3 the draw: sums of the kept weights per warp's run of ids, CTA and cluster, then one warp finds
 //     the id in the run that the target falls in.
@@ -39,7 +39,7 @@ __device__ __forceinline__ float near_level(float d) {
     return fminf(fmaf(d, kFine, kOne), fmaf(d, kCoarse, kOne + 683.0f));
 }
 __device__ __forceinline__ float level_middle(int level) { return level <= 1024 ? level / kFine : (level - 683) / kCoarse; }
-constexpr uint32_t kGather = 3072;     // ids of a bracket that are gathered
+constexpr uint32_t kGather = 3200;     // ids of a bracket that are gathered
 constexpr uint32_t kHalfIds = 16384;   // or of one that leaves room for a second CTA
 constexpr uint32_t kSmemIds = 40960;   // ids of a share that stay in shared memory
 constexpr int kGroups = 10;            // parts of a warp's run of ids in the draw (128 ids of a share in shared memory)
@@ -514,7 +514,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) smp_rows(const __gr
             // the range [lo, hi) that holds it, until one id is left
             if (tid == 0) sh.border_key = 0, sh.key_lo = ~0ull, sh.key_hi = 0;
             __syncthreads();
-            constexpr int kMine = kGather / kThreads;
+            constexpr int kMine = (kGather + kThreads - 1) / kThreads;
+            static_assert(kMine < 8, "a warp's sums of 24-bit parts stay within 32 bits");
             unsigned long long key[kMine], w[kMine];
 #pragma unroll
             for (int j = 0; j < kMine; ++j) {
@@ -528,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) smp_rows(const __gr
             }
             __syncthreads();
             unsigned long long lo = sh.key_lo, hi = sh.key_hi + 1;
-            // ids from `from` on, and their mass (24 and 17 bits apart: 3,072 weights of 2^40 at most)
+            // ids from `from` on, and their mass (24 and 17 bits apart: 3,200 weights of 2^40 at most)
             int turn = 0;
             auto down_to = [&](unsigned long long from, uint32_t& count) {
                 uint32_t c = 0, wl = 0, wh = 0;
