@@ -303,6 +303,7 @@ def test_attention(case, fmt):
 # Prefixes long enough, over the rows together, to be computed once for all (98,304 positions x kv heads)
 SHARED = [  # as above
     (3, 8, 8, 128, 0, 5000, 5000, [1, 2, 3]),
+    (2, 8, 8, 128, 0, 7000, 7000, [1, 2]),
     (40, 16, 8, 256, 0, 400, 400, list(range(1, 121, 3))),
     (64, 16, 2, 512, 0, 1000, 1000, [1 + (i * 5) % 70 for i in range(64)]),
     (33, 8, 1, 128, 0, 3100, 4000, [5] * 33),                           # ring larger than the prefix
@@ -338,6 +339,22 @@ def test_attention_rows_inside_a_prefix_and_beyond():
     fill(cache, 31)
     fill(prefix, 32)
     check_attention(cache, queries(4, 16, 256), [0, 1, 2, 3], [0, 44, 89, 129], 0, prefix, 0, 90)
+
+
+@pytest.mark.parametrize("fmt,hd,H,KV,rise", [("int8", 128, 8, 1, 1.0), ("int8", 128, 8, 1, 2.0), ("e4m3", 256, 8, 1, 2.0), ("int8", 512, 8, 1, 2.0)])
+def test_attention_over_a_prefix_of_many_tiles(fmt, hd, H, KV, rise):
+    """More tiles for a CTA than are summed in one go; with `rise` the later keys' scores pass all before them."""
+    from gtmoe.kvcache import KvCache
+    n, P = 512, 8000
+    cache, prefix = KvCache(n, 2, KV, hd, fmt), KvCache(1, P, KV, hd, fmt)
+    fill(cache, 21)
+    fill(prefix, 22)
+    prefix.k_scale[..., P // 2:] *= rise
+    q, some = queries(n, H, hd), list(range(0, n, 37))
+    got = run_attention(cache, q, list(range(n)), [P] * n, 0, prefix, 0, P).cpu().numpy().astype(np.float64)[some]
+    want, tol = attend(q.cpu().numpy().astype(np.float64)[some], cache, some, [P] * len(some), 0, prefix, 0, P)
+    assert (np.abs(got - want).max(1) <= tol).all()
+    assert np.linalg.norm(got - want) <= 2e-5 * rise * np.linalg.norm(want)   # as above, of S ~ 40 rise
 
 
 @pytest.mark.parametrize("spread", [1e3, 1e-3])

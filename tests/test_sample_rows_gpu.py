@@ -86,7 +86,7 @@ def test_a_step_of_512_rows():
     check(z, [RULES[i % len(RULES)] for i in range(512)], u)
 
 
-@pytest.mark.parametrize("n,V", [(8, 700001), (9, 5000), (9, 70003), (20, 262144), (33, 70000), (40, 262147), (34, 600001), (129, 66001),
+@pytest.mark.parametrize("n,V", [(8, 700001), (9, 5000), (9, 70003), (20, 262144), (33, 70000), (40, 262147), (34, 600001), (129, 66001), (40, 262144), (130, 131072),
                                  (130, 20000)])
 def test_numbers_of_rows(n, V):
     """On either side of every change of the CTAs per row."""

@@ -390,12 +390,13 @@ __global__ void __launch_bounds__(HD / 4) kv_combine(const __grid_constant__ Row
         make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
 }
 
-// Prefix positions x kv heads over all rows from which the prefix is computed once for all (three rows or
-// more). kv_shared costs 8 (128 dims) to 25 us (512) however little it does; kv_rows reads the prefix again
-// for every row at 3.3-4.3 TB/s. Whole calls, once for all against row by row, int8: 16 rows x 2,048
-// positions x 2 heads of 512 (65,536) 44 against 42 us, 32 rows (131,072) 46 against 57, 32 rows x 16,384
-// 104 against 261; 4 rows x 2,048 x 8 heads of 256 (65,536) 32 against 28, 16 rows (262,144) 33 against 50,
-// 32 rows x 16,384 66 against 497; 2 rows x 16,384 x 8 heads of 256 (262,144) 59 against 52.
+// Prefix positions x kv heads over all rows from which the prefix is computed once for all (two rows or more).
+// kv_shared costs 10 (128 dims) to 25 us (512) however little it does; kv_rows reads the prefix again for every
+// row at 3.3-4.3 TB/s. Whole calls, once for all against row by row, int8: 2 heads of 512, 16 rows x 2,048
+// positions (65,536) 40 against 40 us, 32 rows (131,072) 42 against 56, 32 rows x 16,384 83 against 259; 8 heads of
+// 256, 4 rows x 2,048 (65,536) 27 against 23, 8 rows (131,072) 27 against 27, 32 rows x 512 (131,072) 26 against 30,
+// 2 rows x 16,384 (262,144) 46 against 48; 8 heads of 128, 8 rows x 2,048 (131,072) 23 against 21, 16 rows 24
+// against 33.
 constexpr uint64_t kSharedFrom = 98304;
 
 // Items of all rows are at most n plus this (a chunk is at least the total / target).
@@ -538,7 +539,7 @@ GTM_API int gtm_attention_kv_rows(const GtmKvCache* c, const GtmKvCache* prefix,
     SharedPlan plan;
     plan.units = 0;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    a.list_prefix = n < 3 || in_prefix * c->kv_heads < kSharedFrom;
+    a.list_prefix = n < 2 || in_prefix * c->kv_heads < kSharedFrom;
     if (!a.list_prefix) {
         const SharedCall call{prefix, prefix_seq, prefix_len, q_heads, c->kv_heads, c->head_dim, n, window, q};
         plan_shared(call, pos, sms, plan);
