@@ -133,7 +133,7 @@ GTM_API size_t gtm_attention_kv_workspace_bytes(uint32_t q_heads, uint32_t kv_he
  * [first, positions[i]] with first = max(0, positions[i] + 1 - window) (window 0 = all), scores
  * q.k with scale 1.0, softmax, weighted V into ctx_dev row i. Positions below prefix_len are read
  * from sequence prefix_seq of `prefix` (row t % its capacity), the others from sequence seqs[i] of
- * `cache`; the prefix's tiles are read and multiplied once for all rows. prefix_len 0: no prefix
+ * `cache`; a prefix long enough is read and multiplied once for all rows. prefix_len 0: no prefix
  * (`prefix` may be NULL). Rows of one sequence's prompt are attended causally by giving that
  * sequence's own cache as the prefix, with prefix_len one past the last row's position.
  * `prefix` has the cache's format, kv_heads and head_dim. A row's span must fit the rings: its

@@ -84,9 +84,9 @@ cudaError_t launch_after(bool early, void (*kernel)(P...), dim3 grid, int thread
 //
 // Bytes are the floor (a code is read once per row and kv head, for at most 8 heads' products), but the
 // chain of a tile bounds it: load, widening and products, a barrier among the scorers, exponentials, the
-// hand-over, the sums. 32 rows of 77-8,192 positions, 2 heads of 512 (275 MB): 91 us, 3.0 TB/s, with one CTA
+// hand-over, the sums. 32 rows of 77-8,192 positions, 2 heads of 512 (275 MB): 85 us, 3.2 TB/s, with one CTA
 // of 16 warps per SM; 61 windowed rows, 8 heads of 256, two of 8 warps: 55 us; one row of 1,024: 4.3. All warps
-// scoring and then summing took 99 and 64 us; then neither leaving out the products nor codes that stay in L2
+// scoring and then summing took 99 and 64 us (91 and 55 since, with the same runs); then neither leaving out the products nor codes that stay in L2
 // made it faster.
 template <int HD, int FMT>
 __global__ void __launch_bounds__(RowsShape<HD>::kThreads, HD == 512 ? 1 : 2)
@@ -399,12 +399,12 @@ __global__ void __launch_bounds__(HD / 4) kv_combine(const __grid_constant__ Row
 // against 33.
 constexpr uint64_t kSharedFrom = 98304;
 
-// Items of all rows are at most n plus this (a chunk is at least the total / target).
+// Items of all rows are at most n plus this (a run is at least the total / target).
 constexpr uint32_t kTargetCtas = 592;
 uint32_t target_items(uint32_t kv_heads) { return std::max(1u, kTargetCtas / kv_heads); }
 
 template <int HD>
-int launch_rows(RowsArgs& a, Starts& starts, const RowU32& pos, const RowU32& seq, const SharedPlan& sh, uint32_t fmt, cudaStream_t st) {
+int launch_rows(RowsArgs& a, Starts& starts, const RowU32& pos, const RowU32& seq, const SharedPlan& sh, uint32_t fmt, int num_sms, cudaStream_t st) {
     using S = RowsShape<HD>;
     uint64_t sum = 0;
     uint32_t len[kMaxBatchRows];
@@ -416,9 +416,26 @@ int launch_rows(RowsArgs& a, Starts& starts, const RowU32& pos, const RowU32& se
         sum += len[i];
     }
     const uint64_t want = (sum + target_items(a.kv_heads) - 1) / target_items(a.kv_heads);
-    const uint64_t chunk = std::max<uint64_t>(1, (want + S::kTile - 1) / S::kTile) * S::kTile;
-    if (chunk > 0x7FFFFFFFull) return set_error(GTM_ERR_UNSUPPORTED, "gtm_attention_kv_rows: %llu positions", (unsigned long long)sum);
-    a.chunk = static_cast<uint32_t>(chunk);
+    const uint64_t least = std::max<uint64_t>(1, (want + S::kTile - 1) / S::kTile);   // tiles of a run, for the workspace
+    if (least * S::kTile > 0x7FFFFFFFull) return set_error(GTM_ERR_UNSUPPORTED, "gtm_attention_kv_rows: %llu positions", (unsigned long long)sum);
+    // Runs up to twice as long, or four tiles longer, where that makes the rounds of CTAs x (tiles + 1 for a run's
+    // start) fewer by a sixteenth: 32 rows of 77-8,192 positions, 2 heads of 512: 4 tiles, four rounds 106 us, 5
+    // tiles, three rounds 99; 3 rows of 1,000-8,000 36 -> 25. Below that short runs even out better (up to 3%). For
+    // many rows the search would cost the host more than it gives.
+    uint64_t tiles = least;
+    if (a.n <= 128) {
+        const uint64_t slots = static_cast<uint64_t>(num_sms) * (HD == 512 ? 1 : 2);
+        uint64_t best = 0;
+        for (uint64_t t = least; t <= least + std::min<uint64_t>(std::max<uint64_t>(least, 4), 8); ++t) {
+            const uint32_t run = static_cast<uint32_t>(t * S::kTile);
+            uint64_t runs = 0;
+            for (uint32_t i = 0; i < a.n; ++i) runs += (len[i] + run - 1) / run;
+            const uint64_t cost = (runs * a.kv_heads + slots - 1) / slots * (t + 1);
+            if (t == least) best = cost * 15 / 16 + 1;   // what another has to stay below
+            else if (cost < best) best = cost, tiles = t;
+        }
+    }
+    a.chunk = static_cast<uint32_t>(tiles * S::kTile);
     starts.v[0] = 0;
     for (uint32_t i = 0; i < a.n; ++i) {
         const uint32_t items = (len[i] + a.chunk - 1) / a.chunk;
@@ -550,11 +567,11 @@ GTM_API int gtm_attention_kv_rows(const GtmKvCache* c, const GtmKvCache* prefix,
     }
     Starts starts;
     if (c->head_dim == 128)
-        rc = launch_rows<128>(a, starts, pos, seq, plan, c->format, st);
+        rc = launch_rows<128>(a, starts, pos, seq, plan, c->format, sms, st);
     else if (c->head_dim == 256)
-        rc = launch_rows<256>(a, starts, pos, seq, plan, c->format, st);
+        rc = launch_rows<256>(a, starts, pos, seq, plan, c->format, sms, st);
     else
-        rc = launch_rows<512>(a, starts, pos, seq, plan, c->format, st);
+        rc = launch_rows<512>(a, starts, pos, seq, plan, c->format, sms, st);
     if (rc) return rc;
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return set_cuda_error(fn, e);

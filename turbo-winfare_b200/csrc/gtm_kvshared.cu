@@ -31,7 +31,8 @@
 // K, V, S and p each add a wait, and no role is busy throughout (without any one of conversions, softmax or
 // half the products it took 5 to 20% less). 512 rows (16 / 2 heads of 512) over 32,768 positions: 1.49 ms;
 // 32 rows over 16,384: 71 us; 61 windowed rows (8 heads of 256): 18-20 us.
-// kLongest: 16 tiles 1.63 ms and 5.3e-6 of relative error, 20 1.49 and 6.1e-6, 24 1.47 and 7.0e-6.
+// kLongest: 16 tiles 1.63 ms and 5.3e-6 of relative error, 24 1.52 and 7.0e-6, 32 1.52 and 8.7e-6 (before results
+// were added to memory without reading them back); now 20, 1.49 and 6.1e-6.
 //
 // Roles: warps 0-7 softmax and O (32 of the 64 columns each half of them); 8-11 K; 12-15 V; 16 issues
 // S, 17 O; 18 and 19 load the codes of K and V. Every wait is bounded (1 s); one that runs out stops the
