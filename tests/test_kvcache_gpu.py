@@ -589,3 +589,35 @@ def test_a_query_of_nan_spoils_its_own_row_only(prefix):
     got[7, 2] = want[7, 2]
     # the stabilisers of the heads beside it may move by other steps: a few roundings of fp32 sums
     assert float((got - want).abs().max()) <= 1e-5 * float(want.abs().max())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("hd", [128, 256, 512])
+def test_a_shared_prefix_whose_scores_rise_with_every_tile(hd, fmt):
+    """Each tile of 128 keys scores 9 more (base 2) than the one before, so that the sums so far are rescaled at
+    every tile of a CTA's run, while the products of the next wait: equal bits in every repeat, and the formula's
+    values. A key has one value only, so a row's scores are q[0] * k[0], S the largest of them."""
+    import torch
+    from gtmoe.kvcache import KvAttention, KvCache
+    n, H, P = 512, 8, 3000
+    cache, prefix = KvCache(n, 2, 1, hd, fmt), KvCache(1, P, 1, hd, fmt)
+    fill(cache, 91)
+    fill(prefix, 92)
+    for c in (cache, prefix):
+        c.k.view(torch.uint8).zero_()
+        c.k.view(torch.uint8)[..., 0] = 1 if fmt == "int8" else 0x38   # 1.0
+    step = 9 * np.log(2.0)
+    t = torch.arange(P, device="cuda")
+    prefix.k_scale[0, 0] = ((t // 128) * step + (t % 128) * (step / 256) + 1e-3).float()
+    cache.k_scale.fill_(float(P // 128 * step))
+    q = queries(n, H, hd)
+    q.view(n, H, hd)[..., 0] = torch.linspace(1.0, 1.05, n * H, device="cuda").view(n, H)
+    some, pos = list(range(0, n, 37)), [P] * n
+    want, tol = attend(q.cpu().numpy().astype(np.float64)[some], cache, some, [P] * len(some), 0, prefix, 0, P)
+    op, first = KvAttention(H, 1, hd, n), None
+    for _ in range(30):
+        got = run_attention(cache, q, list(range(n)), pos, 0, prefix, 0, P, op=op)
+        first = got if first is None else first
+        assert torch.equal(got, first)
+    off = np.abs(first.cpu().numpy().astype(np.float64)[some] - want).max(1)
+    assert (off <= tol).all(), (off / tol).max()

@@ -360,6 +360,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         tc::tmem_st_wait();
                         tc::tc_fence_before();
+                        // Each warp has rescaled its own 32 of O's 128 lanes, but p_full[0], which lets a product
+                        // into all of them, is the arrival of two of the group's warps only: none goes on before
+                        // all four are done.
+                        tc::named_bar_sync(bar, 128);
                     }
                 }
                 ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&p_empty[half], (x & 1) ^ 1, abort_flag, kWaitNs));
