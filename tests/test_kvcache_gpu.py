@@ -621,3 +621,47 @@ def test_a_shared_prefix_whose_scores_rise_with_every_tile(hd, fmt):
         assert torch.equal(got, first)
     off = np.abs(first.cpu().numpy().astype(np.float64)[some] - want).max(1)
     assert (off <= tol).all(), (off / tol).max()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("hd,shared", [(128, False), (512, False), (128, True), (512, True)])
+def test_a_long_tail_of_small_weights_counts(hd, shared, fmt):
+    """One key 18.4 ahead of thousands of others, whose weights of 10^-8 each (2^-26.5 of the largest) together make
+    the second half of the output's dims: the first key's value is 0 there. Relative to that tail a result is off
+    by 2 (ds + 2^-20), as above, with S = 18.4: 2.9e-4; and by the rounding of the weights, which are all alike: a weight
+    p is held in two fp16 limbs, hi + lo, so within half of fp16's smallest step, 2^-25, where the largest is
+    at least 2^15.9 / 2^8 (over a shared prefix: the stabiliser stays while weights grow by up to 2^8) or 2^15.9. The
+    tail's are e^-18.4 of that: 1.2e-2 of them, or 4.8e-5."""
+    import torch
+    from gtmoe.kvcache import KvCache
+    n, H, KV, T = (512, 8, 1, 8192) if shared else (64, 8, 8, 4096)
+    c = KvCache(1, T, KV, hd, fmt)
+    one, top = (1, 127) if fmt == "int8" else (0x38, 0x7E)   # 1.0, and the largest code
+    k, v = c.k.view(torch.uint8), c.v.view(torch.uint8)
+    k[:, 0, :, 0] = one
+    v[:, 0, :, :hd // 2] = top
+    v[:, 1:, :, hd // 2:] = top
+    c.k_scale.fill_(18.4)
+    c.v_scale.fill_(0.01)
+    q = torch.zeros(n, H, hd, device="cuda")
+    q[..., 0] = 1.0
+    q, pos, some = q.view(n, -1), [T - 1 - i % 7 for i in range(n)], [0, 1, n - 1]
+    kw = dict(prefix=c, pseq=0, plen=T) if shared else {}
+    got = run_attention(c, q, [0] * n, pos, **kw).cpu().numpy().astype(np.float64)[some]
+    want, _ = attend(q.cpu().numpy().astype(np.float64)[some], c, [0] * 3, [pos[i] for i in some], 0, c, 0, T if shared else 0)
+    got, want = (x.reshape(3, H, hd)[..., hd // 2:] for x in (got, want))
+    off = float(np.abs(got / want - 1).max())
+    held = 2.0 ** -25 / (2.0 ** (7.9 if shared else 15.9) * np.exp(-18.4))
+    assert (want > 0).all() and off <= 2 * (64 * 2.0 ** -23 * 18.4 + 2.0 ** -20) + held, off
+
+
+@pytest.mark.parametrize("many", [1, 40, 400])
+def test_values_of_zero_beside_others(many):
+    """Vectors of zeros have the least scale, 2^-100: their weights still count in the softmax's sum."""
+    from gtmoe.kvcache import KvCache
+    cache, prefix = KvCache(1, 40, 2, 128), KvCache(1, 2000, 2, 128)
+    fill(cache, 95)
+    fill(prefix, 96)
+    prefix.v.zero_()
+    prefix.v_scale.fill_(2.0 ** -100)
+    check_attention(cache, queries(many, 8, 128), [0] * many, [2000 + i % 40 for i in range(many)], 0, prefix, 0, 2000)

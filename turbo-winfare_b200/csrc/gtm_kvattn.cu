@@ -7,8 +7,8 @@
 // scales stay outside: a score is multiplied by its position's ks, a weight by its vs.
 //
 // Running softmax in base 2 per query head: with s2 = log2(e) * q.k the stabiliser is m >= max(s2 +
-// log2 vs), so a carried weight p = exp2(s2 - m) * vs is at most about 1 whatever the scales are
-// (fp16 keeps 2^-25 of the largest one), while l = sum of exp2(s2 - m) and the weighted sum O stay
+// log2 vs) - 15.9, so a carried weight p = exp2(s2 - m) * vs fits fp16 whatever the scales are
+// (its limbs are off by up to 2^-40.9 of the largest one), while l = sum of exp2(s2 - m) and the weighted sum O stay
 // in fp32. Masked positions take a weight of exactly 0 by selection, so nothing that a ring row
 // outside a row's span holds reaches a sum. A partial result (m, l, O) is merged by kv_combine.
 //
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(RowsShape<HD>::kThreads, HD == 512 ? 1 : 2)
                 const float2 sc = sc_s[buf][p];
                 valid[r] = j0 + t * T + p < j1;
                 vs[r] = sc.y;
-                const float lg = log2f(fmaxf(sc.y, kKvTiny));
+                const float lg = log2_vs(sc.y) - kWeightTop;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     s[2 * r + h] = valid[r] ? s[2 * r + h] * sc.x * qs[h] : -INFINITY;

@@ -33,6 +33,15 @@ __host__ __device__ __forceinline__ Span row_span(uint32_t pos, uint32_t window,
     return s;
 }
 
+// A carried weight p = exp2(s2 - m) * vs is at most 2^kWeightTop (61,148), which fp16 (65,504) has room for. Its two
+// limbs are off by up to 2^-25 whatever p is, so the top is put as high as it goes: a weight is off by up to 2^-40.9 of
+// the largest one (2^-32.9 in kv_shared, whose m may stay while weights grow). With the largest at 1, keys whose scores
+// were 18 below it (2^-26) were lost, however many they were.
+constexpr float kWeightTop = 15.9f;
+// log2 vs as the stabiliser takes it: from 2^-88 on, so that exp2(s2 - m) <= 2^(16 + 88), and 2^23 of them sum up in
+// fp32. Values of smaller scales (2^-100 is the least) still have p up to 2^3.
+__device__ __forceinline__ float log2_vs(float vs) { return log2f(fmaxf(vs, 3.2311742677852644e-27f)); }
+
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

@@ -54,6 +54,9 @@ constexpr int TP = 128;              // positions of a tile
 constexpr int kThreads = 640;
 constexpr uint64_t kWaitNs = 1000000000ull;
 constexpr int KA = 4;                // K chunks (64 dims) in tensor memory
+// log2 of how far a weight may grow before m moves. Smaller would hold small weights better and move m more often:
+// 512 rows over 32,768 positions 1.51 ms with 8, 1.53 with 6, 1.59 with 4; 32 rows over 16,384 72, 74 and 76 us.
+constexpr float kSlack = 8.0f;
 constexpr uint32_t kLongest = 20;    // tiles summed in tensor memory before the result goes to memory
 
 template <int HD>
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool ok = true;
             for (uint32_t t = 0; t < sg.tiles; ++t) {
                 const uint32_t x = ti + t;
-                const float ks = ks_next, vs = vs_next, lg = log2f(fmaxf(vs, kKvTiny));
+                const float ks = ks_next, vs = vs_next, lg = log2_vs(vs) - (kWeightTop - kSlack);
                 const bool in_ring = slot < a.capacity;
                 const uint32_t at = slot - s0 + (slot < s0 ? a.capacity : 0u);   // from the unit's first position
                 if (t + 1 < sg.tiles) {
@@ -294,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // the group's warps meet in barriers below, so they leave together or not at all
                 if (any_of_128(bar, !ok)) { ok = false; break; }
                 tc::tc_fence_after();
-                float s[H], over = -INFINITY;   // s2, -infinity where masked; whether a weight would pass 2^8
+                float s[H], over = -INFINITY;   // s2, -infinity where masked; whether a weight would pass the top
 #pragma unroll
                 for (int c0 = 0; c0 < H; c0 += 16) {
                     uint32_t v[16], w[16];
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const float4 m4 = *reinterpret_cast<const float4*>(m_c + c);
                     over = fmaxf(over, fmaxf(fmaxf(s[c] - m4.x, s[c + 1] - m4.y), fmaxf(s[c + 2] - m4.z, s[c + 3] - m4.w)));
                 }
-                const bool raise = any_of_128(bar, over + lg > 8.0f);
+                const bool raise = any_of_128(bar, over + lg > kSlack);
                 if (raise) {
                     // new maxima: 15 exchanges and one more leave a column's maximum over the warp's positions
                     // with two lanes
