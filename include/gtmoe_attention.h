@@ -124,8 +124,9 @@ GTM_API int gtm_qkv_cache_rows(const GtmKvCache* cache, uint32_t q_heads, uint32
  * [count][kv_heads * head_dim] (either may be NULL); count <= capacity. */
 GTM_API int gtm_kv_read(const GtmKvCache* cache, uint32_t seq, uint32_t first, uint32_t count, float* k_out_dev,
                         float* v_out_dev, void* stream);
-/* Workspace of gtm_attention_kv_rows for at most n rows (0 for unsupported shapes); no
- * initialisation. It depends on the current device's number of SMs (a B200's where there is no
+/* Workspace of gtm_attention_kv_rows for at most n rows (0 for unsupported shapes). Its first 4
+ * bytes are an error word: zero them once before the first use where gtm_attention_kv_check is to
+ * be called; the rest needs no initialisation. It depends on the current device's number of SMs (a B200's where there is no
  * device). A workspace serves one stream at a time; two captured graphs may share one if their
  * replays do not overlap. */
 GTM_API size_t gtm_attention_kv_workspace_bytes(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t n);
@@ -140,11 +141,21 @@ GTM_API size_t gtm_attention_kv_workspace_bytes(uint32_t q_heads, uint32_t kv_he
  * own positions within capacity, and prefix_len - first within the prefix's. q_heads a multiple of
  * kv_heads, at most 8 query heads per kv head. q_dev and ctx_dev [n][q_heads * head_dim], |q| below
  * 2^100. Infinities, NaN and whatever else the rings hold outside a row's span do not reach it. The
- * waits on the device are bounded: should one run out (1 s), the rows that it served are NaN. */
+ * waits on the device are bounded: should one run out (1 s), the rows that it served are NaN, and
+ * the next gtm_attention_kv_check on the workspace says so. */
 GTM_API int gtm_attention_kv_rows(const GtmKvCache* cache, const GtmKvCache* prefix, uint32_t prefix_seq,
                                   uint32_t prefix_len, uint32_t q_heads, uint32_t n, uint32_t window,
                                   const float* q_dev, const uint32_t* seqs, const uint32_t* positions, float* ctx_dev,
                                   void* workspace_dev, size_t workspace_bytes, void* stream);
+/* Reads back and clears a workspace's error word after gtm_attention_kv_rows calls (synchronises
+ * `stream`). Returns GTM_OK or GTM_ERR_TIMEOUT. */
+GTM_API int gtm_attention_kv_check(void* workspace_dev, void* stream);
+/* Test hook for the bounded waits: in the calling thread's next gtm_attention_kv_rows, where the
+ * prefix is computed once for all rows, one warp of every CTA first waits for an arrival that never
+ * comes, under a 2 ms limit instead of 1 s; it gives up, the other roles leave through the CTA's
+ * abort flag, copies in flight are waited for and tensor memory is freed. Rows with positions in the
+ * prefix are NaN, gtm_attention_kv_check reports GTM_ERR_TIMEOUT, and the workspace stays usable. */
+GTM_API int gtm_attention_kv_test_wait(void);
 
 #ifdef __cplusplus
 }

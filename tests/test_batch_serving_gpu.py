@@ -112,3 +112,16 @@ def test_refusals(model):
         bd.greedy([[1, 2, 3]], 8)
     with pytest.raises(ValueError, match="settings"):
         bd.sample([[1]], 2, [RowParams(), RowParams()])
+
+
+def test_a_wait_that_ran_out_in_attention_ends_the_generation(model):
+    import gtmoe
+    import torch
+    bd = decoder(model, "int8")
+    bd.set_prefix(PREFIX)
+    for call in (lambda: bd.greedy(TAILS, 2, stops=()), lambda: bd.set_prefix(PREFIX)):
+        next(iter(bd.kv_ops.values())).workspace[:4].view(torch.int32).fill_(2)   # as a kernel leaves it
+        with pytest.raises(gtmoe.GtmError, match="timed out"):
+            call()
+    bd.set_prefix(PREFIX)
+    assert len(bd.greedy(TAILS, 2, stops=())[0]) == 2

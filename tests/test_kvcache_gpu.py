@@ -665,3 +665,38 @@ def test_values_of_zero_beside_others(many):
     prefix.v.zero_()
     prefix.v_scale.fill_(2.0 ** -100)
     check_attention(cache, queries(many, 8, 128), [0] * many, [2000 + i % 40 for i in range(many)], 0, prefix, 0, 2000)
+
+
+@pytest.mark.parametrize("fmt,hd,H,KV", [("int8", 256, 16, 8), ("e4m3", 512, 16, 2), ("int8", 128, 8, 2)])
+def test_a_wait_over_the_prefix_runs_out_then_workspace_recovers(fmt, hd, H, KV):
+    """gtm_attention_kv_test_wait: a wait of 2 ms that nothing ends. The call returns, check() reports it once, the rows
+    that attend the prefix are NaN, those past it are right, and the same workspace then gives what it gave before."""
+    import time
+
+    import gtmoe
+    import torch
+    from gtmoe.kvcache import KvAttention, KvCache
+    n, P, window = 64, 6000, 5000
+    cache, prefix = KvCache(n, window, KV, hd, fmt), KvCache(1, P, KV, hd, fmt)
+    for c in (cache, prefix):
+        c.k.view(torch.uint8).random_(0, 120)
+        c.v.view(torch.uint8).random_(0, 120)
+        c.k_scale.uniform_(1e-4, 2e-4)
+        c.v_scale.uniform_(1e-4, 2e-4)
+    op, q, seqs = KvAttention(H, KV, hd, n), queries(n, H, hd), list(range(n))
+    pos = [P + (10 + i if i % 4 else window + i) for i in range(n)]   # every fourth window is past the prefix
+    kw = dict(window=window, prefix=prefix, plen=P, op=op)
+    want = run_attention(cache, q, seqs, pos, **kw)
+    op.check()
+    assert torch.isfinite(want).all()
+    torch.cuda.synchronize()
+    t0 = time.perf_counter()
+    gtmoe.check(gtmoe.lib().gtm_attention_kv_test_wait())
+    got = run_attention(cache, q, seqs, pos, **kw)
+    with pytest.raises(gtmoe.GtmError, match="timed out") as e:
+        op.check()
+    assert e.value.status == gtmoe.ERR_TIMEOUT and time.perf_counter() - t0 < 1.0
+    op.check()   # the failing check cleared the error word
+    assert torch.isnan(got[[i for i in range(n) if i % 4]]).all() and torch.equal(got[::4], want[::4])
+    assert torch.equal(run_attention(cache, q, seqs, pos, **kw), want)
+    op.check()

@@ -198,3 +198,7 @@ def test_python_wrappers_refuse_what_a_uint32_would_wrap():
     for top_k in (-1, 1 << 32):
         with pytest.raises(gtmoe.GtmError, match="top_k"):
             sampling_rows([RowParams(1.0, 1.0, 0.0, top_k)])
+
+
+def test_check_needs_a_workspace():
+    assert gtmoe.lib().gtm_attention_kv_check(None, None) == gtmoe.ERR_INVALID and "workspace" in gtmoe.last_error()

@@ -462,6 +462,10 @@ bool heads_ok(uint32_t q_heads, uint32_t kv_heads) {
     return kv_heads > 0 && q_heads > 0 && q_heads <= 65535u && q_heads % kv_heads == 0 && q_heads / kv_heads <= kKvMaxGroup;
 }
 
+// The workspace: the error word, the rows' partial results, the shared part's.
+constexpr size_t kErrBytes = 256;
+thread_local bool t_test_wait = false;   // gtm_attention_kv_test_wait
+
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 // rows' items: sum of ceil(len / chunk) <= n + sum / chunk <= n + target
 size_t rows_bytes(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t n) {
@@ -495,7 +499,7 @@ GTM_API size_t gtm_attention_kv_workspace_bytes(uint32_t q_heads, uint32_t kv_he
         return 0;
     int sms = 0;
     if (num_sms(&sms) != cudaSuccess) return 0;
-    return rows_bytes(q_heads, kv_heads, head_dim, n) + shared_bytes(q_heads, kv_heads, head_dim, n, sms);
+    return kErrBytes + rows_bytes(q_heads, kv_heads, head_dim, n) + shared_bytes(q_heads, kv_heads, head_dim, n, sms);
 }
 
 GTM_API int gtm_attention_kv_rows(const GtmKvCache* c, const GtmKvCache* prefix, uint32_t prefix_seq, uint32_t prefix_len,
@@ -547,7 +551,7 @@ GTM_API int gtm_attention_kv_rows(const GtmKvCache* c, const GtmKvCache* prefix,
     a.pre = prefix_len ? side(prefix, prefix_seq) : a.own;
     a.q = q;
     a.ctx = ctx;
-    a.part = static_cast<float*>(ws);
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kErrBytes);
     a.q_heads = q_heads, a.kv_heads = c->kv_heads, a.n = n;
     a.window = window, a.prefix_len = prefix_len;
     int sms = 0;
@@ -556,11 +560,13 @@ GTM_API int gtm_attention_kv_rows(const GtmKvCache* c, const GtmKvCache* prefix,
     SharedPlan plan;
     plan.units = 0;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool test_wait = t_test_wait;
+    t_test_wait = false;
     a.list_prefix = n < 2 || in_prefix * c->kv_heads < kSharedFrom;
     if (!a.list_prefix) {
-        const SharedCall call{prefix, prefix_seq, prefix_len, q_heads, c->kv_heads, c->head_dim, n, window, q};
+        const SharedCall call{prefix, prefix_seq, prefix_len, q_heads, c->kv_heads, c->head_dim, n, window, q, static_cast<int*>(ws), test_wait};
         plan_shared(call, pos, sms, plan);
-        plan.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + rows_bytes(q_heads, c->kv_heads, c->head_dim, n));
+        plan.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kErrBytes + rows_bytes(q_heads, c->kv_heads, c->head_dim, n));
         plan.ml = reinterpret_cast<float2*>(plan.part + shared_slots(q_heads, c->kv_heads, n, sms) * kSharedRows * c->head_dim);
         if (plan.start[plan.units]) rc = launch_shared(call, pos, plan, sms, st);
         if (rc) return rc;
@@ -575,6 +581,29 @@ GTM_API int gtm_attention_kv_rows(const GtmKvCache* c, const GtmKvCache* prefix,
     if (rc) return rc;
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return set_cuda_error(fn, e);
+    clear_error();
+    return GTM_OK;
+}
+
+GTM_API int gtm_attention_kv_check(void* ws, void* stream) {
+    const char* fn = "gtm_attention_kv_check";
+    if (!ws) return set_error(GTM_ERR_INVALID, "%s: null workspace", fn);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int flag = 0;
+    cudaError_t e = cudaMemcpyAsync(&flag, ws, sizeof(int), cudaMemcpyDeviceToHost, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e == cudaSuccess && flag) {
+        e = cudaMemsetAsync(ws, 0, sizeof(int), st);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    }
+    if (e != cudaSuccess) return set_cuda_error(fn, e);
+    if (flag) return set_error(GTM_ERR_TIMEOUT, "gtm_attention_kv_rows: a pipeline wait over the prefix timed out (flag %d)", flag);
+    clear_error();
+    return GTM_OK;
+}
+
+GTM_API int gtm_attention_kv_test_wait(void) {
+    t_test_wait = true;
     clear_error();
     return GTM_OK;
 }

@@ -97,6 +97,8 @@ struct SharedCall {
     const GtmKvCache* prefix;
     uint32_t prefix_seq, prefix_len, q_heads, kv_heads, head_dim, n, window;
     const float* q;
+    int* err;          // the workspace's error word
+    bool test_wait;    // gtm_attention_kv_test_wait
 };
 void plan_shared(const SharedCall& c, const RowU32& pos, int num_sms, SharedPlan& plan);
 int launch_shared(const SharedCall& c, const RowU32& pos, const SharedPlan& plan, int num_sms, cudaStream_t st);

@@ -36,7 +36,7 @@
 //
 // Roles: warps 0-7 softmax and O (32 of the 64 columns each half of them); 8-11 K; 12-15 V; 16 issues
 // S, 17 O; 18 and 19 load the codes of K and V. Every wait is bounded (1 s); one that runs out stops the
-// CTA and marks its results NaN.
+// CTA, marks its results NaN and is recorded in the workspace's error word.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -52,7 +52,7 @@ namespace {
 constexpr int N = kSharedRows;
 constexpr int TP = 128;              // positions of a tile
 constexpr int kThreads = 640;
-constexpr uint64_t kWaitNs = 1000000000ull;
+constexpr uint64_t kWaitNs = 1000000000ull, kTestWaitNs = 2000000ull;
 constexpr int KA = 4;                // K chunks (64 dims) in tensor memory
 // log2 of how far a weight may grow before m moves. Smaller would hold small weights better and move m more often:
 // 512 rows over 32,768 positions 1.51 ms with 8, 1.53 with 6, 1.59 with 4; 32 rows over 16,384 72, 74 and 76 us.
@@ -65,7 +65,7 @@ struct Shape {
     static constexpr int kVStages = HD / 64;     // V stages of a tile: 128 dims x 64 positions
     static constexpr int RK = HD == 512 ? 2 : 4, RV = HD == 512 ? 2 : 4, VST = HD == 512 ? 2 : 4;
     static constexpr int kQ = 2 * kChunks * 8192, kP = 2 * 16384, kV = VST * 16384, kRawK = RK * 8192, kRawV = RV * 8192;
-    static constexpr int kBars = 2 * RK + 2 * RV + 2 * KA + 2 * VST + 2 + 4;
+    static constexpr int kBars = 2 * RK + 2 * RV + 2 * KA + 2 * VST + 2 + 4 + 1;
     static constexpr int kSmall = (4 * N + 4 * N + 2 * N) * 4 + kBars * 8 + 16;
     static constexpr int kSmem = kQ + kP + kV + kRawK + kRawV + kSmall;
     // tensor memory columns. An MMA of N <= 128 takes the time of N = 128, so a limb pair goes in one
@@ -84,6 +84,8 @@ struct SharedArgs {
     uint32_t q_heads, kv_heads, n, grp, capacity, ring_tiles, window, prefix_len, total;
     uint32_t lo[kMaxUnitsPerHead], first[kMaxUnitsPerHead], tiles[kMaxUnitsPerHead];   // a unit's first position, its ring tile, and its tiles
     SharedPlan plan;
+    int* err;
+    int test_wait;   // warp 16's first wait is for an arrival that never comes, under kTestWaitNs
 };
 
 // Whether any of a softmax group's 128 threads says so (hardware barrier 1 or 2).
@@ -173,7 +175,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t *rk_full = bars, *rk_empty = rk_full + RK, *rv_full = rk_empty + RK, *rv_empty = rv_full + RV,
              *ka_full = rv_empty + RV, *ka_empty = ka_full + KA, *v_full = ka_empty + KA, *v_empty = v_full + VST,
              *s_full = v_empty + VST, *s_empty = s_full + 1, *p_full = s_empty + 1, *p_empty = p_full + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_empty + 2);
+    uint64_t* never_bar = p_empty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(never_bar + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -184,6 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < VST; ++i) tc::mbar_init(&v_full[i], 4), tc::mbar_init(&v_empty[i], 1);
         tc::mbar_init(s_full, 1), tc::mbar_init(s_empty, 8);
         for (int i = 0; i < 2; ++i) tc::mbar_init(&p_full[i], 4), tc::mbar_init(&p_empty[i], 1);   // a half of the positions
+        tc::mbar_init(never_bar, 1);
         *abort_flag = (tc::smem_u32(smem) & 1023u) ? 1 : 0;   // the swizzled layouts need it
         tc::mbar_fence_init();
     }
@@ -543,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             constexpr uint32_t kQk = tc::idesc_f16(128, 2 * N);
             const uint32_t qa = tc::smem_u32(sQ), d = tmem + S::kSCol;
             uint32_t ik = kc;
-            bool ok = true;
+            bool ok = !a.test_wait || kc || __all_sync(0xffffffffu, tc::mbar_wait(never_bar, 0, abort_flag, kTestWaitNs));
             for (uint32_t t = 0; t < sg.tiles && ok; ++t) {
                 if (!__all_sync(0xffffffffu, tc::mbar_wait(s_empty, ((ti + t) & 1) ^ 1, abort_flag, kWaitNs))) break;
 #pragma unroll
@@ -600,6 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc::tc_fence_before();
     __syncthreads();
+    if (tid == 0 && *abort_flag) atomicExch(a.err, 2);
     if (warp == 17) {
         tc::tmem_relinquish();
         tc::tmem_dealloc(tmem, 512);
@@ -713,6 +718,7 @@ int launch_shared(const SharedCall& c, const RowU32& pos, const SharedPlan& plan
         a.lo[u] = s.lo, a.first[u] = s.first, a.tiles[u] = s.tiles;
     }
     a.plan = plan;
+    a.err = c.err, a.test_wait = c.test_wait ? 1 : 0;
     const uint32_t ctas = (a.total + plan.per - 1) / plan.per;
     if (c.head_dim == 128) return launch<128>(a, pos, p->format, ctas, st);
     if (c.head_dim == 256) return launch<256>(a, pos, p->format, ctas, st);

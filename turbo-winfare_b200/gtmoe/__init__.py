@@ -201,6 +201,8 @@ SIGNATURES = {
     "gtm_attention_kv_workspace_bytes": (_SZ, [_U32, _U32, _U32, _U32]),
     "gtm_attention_kv_rows": (_I, [C.POINTER(KvCacheDesc), C.POINTER(KvCacheDesc), _U32, _U32, _U32, _U32, _U32, _P, _P, _P,
                                    _P, _P, _SZ, _P]),
+    "gtm_attention_kv_check": (_I, [_P, _P]),
+    "gtm_attention_kv_test_wait": (_I, []),
     "gtm_sampling_validate": (_I, [C.POINTER(Sampling)]),
     "gtm_sampling_splitmix64": (_U64, [_U64]),
     "gtm_sampling_seed_for": (_U64, [C.POINTER(Sampling), _I]),

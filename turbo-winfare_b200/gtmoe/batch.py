@@ -225,7 +225,14 @@ class BatchDecoder:
         for p in range(0, len(tokens), self.max_seqs):
             part = [int(t) for t in tokens[p:p + self.max_seqs]]
             self.step([0] * len(part), part, list(range(p, p + len(part))), [], prefill=True)
+        self._check()
         self.prefix_len = len(tokens)
+
+    def _check(self) -> None:
+        """Raises where a bounded wait on the device ran out in one of the steps."""
+        self.moe.check()
+        for op in self.kv_ops.values():
+            op.check()
 
     def _all_done(self, done: bool) -> bool:
         if self.dist is None:
@@ -323,7 +330,7 @@ class BatchDecoder:
             if on_step is not None:
                 on_step(step)
             step += 1
-        self.moe.check()
+        self._check()
         return out
 
 

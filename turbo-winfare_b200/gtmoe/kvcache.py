@@ -162,6 +162,7 @@ class KvAttention:
         if n == 0:
             raise GtmError(ERR_UNSUPPORTED, f"attention of {q_heads} / {kv_heads} heads of {head_dim}, {max_rows} rows")
         self.workspace = torch.empty(n, dtype=torch.uint8, device=device)
+        self.workspace[:4].zero_()   # the error word
         self.ws_ptr, self.ws_bytes, self.device = self.workspace.data_ptr(), n, self.workspace.device
 
     def __call__(self, q, cache: KvCache, seqs, positions, ctx, *, window: int = 0, prefix: KvCache | None = None,
@@ -178,3 +179,7 @@ class KvAttention:
         sq, _s = _u32(seqs, n)
         check(lib().gtm_attention_kv_rows(cache._ref, None if prefix is None else prefix._ref, prefix_seq, prefix_len, self.q_heads, n,
                                           window, qp, sq, pos, out, self.ws_ptr, self.ws_bytes, _raw_stream(stream, dev)))
+
+    def check(self, stream=None) -> None:
+        """gtm_attention_kv_check: raises GtmError (ERR_TIMEOUT) where a wait of an earlier call ran out."""
+        check(lib().gtm_attention_kv_check(self.ws_ptr, _raw_stream(stream, self.device)))
