@@ -190,3 +190,20 @@ def test_greedy_needs_no_uniforms_and_graphs_replay():
     g.replay()
     torch.cuda.synchronize()
     assert s.tokens.cpu().tolist() == [one_row(z2[i], *RULES[1 + i], u2[i])[0] for i in range(4)]
+
+
+@pytest.mark.parametrize("top", [0.0, 25.0, 2000.0, -2000.0])
+def test_weights_around_half_a_unit(top):
+    """41 ln 2 = 28.419 below the largest a weight is half of 2^-40: up to there it is one unit, beyond it 0. At u = 0 the
+    token is the lowest id with a weight. Logits of 2,000 (in steps of 2^-13) take the other form of the weight."""
+    import torch
+    from gtmoe.sampling import RowParams, RowSampler
+    V = 300
+    z = np.full((4, V), top, np.float32)
+    z[:, :V - 1] -= np.linspace(28.4215, 29.3, V - 1).astype(np.float32)   # no weight: (-43,000, -42,000) / 1,024 in base 2
+    z[1, 7] = np.float32(top - 28.4175)
+    z[2, V - 3:V - 1] = np.float32(top - 28.4175), np.float32(top - 28.0)
+    z[3, :V - 1] -= 2.0
+    s = RowSampler(V, 4)
+    r = s(torch.from_numpy(z).cuda(), [RowParams(1.0)] * 4, torch.zeros(4, dtype=torch.float64, device="cuda"))
+    assert r.tokens.cpu().tolist() == [V - 1, 7, V - 3, V - 1] and r.kept.cpu().tolist() == [V] * 4

@@ -144,7 +144,7 @@ __device__ __noinline__ unsigned long long exact_exp(const Sh& sh, float x, floa
     const float d = __fsub_rn(x, top), b = __fsub_rn(d, x);
     if (d == 0.0f) return 1ull << 40;
     const float y = __fmul_rn(d, hi);
-    if (!(y > -42.0f * 1024.0f)) return 0;   // below half of 2^-41
+    if (!(y > -42.0f * 1024.0f)) return 0;   // far below: v is not formed
     const float e = __fsub_rn(__fsub_rn(x, __fsub_rn(d, b)), __fadd_rn(top, b));   // what the difference was rounded by
     const float q = __fmul_rn(d, lo);
     constexpr float kUnit = 1099511627776.0f;   // 2^40
@@ -153,6 +153,7 @@ __device__ __noinline__ unsigned long long exact_exp(const Sh& sh, float x, floa
     v += __float2ll_rn(__fmaf_rn(d, lo2, __fmaf_rn(e, hi, e * lo)) * kUnit);
     v = v > 0 ? 0 : v;
     const int k = static_cast<int>(v >> 40);
+    if (k < -41 * 1024) return 0;   // below half of 2^-40; the shift below stays under 64
     const unsigned long long r = static_cast<unsigned long long>(v) << 24;              // in units of 2^-64
     const unsigned long long z = __umul64hi(r, 12486629536330718ull);                   // times ln 2 / 1024
     const unsigned long long z2 = __umul64hi(z, z) >> 1, z3 = __umul64hi(__umul64hi(z2, z), 6148914691236517205ull);   // / 3
@@ -165,16 +166,18 @@ __device__ __noinline__ unsigned long long exact_exp(const Sh& sh, float x, floa
 template <class Sh>
 __device__ __forceinline__ uint32_t short_exp(const Sh& sh, float x, const Scale& c, bool& big) {
     const float t = __fmaf_rn(x, c.hi, 12582912.0f);   // 1.5 * 2^23: the nearest integer in the low bits
-    const int k = __float_as_int(t) - 0x4B400000 - c.top_i;
-    big = static_cast<uint32_t>(k + 42 * 1024) >= 32u * 1024 || !c.brief;   // a t beyond its range gives a k beyond this one
+    // unsigned, as what a t beyond its range gives wraps around; it gives a k beyond this one
+    const uint32_t ku = __float_as_uint(t) - 0x4B400000u - static_cast<uint32_t>(c.top_i);
+    const int k = static_cast<int>(ku);
+    big = ku + 42u * 1024 >= 32u * 1024 || !c.brief;
     float r = __fmaf_rn(x, c.hi, -__fsub_rn(t, 12582912.0f));
     r = __fsub_rn(__fmaf_rn(x, c.lo, r), c.top_f);
     constexpr float kLn = 0.69314718055994530942f / 1024.0f;
     // (z + z^2 / 2) * 2^32 with z = r kLn, to the nearest integer (below 2^22 in magnitude)
     const float g = __fmaf_rn(r, 0.5f * kLn * kLn * 4294967296.0f, kLn * 4294967296.0f);
-    const int p = __float_as_int(__fmaf_rn(r, g, 12582912.0f)) - 0x4B400000;
+    const int p = static_cast<int>(__float_as_uint(__fmaf_rn(r, g, 12582912.0f)) - 0x4B400000u);
     const int m = sh.power30[k & 1023];
-    const uint32_t w = static_cast<uint32_t>(m + __mulhi(m, p)) >> ((-11 - (k >> 10)) & 31);   // twice the weight
+    const uint32_t w = (static_cast<uint32_t>(m) + static_cast<uint32_t>(__mulhi(m, p))) >> ((-11 - (k >> 10)) & 31);   // twice the weight
     return big ? 0u : (w + 1) >> 1;
 }
 template <class Sh>
