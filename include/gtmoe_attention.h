@@ -139,10 +139,13 @@ GTM_API size_t gtm_attention_kv_workspace_bytes(uint32_t q_heads, uint32_t kv_he
  * sequence's own cache as the prefix, with prefix_len one past the last row's position.
  * `prefix` has the cache's format, kv_heads and head_dim. A row's span must fit the rings: its
  * own positions within capacity, and prefix_len - first within the prefix's. q_heads a multiple of
- * kv_heads, at most 8 query heads per kv head. q_dev and ctx_dev [n][q_heads * head_dim], |q| below
- * 2^100. Infinities, NaN and whatever else the rings hold outside a row's span do not reach it. The
- * waits on the device are bounded: should one run out (1 s), the rows that it served are NaN, and
- * the next gtm_attention_kv_check on the workspace says so. */
+ * kv_heads, at most 8 query heads per kv head. q_dev and ctx_dev [n][q_heads * head_dim]. Scores
+ * are fp32, off by about 2^-20 of the sum of |q_d k_d| over a head's dims at most: |q| below 2^100
+ * and that sum up to 2^20 for every attended key, beyond which a row may be NaN (its stabiliser's
+ * steps would pass 1/8). Infinities, NaN and whatever else the rings hold outside a row's span do
+ * not reach it. The waits on the device are bounded: should one
+ * run out (1 s), the rows that it served are NaN, and the next gtm_attention_kv_check on the
+ * workspace says so. */
 GTM_API int gtm_attention_kv_rows(const GtmKvCache* cache, const GtmKvCache* prefix, uint32_t prefix_seq,
                                   uint32_t prefix_len, uint32_t q_heads, uint32_t n, uint32_t window,
                                   const float* q_dev, const uint32_t* seqs, const uint32_t* positions, float* ctx_dev,

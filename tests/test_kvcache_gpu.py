@@ -700,3 +700,34 @@ def test_a_wait_over_the_prefix_runs_out_then_workspace_recovers(fmt, hd, H, KV)
     assert torch.isnan(got[[i for i in range(n) if i % 4]]).all() and torch.equal(got[::4], want[::4])
     assert torch.equal(run_attention(cache, q, seqs, pos, **kw), want)
     op.check()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("hd,many", [(128, 1), (128, 64), (512, 64)])
+@pytest.mark.parametrize("q_top", [2.0 ** 99, 1.0, 2.0 ** -10])
+def test_scores_at_their_bound(hd, many, q_top, fmt):
+    """sum |q_d k_d| up to 2^20, with value scales of all sizes: a head whose best key's part of the result is e^30 times
+    the next one's (nine in ten of them here) gives that key's value, to 2^-20 (the weight's two limbs and the last
+    division); all are finite."""
+    import torch
+    from gtmoe.kvcache import KvCache
+    P, KV, H = 1600, 1, 8
+    prefix, cache = KvCache(1, P, KV, hd, fmt), KvCache(1, 1, KV, hd, fmt)
+    fill(prefix, 97)
+    fill(cache, 98)
+    prefix.v_scale.mul_(torch.exp2(torch.linspace(-40, 20, P))[torch.randperm(P, generator=torch.Generator().manual_seed(1))].cuda())
+    q = queries(many, H, hd)
+    q *= q_top * 0.999 / q.abs().max()
+    qs = q.cpu().numpy().astype(np.float64).reshape(-1, hd)
+    keys = np.concatenate([values(c, "k")[0] for c in (prefix, cache)])[:, 0]
+    scale = 2.0 ** 19.99 / (np.abs(qs) @ np.abs(keys).T).max()
+    for c in (prefix, cache):
+        c.k_scale.mul_(scale)
+    got = run_attention(cache, q, [0] * many, [P] * many, 0, prefix, 0, P).cpu().numpy().astype(np.float64).reshape(-1, hd)
+    keys, vals = (np.concatenate([values(c, w)[0] for c in (prefix, cache)])[:, 0] for w in "kv")
+    parts = qs @ keys.T + np.log(np.concatenate([c.v_scale[0, 0].cpu().numpy() for c in (prefix, cache)]).astype(np.float64))
+    best, two = (qs @ keys.T).argmax(1), np.sort(parts, 1)[:, -2:]
+    clear = (two[:, 1] - two[:, 0] >= 30) & (parts.argmax(1) == best)
+    assert clear.mean() >= 0.9 and np.isfinite(got).all()
+    want = vals[best][clear]
+    assert (np.abs(got[clear] - want).max(1) <= 2.0 ** -20 * np.abs(want).max(1)).all()
