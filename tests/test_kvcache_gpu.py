@@ -731,3 +731,19 @@ def test_scores_at_their_bound(hd, many, q_top, fmt):
     assert clear.mean() >= 0.9 and np.isfinite(got).all()
     want = vals[best][clear]
     assert (np.abs(got[clear] - want).max(1) <= 2.0 ** -20 * np.abs(want).max(1)).all()
+
+
+@pytest.mark.parametrize("n,H,KV,hd", [(1, 16, 8, 256), (300, 21, 3, 128), (512, 16, 2, 512)])
+def test_write_in_place_over_many_heads(n, H, KV, hd):
+    """q_out is q, a warp taking several heads of a row in turn: the bits of the call with an output of its own."""
+    import torch
+    from gtmoe.kvcache import KvCache
+    g = torch.Generator(device="cuda").manual_seed(n)
+    q, k = (torch.randn(n, heads * hd, generator=g, device="cuda") for heads in (H, KV))
+    a, b = KvCache(1, n, KV, hd), KvCache(1, n, KV, hd)
+    own = torch.empty_like(q)
+    a.write(q, k, k, own, range(n), [0] * n, rotated_pairs=hd // 2)
+    b.write(q, k, k, q, range(n), [0] * n, rotated_pairs=hd // 2)
+    assert torch.equal(q, own)
+    for x in ("k", "v", "k_scale", "v_scale"):
+        assert torch.equal(getattr(a, x), getattr(b, x))

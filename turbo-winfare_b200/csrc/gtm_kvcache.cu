@@ -45,23 +45,24 @@ __device__ __forceinline__ double warp_max(double a) {
     return a;
 }
 
-// V consecutive floats at p.
+// V consecutive floats at p. Plain loads: q may be written in place by this very launch (each warp writes a head that
+// it has read), and __ldg is for what no one writes meanwhile.
 template <int V>
 __device__ __forceinline__ void load_vals(const float* p, bool vec, float (&x)[V]) {
     if (vec) {
         if constexpr (V == 2) {
-            const float2 t = __ldg(reinterpret_cast<const float2*>(p));
+            const float2 t = *reinterpret_cast<const float2*>(p);
             x[0] = t.x, x[1] = t.y;
         } else {
 #pragma unroll
             for (int j = 0; j < V / 4; ++j) {
-                const float4 t = __ldg(reinterpret_cast<const float4*>(p) + j);
+                const float4 t = reinterpret_cast<const float4*>(p)[j];
                 x[4 * j] = t.x, x[4 * j + 1] = t.y, x[4 * j + 2] = t.z, x[4 * j + 3] = t.w;
             }
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = __ldg(p + j);
+        for (int j = 0; j < V; ++j) x[j] = p[j];
     }
 }
 
