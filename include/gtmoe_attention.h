@@ -108,7 +108,8 @@ typedef struct GtmKvCache {
  * apart) belongs to sequence seqs[i] at positions[i] (HOST arrays, as in the *_rows entries: read
  * during the call, so a captured launch keeps the values it was captured with).
  *   q: RMS norm per head with weight q_w_dev (bf16, NULL = none), rotation -> q_out_dev
- *      [n][q_heads * head_dim] (q_out_dev may be q_dev where q_stride is q_heads * head_dim)
+ *      [n][q_heads * head_dim] (q_out_dev may be q_dev where q_stride is q_heads * head_dim; any
+ *      other overlap with an input's rows is refused)
  *   k: RMS norm with k_w_dev, rotation -> cache;   v: RMS norm without a weight -> cache
  * v_dev may be k_dev. The rotation is NeoX over the first rotated_pairs pairs, angle position *
  * theta^(-2i / head_dim). Norms, angles and the codes' rounding are in 64 bits, each result
@@ -139,7 +140,8 @@ GTM_API size_t gtm_attention_kv_workspace_bytes(uint32_t q_heads, uint32_t kv_he
  * sequence's own cache as the prefix, with prefix_len one past the last row's position.
  * `prefix` has the cache's format, kv_heads and head_dim. A row's span must fit the rings: its
  * own positions within capacity, and prefix_len - first within the prefix's. q_heads a multiple of
- * kv_heads, at most 8 query heads per kv head. q_dev and ctx_dev [n][q_heads * head_dim]. Scores
+ * kv_heads, at most 8 query heads per kv head. q_dev and ctx_dev [n][q_heads * head_dim], one buffer
+ * or two that do not overlap. Scores
  * are fp32, off by about 2^-20 of the sum of |q_d k_d| over a head's dims at most: |q| below 2^100
  * and that sum up to 2^20 for every attended key, beyond which a row may be NaN (its stabiliser's
  * steps would pass 1/8). Infinities, NaN and whatever else the rings hold outside a row's span do

@@ -747,3 +747,17 @@ def test_write_in_place_over_many_heads(n, H, KV, hd):
     assert torch.equal(q, own)
     for x in ("k", "v", "k_scale", "v_scale"):
         assert torch.equal(getattr(a, x), getattr(b, x))
+
+
+@pytest.mark.parametrize("n,P,own", [(1, 0, 40), (1, 0, 3000), (40, 3000, 50), (3, 20, 300)])
+def test_attention_in_place(n, P, own):
+    """ctx is q: one run a row, several, and a shared prefix, each with the bits of the call with two buffers."""
+    from gtmoe.kvcache import KvAttention, KvCache
+    cache, prefix = KvCache(n, own, 2, 256), KvCache(1, max(1, P), 2, 256)
+    fill(cache, 99)
+    fill(prefix, 100)
+    q, pos = queries(n, 16, 256), [P + own - 1 - i % own for i in range(n)]
+    want = run_attention(cache, q, range(n), pos, 0, prefix, 0, P)
+    KvAttention(16, 2, 256, n)(q, cache, range(n), pos, q, prefix=prefix, prefix_len=P)
+    import torch
+    assert torch.equal(q, want)

@@ -202,3 +202,33 @@ def test_python_wrappers_refuse_what_a_uint32_would_wrap():
 
 def test_check_needs_a_workspace():
     assert gtmoe.lib().gtm_attention_kv_check(None, None) == gtmoe.ERR_INVALID and "workspace" in gtmoe.last_error()
+
+
+A = 1 << 20   # addresses apart from one another; never dereferenced
+
+
+@pytest.mark.parametrize("kw,bad", [
+    (dict(out=A + 16), True), (dict(q=A + 4, out=A + 4 * 4096), True),     # q, shifted by a little; q's last float
+    (dict(k=2 * A, out=2 * A - 4 * 4096 + 16), True), (dict(k=2 * A, out=2 * A - 4 * 4096), False),   # k's first floats, and just before them
+    (dict(v=3 * A, out=3 * A + 4 * 508), True), (dict(v=3 * A, out=3 * A + 4 * 512), False),           # v's last ones, and just behind
+    (dict(n=2, pos=(3, 4), seqs=(0, 0), qs=100000, out=A + 4 * 4096), False),         # between two strided rows
+    (dict(n=2, pos=(3, 4), seqs=(0, 0), qs=12284, out=A + 4 * 4096), True),            # not quite
+    (dict(out=A), False),                                                               # in place
+    (dict(out=A, k=A + 4 * 4000), True),
+])
+def test_write_refuses_an_output_over_its_inputs(kw, bad):
+    args = dict(q=A, k=4 * A, v=5 * A, out=8 * A)
+    args.update(kw)
+    import torch
+    if not bad and torch.cuda.is_available():
+        pytest.skip("made-up addresses: only on a machine without a GPU")
+    rc = write(**args)
+    assert (rc == gtmoe.ERR_INVALID and "overlap" in gtmoe.last_error()) == bad
+
+
+def test_attention_refuses_overlaps():
+    n = dict(n=2, seqs=(0, 0), pos=(3, 3))
+    size, ws = 2 * 16 * 256 * 4, gtmoe.lib().gtm_attention_kv_workspace_bytes(16, 2, 256, 2)
+    for kw in (dict(q=A, ctx=A + 16), dict(q=A, ctx=A - size + 16), dict(q=A, ctx=2 * A, ws=A + size - 16),
+               dict(q=A, ctx=A + 64 * A, ws=A + 64 * A - ws + 16)):
+        assert attend(**{**n, **{"ws": 512 * A}, **kw}) == gtmoe.ERR_INVALID and "overlap" in gtmoe.last_error(), kw

@@ -150,7 +150,8 @@ __global__ void __launch_bounds__(RowsShape<HD>::kThreads, HD == 512 ? 1 : 2)
         float x[HD / 32], top = 0.0f;
 #pragma unroll
         for (int i = 0; i < HD / 128; ++i) {
-            const float4 v = h < grp ? __ldg(reinterpret_cast<const float4*>(src) + lane + 32 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+            // a plain load: ctx may be q's own buffer
+            const float4 v = h < grp ? reinterpret_cast<const float4*>(src)[lane + 32 * i] : make_float4(0.f, 0.f, 0.f, 0.f);
             x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
         }
 #pragma unroll
@@ -541,6 +542,9 @@ GTM_API int gtm_attention_kv_rows(const GtmKvCache* c, const GtmKvCache* prefix,
     }
     const size_t need = gtm_attention_kv_workspace_bytes(q_heads, c->kv_heads, c->head_dim, n);
     if (!ws || ws_bytes < need) return set_error(GTM_ERR_WORKSPACE, "%s: workspace needs %zu bytes", fn, need);
+    const size_t row_bytes = static_cast<size_t>(n) * q_heads * c->head_dim * sizeof(float);
+    if ((ctx != q && overlap(q, row_bytes, ctx, row_bytes)) || overlap(ws, need, q, row_bytes) || overlap(ws, need, ctx, row_bytes))
+        return set_error(GTM_ERR_INVALID, "%s: q, ctx and workspace overlap", fn);
     const auto side = [](const GtmKvCache* x, size_t s) {
         const size_t vec = s * x->capacity * x->kv_heads;
         return Side{static_cast<const uint8_t*>(x->k_dev) + vec * x->head_dim, static_cast<const uint8_t*>(x->v_dev) + vec * x->head_dim,

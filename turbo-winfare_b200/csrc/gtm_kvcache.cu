@@ -285,6 +285,14 @@ bool ring_row_twice(const uint32_t* seqs, const uint32_t* positions, uint32_t n,
     return false;
 }
 
+// Whether `out` touches a row of x (n rows of `width` floats, `stride` apart).
+bool rows_touch(const float* x, uint64_t stride, uint64_t width, uint32_t n, const float* out, uint64_t out_floats) {
+    if (!overlap(x, ((n - 1) * stride + width) * 4, out, out_floats * 4)) return false;
+    for (uint32_t i = 0; i < n; ++i)
+        if (overlap(x + i * stride, width * 4, out, out_floats * 4)) return true;
+    return false;
+}
+
 template <int HD>
 void launch_write(const WriteArgs& a, const RowU32& pos, const RowU32& seq, uint32_t n, uint32_t fmt, cudaStream_t st) {
     // A CTA per row forms each angle once; few rows are split over their heads (a CTA per 8, an
@@ -341,6 +349,10 @@ GTM_API int gtm_qkv_cache_rows(const GtmKvCache* c, uint32_t q_heads, uint32_t n
     }
     if (ring_row_twice(seqs, positions, n, c->capacity))
         return set_error(GTM_ERR_INVALID, "%s: two rows write the same ring row of one sequence", fn);
+    // a head's warp writes q_out while others still read: only where each reads what it writes, in place, is that sound
+    if ((q_out != q && rows_touch(q, q_stride, q_width, n, q_out, n * q_width)) ||
+        rows_touch(k, k_stride, kv_width, n, q_out, n * q_width) || rows_touch(v, v_stride, kv_width, n, q_out, n * q_width))
+        return set_error(GTM_ERR_INVALID, "%s: q_out overlaps an input's rows (it may be q itself)", fn);
     WriteArgs a;
     a.q = q, a.k = k, a.v = v;
     a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride;

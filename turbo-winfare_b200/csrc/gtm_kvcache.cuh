@@ -19,6 +19,12 @@ constexpr float kKvTiny = 7.8886090522101181e-31f;   // 2^-100, the least scale 
 
 inline bool ptr_aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; }
 
+// Whether [a, a + na) and [b, b + nb) share bytes.
+inline bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + nb && y < x + na;
+}
+
 // GTM_OK, or the error of a cache descriptor that no kernel may be given.
 inline int check_kv(const char* fn, const char* what, const GtmKvCache* c) {
     if (!c) return set_error(GTM_ERR_INVALID, "%s: null %s", fn, what);
