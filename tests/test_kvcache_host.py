@@ -232,3 +232,16 @@ def test_attention_refuses_overlaps():
     for kw in (dict(q=A, ctx=A + 16), dict(q=A, ctx=A - size + 16), dict(q=A, ctx=2 * A, ws=A + size - 16),
                dict(q=A, ctx=A + 64 * A, ws=A + 64 * A - ws + 16)):
         assert attend(**{**n, **{"ws": 512 * A}, **kw}) == gtmoe.ERR_INVALID and "overlap" in gtmoe.last_error(), kw
+
+
+def test_norm_weights_are_bf16_or_its_bits():
+    import torch
+    from gtmoe.kvcache import _bf16
+    cpu = torch.device("cpu")
+    for dt in (torch.bfloat16, torch.int16, torch.uint16):
+        t = torch.zeros(4, dtype=dt)
+        assert _bf16(t, "q_w", cpu, 4) == t.data_ptr()
+    assert _bf16(None, "q_w", cpu, 4) is None
+    for t in (torch.zeros(4, dtype=torch.float16), torch.zeros(4), torch.zeros(4, dtype=torch.int8), torch.zeros(8, dtype=torch.bfloat16)[::2]):
+        with pytest.raises(gtmoe.GtmError, match="q_w must be 4 contiguous bf16"):
+            _bf16(t, "q_w", cpu, 4)

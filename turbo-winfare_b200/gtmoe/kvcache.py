@@ -73,9 +73,11 @@ def _rows(t, name: str, device, n: int, width: int):
 
 
 def _bf16(t, name: str, device, n: int):
+    """A bfloat16 tensor, or one of its bits as int16 or uint16 (an fp16 one would be read as what it is not)."""
+    import torch
     if t is None:
         return None
-    if t.element_size() != 2 or t.numel() != n or not t.is_contiguous() or t.device != device:
+    if t.dtype not in (torch.bfloat16, torch.int16, torch.uint16) or t.numel() != n or not t.is_contiguous() or t.device != device:
         raise GtmError(ERR_INVALID, f"{name} must be {n} contiguous bf16 values on {device}")
     return t.data_ptr()
 
