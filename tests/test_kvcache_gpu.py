@@ -761,3 +761,29 @@ def test_attention_in_place(n, P, own):
     KvAttention(16, 2, 256, n)(q, cache, range(n), pos, q, prefix=prefix, prefix_len=P)
     import torch
     assert torch.equal(q, want)
+
+
+def test_read_on_another_stream_leaves_what_is_queued_alone():
+    """Outputs allocated for another stream must not be memory that the current stream has given up and still reads."""
+    import torch
+    from gtmoe.kvcache import KvCache
+    c = KvCache(1, 4096, 2, 128)
+    fill(c, 101)
+    want, _ = c.read(0, 0, 4096)
+    s = torch.cuda.Stream()
+    kept = torch.empty(4096, 256, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(3):
+        given_up = [torch.full((4096, 256), 5.0, device="cuda") for _ in range(4)]
+        torch.cuda._sleep(20_000_000)   # ~10 ms of the current stream
+        for t in given_up:
+            kept.copy_(t)
+        ptrs = {t.data_ptr() for t in given_up}
+        del given_up, t
+        k, v = c.read(0, 0, 4096, stream=s)
+        assert not ptrs & {k.data_ptr(), v.data_ptr()}
+        s.synchronize()
+        assert torch.equal(k, want)
+        torch.cuda.synchronize()
+        assert (kept == 5.0).all()
+        del k, v

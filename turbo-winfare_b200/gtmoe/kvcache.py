@@ -141,12 +141,16 @@ class KvCache:
 
     def read(self, seq: int, first: int, count: int, k_out=None, v_out=None, stream=None):
         """gtm_kv_read: positions [first, first + count) of `seq` as fp32 [count, kv_heads * head_dim];
-        (k_out, v_out), allocated where both are None."""
+        (k_out, v_out), allocated where both are None, as memory of the stream that writes them."""
         _uint(seq=seq, first=first, count=count)
         shape = (count, self.kv_heads * self.head_dim)
         if k_out is None and v_out is None:
+            import contextlib
+
             import torch
-            k_out, v_out = (torch.empty(shape, dtype=torch.float32, device=self.device) for _ in range(2))
+            # memory that the current stream has given up may still be read by what is queued there
+            with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
+                k_out, v_out = (torch.empty(shape, dtype=torch.float32, device=self.device) for _ in range(2))
         kp = None if k_out is None else _f32(k_out, "k_out", self.device, shape)
         vp = None if v_out is None else _f32(v_out, "v_out", self.device, shape)
         check(lib().gtm_kv_read(self._ref, seq, first, count, kp, vp, _raw_stream(stream, self.device)))
