@@ -787,3 +787,37 @@ def test_read_on_another_stream_leaves_what_is_queued_alone():
         torch.cuda.synchronize()
         assert (kept == 5.0).all()
         del k, v
+
+
+def test_two_threads_attend_at_once():
+    """Each on its own stream with its own workspace, the first calls over a shared prefix among them."""
+    import threading
+
+    import torch
+    from gtmoe.kvcache import KvAttention, KvCache
+    n, P = 32, 4096
+    cache, prefix = KvCache(n, 8, 2, 256), KvCache(1, P, 2, 256)
+    fill(cache, 102)
+    fill(prefix, 103)
+    torch.cuda.synchronize()
+    out, errors = {}, []
+
+    def work(i):
+        try:
+            q, s = queries(n, 16, 256, i % 2), torch.cuda.Stream()
+            op, ctx = KvAttention(16, 2, 256, n), torch.empty(n, 16 * 256, device="cuda")
+            torch.cuda.synchronize()
+            for _ in range(20):
+                op(q, cache, range(n), [P + j % 8 for j in range(n)], ctx, prefix=prefix, prefix_len=P, stream=s)
+            s.synchronize()
+            out[i] = ctx
+        except Exception as e:   # told to the test's own thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    assert torch.equal(out[0], out[2]) and torch.equal(out[1], out[3]) and not torch.equal(out[0], out[1])

@@ -41,6 +41,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "gtm_frag.cuh"
 #include "gtm_kvattn.cuh"
@@ -617,13 +618,15 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
 
 int map_codes(CUtensorMap* m, const void* codes, uint64_t width, uint64_t rows, uint32_t box_w, uint32_t box_rows,
               CUtensorMapSwizzle swizzle) {
-    static EncodeTiledFn encode = nullptr;
+    static std::atomic<EncodeTiledFn> found{nullptr};   // two threads' first calls may look it up at once
+    EncodeTiledFn encode = found.load(std::memory_order_relaxed);
     if (!encode) {
         void* f = nullptr;
         cudaDriverEntryPointQueryResult q;
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
             return set_error(GTM_ERR_CUDA, "cuTensorMapEncodeTiled not available");
         encode = reinterpret_cast<EncodeTiledFn>(f);
+        found.store(encode, std::memory_order_relaxed);
     }
     const cuuint64_t dims[2] = {width, rows}, strides[1] = {width};
     const cuuint32_t box[2] = {box_w, box_rows}, estr[2] = {1, 1};
