@@ -127,9 +127,9 @@ GTM_API int gtm_kv_read(const GtmKvCache* cache, uint32_t seq, uint32_t first, u
                         float* v_out_dev, void* stream);
 /* Workspace of gtm_attention_kv_rows for at most n rows (0 for unsupported shapes). Its first 4
  * bytes are an error word: zero them once before the first use where gtm_attention_kv_check is to
- * be called; the rest needs no initialisation. It depends on the current device's number of SMs (a B200's where there is no
- * device). A workspace serves one stream at a time; two captured graphs may share one if their
- * replays do not overlap. */
+ * be called; the rest needs no initialisation. Its size depends on the current device's number of
+ * SMs (a B200's where there is no device). A workspace serves one stream at a time; two captured
+ * graphs may share one if their replays do not overlap. */
 GTM_API size_t gtm_attention_kv_workspace_bytes(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t n);
 /* Attention of n rows (n <= 512) at positions[i] of sequences seqs[i] (HOST arrays): row i attends
  * [first, positions[i]] with first = max(0, positions[i] + 1 - window) (window 0 = all), scores
@@ -141,13 +141,14 @@ GTM_API size_t gtm_attention_kv_workspace_bytes(uint32_t q_heads, uint32_t kv_he
  * `prefix` has the cache's format, kv_heads and head_dim. A row's span must fit the rings: its
  * own positions within capacity, and prefix_len - first within the prefix's. q_heads a multiple of
  * kv_heads, at most 8 query heads per kv head. q_dev and ctx_dev [n][q_heads * head_dim], one buffer
- * or two that do not overlap. Scores
- * are fp32, off by about 2^-20 of the sum of |q_d k_d| over a head's dims at most: |q| below 2^100
- * and that sum up to 2^20 for every attended key, beyond which a row may be NaN (its stabiliser's
- * steps would pass 1/8). Infinities, NaN and whatever else the rings hold outside a row's span do
- * not reach it. The waits on the device are bounded: should one
- * run out (1 s), the rows that it served are NaN, and the next gtm_attention_kv_check on the
- * workspace says so. */
+ * or two that do not overlap. Scores are fp32, off by at most 2^-17 of the sum of |q_d k_d| over a head's dims (q and the softmax
+ * weights are multiplied as two fp16 limbs, 22 bits): |q| below 2^100, and that sum up to 2^20 for
+ * every attended key, beyond which a row may be NaN (its stabiliser's steps would pass 1/8).
+ * Outputs were within 6.3e-6 of 64-bit ones (2-norm, 32,768 positions; a plain fp32 form 4.4e-6).
+ * Codes that a caller brings are taken as numbers: an e4m3 0x7F or 0xFF (NaN, which gtm_kv_read
+ * gives) counts as 480 here. Infinities, NaN and whatever else the rings hold outside a row's span
+ * do not reach it. The waits on the device are bounded: should one run out (1 s), the rows that it
+ * served are NaN, and the next gtm_attention_kv_check on the workspace says so. */
 GTM_API int gtm_attention_kv_rows(const GtmKvCache* cache, const GtmKvCache* prefix, uint32_t prefix_seq,
                                   uint32_t prefix_len, uint32_t q_heads, uint32_t n, uint32_t window,
                                   const float* q_dev, const uint32_t* seqs, const uint32_t* positions, float* ctx_dev,

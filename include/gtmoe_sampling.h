@@ -93,8 +93,9 @@ GTM_API int gtm_sample_token(const float* logits_dev, uint32_t vocab, const GtmS
  * over the kept ids in id order exceeds u times their whole sum; temperature 0 takes the first
  * id. All cuts see the full distribution (no shortlist: top_k is not bounded by 256). Weights are
  * rounded to multiples of 2^-40 of the largest and summed as integers, so a row's token depends
- * neither on the other rows nor on the order of a sum. A logit of NaN counts as -infinity. A row whose largest logit is
- * infinite has no token: 0xFFFFFFFF, kept 0, logprob NaN.
+ * neither on the other rows nor on the order of a sum; ids below 2^-41 of the largest weigh nothing:
+ * they count as kept where no cut takes them, and are never drawn. A logit of NaN counts as
+ * -infinity. A row whose largest logit is infinite has no token: 0xFFFFFFFF, kept 0, logprob NaN.
  * ------------------------------------------------------------------------------------- */
 typedef struct GtmSamplingRow {
     float temperature;          /* >= 0; 0 = greedy                */

@@ -84,7 +84,7 @@ cudaError_t launch_after(bool early, void (*kernel)(P...), dim3 grid, int thread
 //
 // Bytes are the floor (a code is read once per row and kv head, for at most 8 heads' products), but the
 // chain of a tile bounds it: load, widening and products, a barrier among the scorers, exponentials, the
-// hand-over, the sums. 32 rows of 77-8,192 positions, 2 heads of 512 (275 MB): 85 us, 3.2 TB/s, with one CTA
+// hand-over, the sums. 32 rows of 77-8,192 positions, 2 heads of 512 (275 MB): 84 us, 3.3 TB/s, with one CTA
 // of 16 warps per SM; 61 windowed rows, 8 heads of 256, two of 8 warps: 55 us; one row of 1,024: 4.3. All warps
 // scoring and then summing took 99 and 64 us (91 and 55 since, with the same runs); then neither leaving out the products nor codes that stay in L2
 // made it faster.
@@ -393,11 +393,12 @@ __global__ void __launch_bounds__(HD / 4) kv_combine(const __grid_constant__ Row
 
 // Prefix positions x kv heads over all rows from which the prefix is computed once for all (two rows or more).
 // kv_shared costs 10 (128 dims) to 25 us (512) however little it does; kv_rows reads the prefix again for every
-// row at 3.3-4.3 TB/s. Whole calls, once for all against row by row, int8: 2 heads of 512, 16 rows x 2,048
-// positions (65,536) 40 against 40 us, 32 rows (131,072) 42 against 56, 32 rows x 16,384 83 against 259; 8 heads of
-// 256, 4 rows x 2,048 (65,536) 27 against 23, 8 rows (131,072) 27 against 27, 32 rows x 512 (131,072) 26 against 30,
-// 2 rows x 16,384 (262,144) 46 against 48; 8 heads of 128, 8 rows x 2,048 (131,072) 23 against 21, 16 rows 24
-// against 33.
+// row at 3.3-4.3 TB/s. Calls replayed from a graph, us, once for all against row by row, int8 (e4m3 takes 1-2 us
+// more on both sides): 2 heads of 512, 16 rows x 2,048 positions (65,536) 38 against 29, 32 rows (131,072) 39 against
+// 53, but 2 rows x 32,768 (131,072) 75 against 60; 8 heads of 256, 4 rows x 2,048 (65,536) 25 against 15, 8 rows
+// (131,072) 25 against 25, 32 rows x 512 (131,072) 24 against 25, 2 rows x 16,384 (262,144) 48 against 47; 8 heads
+// of 128, 8 rows x 2,048 (131,072) 21 against 18, 16 rows 22 against 29; 4 heads of 128 under 32, 16 rows x 2,048
+// (131,072) 23 against 19. The rule knows neither the heads' width nor how full a unit's 64 columns are.
 constexpr uint64_t kSharedFrom = 98304;
 
 // Items of all rows are at most n plus this (a run is at least the total / target).

@@ -29,10 +29,11 @@
 // is used, so two limbs of 64 rows cost (HD / 16) x 62 for S and, where the limbs do not fit side by side
 // (512 dims), twice that for O: ~6,000 cycles a tile of 512 dims. A tile takes ~10,000: the hand-overs of
 // K, V, S and p each add a wait, and no role is busy throughout (without any one of conversions, softmax or
-// half the products it took 5 to 20% less). 512 rows (16 / 2 heads of 512) over 32,768 positions: 1.49 ms;
-// 32 rows over 16,384: 71 us; 61 windowed rows (8 heads of 256): 18-20 us.
-// kLongest: 16 tiles 1.63 ms and 5.3e-6 of relative error, 24 1.52 and 7.0e-6, 32 1.52 and 8.7e-6 (before results
-// were added to memory without reading them back); now 20, 1.49 and 6.1e-6.
+// half the products it took 5 to 20% less). 512 rows (16 / 2 heads of 512) over 32,768 positions: 1.49-1.52 ms;
+// 32 rows over 16,384: 72 us; 61 windowed rows (8 heads of 256): 20 us.
+// kLongest, that prompt's time and error against 64 bits: 8 tiles 1.74 ms and 3.6e-6, 12 1.63 and 4.4e-6 (as the
+// plain fp32 form), 16 1.55 and 5.3e-6, 20 1.52 and 6.2e-6. 20 is taken: still within fp32 sums of that length. Runs
+// of up to 20 tiles (32 rows over 16,384 positions: 3.4e-6 against the plain form's 3.7e-6) do not notice.
 //
 // Roles: warps 0-7 softmax and O (32 of the 64 columns each half of them); 8-11 K; 12-15 V; 16 issues
 // S, 17 O; 18 and 19 load the codes of K and V. Every wait is bounded (1 s); one that runs out stops the

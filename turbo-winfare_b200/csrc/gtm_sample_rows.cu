@@ -2,9 +2,10 @@
 //
 // One cluster of CTAs per row: each keeps its share of the row's logits in shared memory (larger
 // shares are read from L2 again), so HBM is read once and every later pass runs on chip, with no
-// workspace and one launch. Instructions bound it, ~25 for an id's weight, as many for the counts and the
-// bracket's test, and ten cluster barriers a row: one row of 262,144 ids takes 46 us, 64 rows under mixed
-// rules 162-178, 512 rows 871 (1.7 each); the bytes of 64 are 10.4 us.
+// workspace and one launch. Two things take its time: instructions, ~25 for an id's weight, as many for the counts
+// and the bracket's test (half of the issue slots at 64 rows), and ten cluster barriers a row (its largest stall):
+// one row of 262,144 ids takes 47 us, 64 rows under mixed rules 170-181, 512 rows 871 (1.7 each); the bytes of 64 are
+// 10.4 us.
 //   1 the largest logit, and its lowest id;
 //   2 the cuts. Ranked by logit, every cut keeps a run from the top, so the kept set is the ids whose
 //     key (logit, then lower id) is at least a border's. Ids are counted per level of max - logit,
