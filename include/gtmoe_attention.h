@@ -141,9 +141,10 @@ GTM_API size_t gtm_attention_kv_workspace_bytes(uint32_t q_heads, uint32_t kv_he
  * `prefix` has the cache's format, kv_heads and head_dim. A row's span must fit the rings: its
  * own positions within capacity, and prefix_len - first within the prefix's. q_heads a multiple of
  * kv_heads, at most 8 query heads per kv head. q_dev and ctx_dev [n][q_heads * head_dim], one buffer
- * or two that do not overlap. Scores are fp32, off by at most 2^-17 of the sum of |q_d k_d| over a head's dims (q and the softmax
- * weights are multiplied as two fp16 limbs, 22 bits): |q| below 2^100, and that sum up to 2^20 for
- * every attended key, beyond which a row may be NaN (its stabiliser's steps would pass 1/8).
+ * or two that do not overlap. Scores are fp32, off by at most 2^-17 of the sum of |q_d k_d| over a
+ * head's dims and 2^-39 of max |q| times the sum of |k_d| (q and the softmax weights are multiplied
+ * as two fp16 limbs, 22 bits): |q| below 2^100, and the first sum up to 2^20 for every attended key,
+ * beyond which a row may be NaN (its stabiliser's steps would pass 1/8).
  * Outputs were within 6.3e-6 of 64-bit ones (2-norm, 32,768 positions; a plain fp32 form 4.4e-6).
  * Codes that a caller brings are taken as numbers: an e4m3 0x7F or 0xFF (NaN, which gtm_kv_read
  * gives) counts as 480 here. Infinities, NaN and whatever else the rings hold outside a row's span

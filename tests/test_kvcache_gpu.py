@@ -821,3 +821,23 @@ def test_two_threads_attend_at_once():
         t.join()
     assert not errors, errors
     assert torch.equal(out[0], out[2]) and torch.equal(out[1], out[3]) and not torch.equal(out[0], out[1])
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("hd,many", [(128, 2), (512, 2), (128, 64), (512, 64)])
+@pytest.mark.parametrize("outlier", [2.0 ** 13, 2.0 ** 20])
+def test_an_outlier_in_a_query_leaves_its_other_dims_their_bits(hd, many, outlier, fmt):
+    """One dim of each query is thousands of times the others, and no key has a value there: the scores are the other
+    dims', S too, and as exact as without it, beside the limbs' end, 2^-39 of the largest |q| times the keys' sum of
+    |k_d|: a quarter of ds for an outlier of 2^20, which the bar's 64 steps cover, as a sum has at most 32."""
+    import torch
+    from gtmoe.kvcache import KvCache
+    P, H = 1600, 8
+    prefix, cache = KvCache(1, P, 1, hd, fmt), KvCache(1, 1, 1, hd, fmt)
+    fill(prefix, 104)
+    fill(cache, 105)
+    for c in (prefix, cache):
+        c.k.view(torch.uint8)[..., 7] = 0
+    q = queries(many, H, hd)
+    q.view(many, H, hd)[..., 7] = outlier * 3.0 / hd ** 0.5
+    check_attention(cache, q, [0] * many, [P] * many, 0, prefix, 0, P)

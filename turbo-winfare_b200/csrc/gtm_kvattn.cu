@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(RowsShape<HD>::kThreads, HD == 512 ? 1 : 2)
     float2 sc_next = make_float2(0.0f, 0.0f);
     write_places(0, sc_next);
     if (tid < T) sc_s[0][tid] = sc_next;
-    // q of head h: scaled by a power of two into [1, 2), then high and low fp16 parts
+    // q of head h: scaled by a power of two, then high and low fp16 parts
     for (int h = warp; h < 8; h += 2 * W) {
         const float* src = a.q + (static_cast<size_t>(row) * a.q_heads + static_cast<size_t>(kvh) * grp + h) * HD;
         float x[HD / 32], top = 0.0f;
@@ -157,9 +157,9 @@ __global__ void __launch_bounds__(RowsShape<HD>::kThreads, HD == 512 ? 1 : 2)
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i) top = fmaxf(top, fabsf(x[i]));
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int e = top > 0.0f ? max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127)) : 0;
-        const float down = __int_as_float((127 - e) << 23);
-        if (lane == 0) qscale[h] = __int_as_float((127 + e) << 23) * kLog2e * (FMT == GTM_KV_E4M3 ? 256.0f : 1.0f);
+        const int e = query_exponent(top);
+        const float down = query_down(e);
+        if (lane == 0) qscale[h] = query_up(e) * kLog2e * (FMT == GTM_KV_E4M3 ? 256.0f : 1.0f);
 #pragma unroll
         for (int i = 0; i < HD / 128; ++i) {
             const int d = 4 * lane + 128 * i;   // four dims of one 16-dim run

@@ -42,6 +42,15 @@ constexpr float kWeightTop = 15.9f;
 // fp32. Values of smaller scales (2^-100 is the least) still have p up to 2^3.
 __device__ __forceinline__ float log2_vs(float vs) { return log2f(fmaxf(vs, 3.2311742677852644e-27f)); }
 
+// A query head is split with its largest value in [2^14, 2^15), as its limbs, too, end at 2^-25: from [1, 2) on,
+// one value thousands of times the others cost those their low bits. The power of two, from the largest |q|, and
+// the factors 2^(14 - e) and 2^(e - 14).
+__device__ __forceinline__ int query_exponent(float top) {
+    return max(-112, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+}
+__device__ __forceinline__ float query_down(int e) { return __int_as_float((141 - e) << 23); }
+__device__ __forceinline__ float query_up(int e) { return __int_as_float((113 + e) << 23); }
+
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

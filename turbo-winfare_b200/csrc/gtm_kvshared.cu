@@ -224,8 +224,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < HD / 32; ++i) top = fmaxf(top, fabsf(x[i]));
             for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const int e = top > 0.0f ? max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127)) : 0;
-            const float down = __int_as_float((127 - e) << 23);
+            const int e = query_exponent(top);
+            const float down = query_down(e);
 #pragma unroll
             for (int i = 0; i < HD / 128; ++i) {
                 const int d = 4 * lane + 128 * i;
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 *reinterpret_cast<uint2*>(sQ + 8192 + off) = make_uint2(lo[0], lo[1]);
             }
             if (lane == 0) {
-                qf_s[r] = __int_as_float((127 + e) << 23) * kLog2e * (FMT == GTM_KV_E4M3 ? 256.0f : 1.0f);
+                qf_s[r] = query_up(e) * kLog2e * (FMT == GTM_KV_E4M3 ? 256.0f : 1.0f);
                 m_s[r] = -INFINITY;
                 const Span sp = live ? row_span(pos.v[row], a.window, a.prefix_len) : Span{0, 0, 0, 0};
                 // columns without a row are never read: they need no mask
